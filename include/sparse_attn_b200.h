@@ -320,6 +320,126 @@ typedef struct sa_topk_args {
 SA_API int sa_topk_softmax_pv(const sa_topk_args* args, sa_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Paged key/value cache. No counterpart in the reference, whose cache is one
+ * dense tensor of equal lengths (modeling_sparse_qwen3.py:222-231).
+ *
+ * A packed batch holds the new tokens of B sequences one after the other:
+ * sequence b owns rows [cu_q[b], cu_q[b+1]) (none is allowed) of the N rows;
+ * rows from cu_q[B] on belong to nobody and are neither read nor written.
+ * seq_lens[b] counts all keys of the sequence with the new ones, so its row i
+ * stands at position seq_lens[b] - n_b + i. Position p of sequence b lives in
+ * page table[b * table_stride + p / page_size], slot p % page_size, of pools
+ * [num_pages, Hkv, page_size, D] given by their strides. cu_q, seq_lens and the
+ * table are read on the device, so that a captured launch serves every step.
+ * What they must keep (0 <= cu_q[b] <= cu_q[b+1] <= N, n_b <= seq_lens[b] <=
+ * max_pages * page_size, page numbers in [0, num_pages)) is checked there: a
+ * violation sets SA_DEV_ERR_INDEX in the device error word and the sequence, or
+ * the page's keys, are left out.
+ * page_size: 16, 32, 64 or 128. D: 64 or 128. dtype: SA_BF16 or SA_FP16, one
+ * for every 16-bit tensor of a call.
+ * ------------------------------------------------------------------------- */
+enum { SA_BF16 = 0, SA_FP16 = 1 };
+
+typedef struct sa_paged_batch {
+  const int32_t* table;
+  const int32_t* cu_q;     /* [B + 1] */
+  const int32_t* seq_lens; /* [B] */
+  int64_t table_stride;
+  int32_t B, N, max_pages, num_pages, page_size;
+} sa_paged_batch;
+
+/* q/k RMSNorm (weights [D]; NULL leaves the norm out), rotate-half RoPE from the
+ * cos/sin tables [positions, D] and the append of k and v, from the fused
+ * projection output qkv [N, Hq + 2 Hkv, D] (token stride qkv_st; heads
+ * contiguous), as sa_qk_norm_rope_append does it for a dense cache:
+ *   q_out[t, h] = RoPE(RMSNorm(q)); k -> k_pages; v -> v_pages.
+ * bounds [num_pages, Hkv, 2, D] (strides page, head, low/high; may be NULL):
+ * lowest and highest value per channel over the keys that a page holds, as
+ * stored; a page's first key starts them anew. fp32 arithmetic, one rounding
+ * per stored value. A position >= positions or a bad page sets
+ * SA_DEV_ERR_INDEX and that token (that page's k and v) is left out. */
+typedef struct sa_paged_append_args {
+  sa_paged_batch batch;
+  const void* qkv;
+  int64_t qkv_st;
+  const void* q_weight;
+  const void* k_weight;
+  const void* cos;
+  const void* sin;
+  void* q_out;
+  int64_t q_strides[2]; /* token, head */
+  void* k_pages;
+  int64_t k_strides[3]; /* page, head, slot */
+  void* v_pages;
+  int64_t v_strides[3];
+  void* bounds;
+  int64_t b_strides[3]; /* page, head, low/high */
+  int32_t Hq, Hkv, D, positions, dtype;
+  float eps;
+} sa_paged_append_args;
+
+SA_API int sa_paged_append(const sa_paged_append_args* args, sa_stream_t stream);
+
+/* Causal attention of the packed new tokens over the pages:
+ *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j,  j <= position of t,
+ * kv head h / (Hq / Hkv). With blocks [N, Hkv, n_blocks] (logical page indexes,
+ * strictly ascending, -1 behind the last) token t of a kv head sees only the
+ * listed pages; an index that does not ascend or lies behind the token sets
+ * SA_DEV_ERR_INDEX and is left out. A row that sees no key is 0. Slots past a
+ * sequence's length are never used, whatever they hold.
+ * max_q (most new tokens of one sequence) and max_len (most keys) only steer the
+ * choice of kernel and the split of long sequences: any value >= 1 is correct
+ * for max_q; max_len must not be exceeded (SA_DEV_ERR_INDEX, keys cut).
+ * workspace: sa_paged_attn_workspace(args) floats of device memory, used by this
+ * call alone while it runs; 0 floats = may be NULL. */
+typedef struct sa_paged_attn_args {
+  sa_paged_batch batch;
+  const void* q;
+  void* out;
+  int64_t q_strides[2]; /* token, head */
+  int64_t o_strides[2];
+  const void* k_pages;
+  int64_t k_strides[3]; /* page, head, slot */
+  const void* v_pages;
+  int64_t v_strides[3];
+  const int32_t* blocks; /* or NULL */
+  int64_t blocks_strides[2]; /* token, kv head */
+  int32_t n_blocks;
+  int32_t Hq, Hkv, D, dtype;
+  float scale;
+  int32_t max_q, max_len;
+  int32_t split_len; /* keys per split (rounded up to 64); 0 = by the batch's size */
+  int32_t num_sms;   /* 0 = all */
+  float* workspace;
+} sa_paged_attn_args;
+
+SA_API int sa_paged_attn_workspace(const sa_paged_attn_args* args, int64_t* floats);
+SA_API int sa_paged_attn(const sa_paged_attn_args* args, sa_stream_t stream);
+
+/* The pages each new token keeps, per kv head: of the pages up to its own, the
+ * first `first`, the last `recent` (>= 1) and the best others by
+ *   s = sum_{g in the kv head's group} sum_d max(q_gd * low_d, q_gd * high_d),
+ * low/high the page's bounds: s bounds the group's summed scores q_g . k from
+ * above for every key of the page. Equal scores go to the lower index, NaN counts
+ * as -infinity. Order is that of the scores in 64 bits.
+ * out [N, Hkv, keep] (strides token, head): ascending logical page indexes, -1
+ * behind the last. first + recent <= keep <= 4096, max_pages <= 16384. */
+typedef struct sa_paged_select_args {
+  sa_paged_batch batch;
+  const void* q;
+  int64_t q_strides[2];
+  const void* bounds;
+  int64_t b_strides[3]; /* page, head, low/high */
+  int32_t* out;
+  int64_t out_strides[2];
+  int32_t Hq, Hkv, D, dtype;
+  int32_t keep, first, recent;
+  int32_t max_q;
+} sa_paged_select_args;
+
+SA_API int sa_paged_select(const sa_paged_select_args* args, sa_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Tensor-parallel all-reduce over NVLink peer memory, fused with the residual
  * add and the next RMSNorm (no counterpart in the reference, which runs on one
  * device; it replaces the NCCL all-reduce after o_proj / down_proj for small,

@@ -35,6 +35,10 @@ EXPORTED = (
     "sa_silu_mul",
     "sa_linear_m8",
     "sa_topk_softmax_pv",
+    "sa_paged_append",
+    "sa_paged_attn_workspace",
+    "sa_paged_attn",
+    "sa_paged_select",
     "sa_ar_alloc",
     "sa_ar_free",
     "sa_ar_ipc_handle",
@@ -51,6 +55,8 @@ SA_ERR_TIMEOUT = -4
 SA_ERR_CSR = -5
 SA_BIGBIRD = 0
 SA_BIGBIRD2 = 1
+SA_BF16 = 0
+SA_FP16 = 1
 
 _c_i32 = ctypes.c_int32
 _c_i64 = ctypes.c_int64
@@ -97,6 +103,35 @@ class TopkArgs(ctypes.Structure):
                 ("top_k", _c_i32)]
 
 
+class PagedBatch(ctypes.Structure):
+    _fields_ = [("table", _c_p), ("cu_q", _c_p), ("seq_lens", _c_p), ("table_stride", _c_i64),
+                ("B", _c_i32), ("N", _c_i32), ("max_pages", _c_i32), ("num_pages", _c_i32), ("page_size", _c_i32)]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [("batch", PagedBatch), ("qkv", _c_p), ("qkv_st", _c_i64), ("q_weight", _c_p), ("k_weight", _c_p),
+                ("cos", _c_p), ("sin", _c_p), ("q_out", _c_p), ("q_strides", _c_i64 * 2), ("k_pages", _c_p),
+                ("k_strides", _c_i64 * 3), ("v_pages", _c_p), ("v_strides", _c_i64 * 3), ("bounds", _c_p),
+                ("b_strides", _c_i64 * 3), ("Hq", _c_i32), ("Hkv", _c_i32), ("D", _c_i32), ("positions", _c_i32),
+                ("dtype", _c_i32), ("eps", ctypes.c_float)]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = [("batch", PagedBatch), ("q", _c_p), ("out", _c_p), ("q_strides", _c_i64 * 2),
+                ("o_strides", _c_i64 * 2), ("k_pages", _c_p), ("k_strides", _c_i64 * 3), ("v_pages", _c_p),
+                ("v_strides", _c_i64 * 3), ("blocks", _c_p), ("blocks_strides", _c_i64 * 2), ("n_blocks", _c_i32),
+                ("Hq", _c_i32), ("Hkv", _c_i32), ("D", _c_i32), ("dtype", _c_i32), ("scale", ctypes.c_float),
+                ("max_q", _c_i32), ("max_len", _c_i32), ("split_len", _c_i32), ("num_sms", _c_i32),
+                ("workspace", _c_p)]
+
+
+class PagedSelectArgs(ctypes.Structure):
+    _fields_ = [("batch", PagedBatch), ("q", _c_p), ("q_strides", _c_i64 * 2), ("bounds", _c_p),
+                ("b_strides", _c_i64 * 3), ("out", _c_p), ("out_strides", _c_i64 * 2), ("Hq", _c_i32),
+                ("Hkv", _c_i32), ("D", _c_i32), ("dtype", _c_i32), ("keep", _c_i32), ("first", _c_i32),
+                ("recent", _c_i32), ("max_q", _c_i32)]
+
+
 class ArPeers(ctypes.Structure):
     _fields_ = [("rank", _c_i32), ("world", _c_i32), ("data", _c_p * 8), ("flags", _c_p * 8), ("epoch", _c_p),
                 ("max_ctas", _c_i32)]
@@ -140,6 +175,10 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     lib.sa_silu_mul.argtypes = [_c_p, _c_p, _c_i64, _c_i32, _c_i64, _c_i64, _c_p]
     lib.sa_linear_m8.argtypes = [_c_p, _c_i32, _c_i32, _c_i64, _c_p, _c_i32, _c_i64, _c_p, _c_i64, _c_i32, _c_p]
     lib.sa_topk_softmax_pv.argtypes = [ctypes.POINTER(TopkArgs), _c_p]
+    lib.sa_paged_append.argtypes = [ctypes.POINTER(PagedAppendArgs), _c_p]
+    lib.sa_paged_attn_workspace.argtypes = [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(_c_i64)]
+    lib.sa_paged_attn.argtypes = [ctypes.POINTER(PagedAttnArgs), _c_p]
+    lib.sa_paged_select.argtypes = [ctypes.POINTER(PagedSelectArgs), _c_p]
     lib.sa_ar_alloc.argtypes = [ctypes.c_size_t, ctypes.POINTER(_c_p)]
     lib.sa_ar_free.argtypes = [_c_p]
     lib.sa_ar_ipc_handle.argtypes = [_c_p, _c_p]

@@ -1,0 +1,126 @@
+// sa_paged.cuh — what the paged-cache kernels share: the packed batch over a
+// page pool, and the map from work units to sequences.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "sa_common.cuh"
+
+namespace sa {
+
+// Last sequence whose entry of the non-decreasing map start(b) is <= u, among
+// [0, B); start(0) <= u. The whole warp searches: 32 probes a step, so that a
+// batch of up to 33 sequences costs one load latency and 1,000 cost two.
+template <typename F>
+__device__ __forceinline__ int last_start(int B, int64_t u, F start) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int step = (hi - lo + 31) >> 5;
+    const int64_t at = lo + (int64_t)(lane + 1) * step;
+    const bool ok = at <= hi && start((int)at) <= u;
+    const unsigned m = __ballot_sync(0xffffffffu, ok);
+    const int c = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+    lo += c * step;
+    hi = min(hi, lo + step - 1);
+  }
+  return lo;
+}
+
+// Tokens of one work unit: tokens [t0, t0 + n) of the packed batch, all of
+// sequence b; the first is at position pos0.
+struct UnitTokens {
+  int b, t0, n, pos0, len;
+};
+
+// Unit u of the batch cut into tiles of tq tokens. The tiles of sequence b take
+// the unit numbers from cu_q[b] / tq + b on: floor(c / tq) + b grows by at least
+// ceil(n / tq) from one sequence to the next, so no sum over sequences is
+// needed; the numbers in between are empty units. With tq == 1 units are tokens.
+// All lanes of a warp call it with the same u.
+// Sequences whose offsets decrease or leave [0, N], or that hold fewer keys than
+// new tokens, are dropped (with SA_DEV_ERR_INDEX); a length beyond the table is cut.
+__device__ __forceinline__ bool unit_tokens(const sa_paged_batch& bt, int64_t u, int tq, int32_t* err,
+                                            UnitTokens& r) {
+  const int32_t* cu = bt.cu_q;
+  if (tq == 1) {
+    if (u >= __ldg(cu + bt.B)) return false;  // rows behind the last sequence
+    r.b = last_start(bt.B, u, [&](int b) { return (int64_t)__ldg(cu + b); });
+  } else {
+    r.b = last_start(bt.B, u, [&](int b) { return (int64_t)__ldg(cu + b) / tq + b; });
+  }
+  const int c0 = __ldg(cu + r.b), c1 = __ldg(cu + r.b + 1);
+  const int64_t first = tq == 1 ? u : c0 + (u - (c0 / tq + r.b)) * (int64_t)tq;
+  if (first < c0 || first >= c1) return false;
+  const int cap = (int)min((int64_t)bt.max_pages * bt.page_size, (int64_t)0x7fffffff);
+  const int full = __ldg(bt.seq_lens + r.b);
+  if (c0 < 0 || c1 > bt.N || full < c1 - c0 || full > cap) {
+    record_error(err, SA_DEV_ERR_INDEX);
+    if (c0 < 0 || c1 > bt.N || full < c1 - c0) return false;
+  }
+  r.t0 = (int)first;
+  r.n = (int)min((int64_t)tq, (int64_t)c1 - first);
+  r.pos0 = full - (c1 - (int)first);
+  r.len = min(full, cap);
+  return true;
+}
+
+// Units that cover any batch of N tokens in B sequences.
+inline int64_t unit_count(int64_t N, int64_t B, int tq) { return tq == 1 ? N : N / tq + B; }
+
+// 16-bit element types of the cache.
+template <typename T>
+struct Half;
+template <>
+struct Half<__nv_bfloat16> {
+  __device__ static __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
+  __device__ static __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
+  __device__ static __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
+  __device__ static __forceinline__ float2 unpack(uint32_t v) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+  }
+  __device__ static __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    mma_bf16(d, a0, a1, a2, a3, b0, b1);
+  }
+};
+template <>
+struct Half<__half> {
+  __device__ static __forceinline__ float to(__half x) { return __half2float(x); }
+  __device__ static __forceinline__ __half from(float x) { return __float2half_rn(x); }
+  __device__ static __forceinline__ uint32_t pack(float lo, float hi) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  __device__ static __forceinline__ float2 unpack(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  }
+  __device__ static __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+// Orders NaN into the result, as elementwise minimum and maximum do.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+}  // namespace sa
+
+// Host checks of a packed batch (sa_paged_append.cu).
+int sa_check_paged_batch(const sa_paged_batch* b, const char* what);
+// Pages of 16-bit elements: 16-byte aligned base, strides (page, head, slot) that are multiples of 8
+// elements, below 2^36 elements, and at least D.
+int sa_check_pages(const void* base, const int64_t strides[3], int D, const char* name);

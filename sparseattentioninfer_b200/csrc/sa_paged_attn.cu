@@ -1,0 +1,570 @@
+// sa_paged_attn.cu — causal attention of a packed batch's new tokens over a
+// paged cache, for few query rows: single tokens, drafts, and every token's own
+// kept pages.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(x_j - m),  x = scale log2(e) q . k
+//
+// in one pass with a running maximum m (rescaling o and the sum when it grows).
+// One CTA serves up to 16 query rows of one kv head (the group's heads times
+// consecutive tokens; with kept pages, one token's heads) over one split of the
+// keys, so a key is read once for all of them. A producer warp streams stages of
+// 64 keys through a ring of TMA loads, page by page (a box is one page's rows of
+// one head, at most 64, SWIZZLE_128B); four consumer warps take 16 keys each and
+// run both products with mma.sync m16n8k16 (fp32 accumulation): with 16 rows at
+// most the cache read bounds the kernel, not the products. Slots past the last
+// visible key hold anything: their scores are masked and their V rows set to
+// zero in shared memory before the product (0 * NaN is NaN).
+// Splits are split_len keys long whatever the sequence's length, so that a
+// ragged batch still makes equal CTAs; a second kernel joins them.
+#include <cstring>
+
+#include "sa_paged.cuh"
+
+namespace sa {
+
+constexpr int kRowConsumers = 4;
+constexpr int kRowThreads = 32 * (kRowConsumers + 1);
+constexpr int kRowStages = 3;
+constexpr int kRowKeys = 64;  // keys per stage
+constexpr int kRowMax = 16;   // query rows per CTA
+
+struct PagedRowParams {
+  CUtensorMap tm_k;
+  CUtensorMap tm_v;
+  sa_paged_attn_args a;
+  int32_t tq;       // tokens per unit
+  int32_t gh;       // heads per unit: min(group, 16)
+  int32_t nhg;      // units per kv head: ceil(group / 16)
+  int32_t n_split;  // grid splits: ceil(max_len / split_len)
+  float scale_log2;
+  float* part_o;    // [N, Hq, n_split, D]
+  float* part_ml;   // [N, Hq, n_split, 2]
+  int32_t* err;
+};
+
+// Keys that the unit's last token may see.
+__device__ __forceinline__ int unit_keys(const UnitTokens& ut, int max_len) {
+  return max(0, min(min(ut.pos0 + ut.n, ut.len), max_len));
+}
+__device__ __forceinline__ int unit_splits(int keys, int split_len) { return max(1, (keys + split_len - 1) / split_len); }
+
+template <int D>
+struct PagedRowCfg {
+  static constexpr int kRegions = D / 64;
+  static constexpr int kHalfBytes = kRowKeys * D * 2;
+  static constexpr int kStageBytes = 2 * kHalfBytes;
+  static constexpr int kSmemBytes = kRowStages * kStageBytes;
+  static_assert(kRowConsumers * kRowMax * D * 4 <= kSmemBytes, "ring too small for the partial outputs");
+};
+
+// ROWS 8: at most 8 query rows, half of the products' rows are padding that
+// costs nothing but tensor rate; ROWS 16 holds twice the accumulators.
+template <typename T, int D, bool SPARSE, int ROWS>
+__global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_constant__ PagedRowParams p) {
+  using Cfg = PagedRowCfg<D>;
+  constexpr int R = Cfg::kRegions;
+  constexpr int NT = D / 8;
+  constexpr int HR = ROWS / 8;  // rows per thread
+  __shared__ __align__(8) uint64_t bar_full[kRowStages], bar_empty[kRowStages];
+  __shared__ int s_key0[kRowStages][4];  // first key of each 16-key group, -1: none
+  __shared__ float s_m[kRowConsumers][ROWS], s_l[kRowConsumers][ROWS];
+  __shared__ int abort_flag;
+  extern __shared__ __align__(1024) uint8_t dsmem[];
+  const uint32_t sbase = smem_u32(dsmem);
+  float(*s_o)[ROWS][D] = reinterpret_cast<float(*)[ROWS][D]>(dsmem);
+  const sa_paged_attn_args& a = p.a;
+  const sa_paged_batch& bt = a.batch;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = blockIdx.x % p.n_split;
+  const int kvh = blockIdx.y / p.nhg, hg = blockIdx.y % p.nhg;
+  const int group = a.Hq / a.Hkv;
+  const int h0 = kvh * group + hg * kRowMax;      // first query head
+  const int nh = min(p.gh, group - hg * kRowMax);  // heads of this unit
+  const int ps = bt.page_size;
+
+  UnitTokens ut;
+  if (!unit_tokens(bt, blockIdx.x / p.n_split, p.tq, p.err, ut)) return;
+  const int keys = unit_keys(ut, a.max_len);
+  if (keys < min(ut.pos0 + ut.n, ut.len) && lane == 0) record_error(p.err, SA_DEV_ERR_INDEX);
+  const int rows = ut.n * nh;
+  // Stages [st0, st1) of this split: 64 keys each, or with kept pages the list's
+  // entries (64 / ps of them, or a part of one).
+  const int pps = ps < kRowKeys ? kRowKeys / ps : 1;  // pages per stage
+  const int spp = ps > kRowKeys ? ps / kRowKeys : 1;  // stages per page
+  const int box = min(ps, kRowKeys);
+  const int32_t* list = nullptr;
+  int st0, st1, n_used, n_list = 0x7fffffff;  // entries of the list
+  if constexpr (SPARSE) {
+    list = a.blocks + (int64_t)ut.t0 * a.blocks_strides[0] + (int64_t)kvh * a.blocks_strides[1];
+    const int per = max(1, a.split_len / kRowKeys);
+    int cnt = 0;
+    for (int i = lane; i - lane < a.n_blocks; i += 32) {
+      const unsigned m = __ballot_sync(0xffffffffu, i < a.n_blocks && __ldg(list + i) >= 0);
+      cnt += m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+      if (m != 0xffffffffu) break;
+    }
+    n_list = cnt;
+    const int nst = (cnt + pps - 1) / pps * spp;
+    n_used = max(1, (nst + per - 1) / per);
+    st0 = split * per;
+    st1 = min(nst, st0 + per);
+    n_used = min(n_used, p.n_split);
+    if (split == p.n_split - 1) st1 = nst;
+    if (split >= n_used) {
+      // The join reads every split of the row: this one has nothing.
+      if (p.n_split > 1)
+        for (int r = tid; r < rows; r += kRowThreads) {
+          const int64_t at = ((int64_t)(ut.t0 + r / nh) * a.Hq + h0 + r % nh) * p.n_split + split;
+          p.part_ml[at * 2] = -INFINITY;
+          p.part_ml[at * 2 + 1] = 0.f;
+        }
+      return;
+    }
+  } else {
+    n_used = unit_splits(keys, a.split_len);
+    if (split >= n_used) return;
+    st0 = split * (a.split_len / kRowKeys);
+    st1 = min((keys + kRowKeys - 1) / kRowKeys, st0 + a.split_len / kRowKeys);
+  }
+  const int nst = max(0, st1 - st0);
+
+  if (tid == 0) {
+    if (sbase & 1023u) record_error(p.err, SA_DEV_ERR_INDEX);
+    for (int i = 0; i < kRowStages; ++i) {
+      mbar_init(smem_u32(&bar_full[i]), 1);
+      mbar_init(smem_u32(&bar_empty[i]), kRowConsumers);
+    }
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (sbase & 1023u) return;  // block-uniform
+  __syncthreads();
+  volatile int* abort_v = &abort_flag;
+
+  float m_run[HR], l_run[HR], o_acc[NT][2 * HR];
+#pragma unroll
+  for (int r = 0; r < HR; ++r) {
+    m_run[r] = -INFINITY;
+    l_run[r] = 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 2 * HR; ++e) o_acc[j][e] = 0.f;
+  const int row = lane >> 2;
+
+  if (warp == kRowConsumers) {
+    // ------------------------------------------------------------ producer
+    // Lane j < pps loads page j of the stage; the page numbers of the next 32
+    // pages are read ahead, one a lane.
+    const int32_t* trow = bt.table + (int64_t)ut.b * bt.table_stride;
+    const int e0 = st0 / spp * pps;                        // first entry of the split
+    const int ne = min((st1 + spp - 1) / spp * pps, n_list) - e0;  // entries of the split
+    int blk = -1, page = -1, bad = 0;
+    auto fetch = [&](int i) {  // entry e0 + i: logical block and page, -1: none
+      blk = -1;
+      page = -1;
+      if (i < ne) {
+        if constexpr (SPARSE) {
+          const int e = e0 + i;
+          blk = __ldg(list + e);
+          if (blk <= (e > 0 ? __ldg(list + e - 1) : -1) || (int64_t)blk * ps >= keys) {
+            bad = 1;
+            blk = -1;
+          }
+        } else {
+          blk = e0 + i;
+          if ((int64_t)blk * ps >= keys) blk = -1;
+        }
+        if (blk >= 0) {
+          page = __ldg(trow + blk);
+          if (page < 0 || page >= bt.num_pages) {
+            bad = 1;
+            page = -1;
+          }
+        }
+      }
+    };
+    bool ok = true;
+    int base = -32;
+    for (int i = 0; i < nst; ++i) {
+      const int slot = i % kRowStages;
+      const int first = (st0 + i) / spp * pps - e0;  // entry of the stage's first page
+      if (first >= base + 32) {
+        base = first;
+        fetch(base + lane);
+      }
+      const int src = (first - base + (lane < pps ? lane : 0)) & 31;
+      const int pg = __shfl_sync(0xffffffffu, page, src);
+      const int bk = __shfl_sync(0xffffffffu, blk, src);
+      const int off = spp > 1 ? ((st0 + i) % spp) * kRowKeys : 0;
+      const bool mine = lane < pps && pg >= 0 && (int64_t)bk * ps + off < keys;
+      const int n = __popc(__ballot_sync(0xffffffffu, mine));
+      if (i >= kRowStages) {
+        ok = mbar_wait(smem_u32(&bar_empty[slot]), ((i / kRowStages) - 1) & 1, abort_v, p.err);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          // stages from i on were not loaded
+          st1 = st0 + i;
+          break;
+        }
+      }
+      if (lane < pps)
+        for (int g = 0; g < box / 16; ++g) s_key0[slot][lane * (box / 16) + g] = mine ? bk * ps + off + 16 * g : -1;
+      __syncwarp();
+      const uint32_t bar = smem_u32(&bar_full[slot]);
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)n * box * D * 4);
+      __syncwarp();
+      if (mine) {
+        const uint32_t dst = sbase + slot * Cfg::kStageBytes + lane * box * 128;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          tma_load_4d(dst + r * kRowKeys * 128, &p.tm_k, bar, r * 64, off, kvh, pg);
+          tma_load_4d(dst + Cfg::kHalfBytes + r * kRowKeys * 128, &p.tm_v, bar, r * 64, off, kvh, pg);
+        }
+      }
+    }
+    if (__any_sync(0xffffffffu, bad) && lane == 0) record_error(p.err, SA_DEV_ERR_INDEX);
+    int zero = 0;  // drain (bounded) copies still in flight
+    const int done = max(0, st1 - st0);
+    for (int i = max(0, done - kRowStages); i < done; ++i)
+      mbar_wait(smem_u32(&bar_full[i % kRowStages]), (i / kRowStages) & 1, &zero, nullptr);
+  } else {
+    // ------------------------------------------------------------ consumers
+    uint32_t qa[D / 16][2 * HR];
+    int pos[HR];
+#pragma unroll
+    for (int r = 0; r < HR; ++r) {
+      const int rr = row + 8 * r;
+      const bool live = rr < rows;
+      const int tok = live ? rr / nh : 0, h = live ? rr % nh : 0;
+      pos[r] = live ? min(ut.pos0 + tok, keys - 1) : -1;
+      const T* qrow = reinterpret_cast<const T*>(a.q) + (int64_t)(ut.t0 + tok) * a.q_strides[0] +
+                      (int64_t)(h0 + h) * a.q_strides[1];
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const int d = kk * 16 + 2 * (lane & 3);
+        qa[kk][2 * r] = live ? *reinterpret_cast<const uint32_t*>(qrow + d) : 0u;
+        qa[kk][2 * r + 1] = live ? *reinterpret_cast<const uint32_t*>(qrow + d + 8) : 0u;
+      }
+    }
+    const int k_lo = warp * 16;
+    for (int i = 0; i < nst; ++i) {
+      const int slot = i % kRowStages;
+      const bool ok = mbar_wait(smem_u32(&bar_full[slot]), (i / kRowStages) & 1, abort_v, p.err);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const int key0 = s_key0[slot][warp];
+      if (key0 >= 0 && key0 < keys) {
+        const uint32_t sk = sbase + slot * Cfg::kStageBytes;
+        const uint32_t sv = sk + Cfg::kHalfBytes;
+        if (key0 + 16 > keys) {
+          // V rows past the last key: zero, whatever the page holds there.
+          const int first = keys - key0;
+          for (int r = first + (lane >> 3); r < 16; r += 4)
+#pragma unroll
+            for (int reg = 0; reg < R; ++reg)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + reg * kRowKeys * 128 +
+                                                                           (k_lo + r) * 128 + (lane & 7) * 16),
+                           "r"(0u)
+                           : "memory");
+          // (the next TMA load into this slot is ordered behind these stores)
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+        const int kr = k_lo + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const int ch = ((kk & 3) << 1) + ((lane >> 3) & 1);
+          uint32_t b0, b1, b2, b3;
+          ldsm_x4(sw128(sk + (kk >> 2) * kRowKeys * 128, kr, ch), b0, b1, b2, b3);
+          const uint32_t a1 = HR == 2 ? qa[kk][2 * (HR - 1)] : 0u, a3 = HR == 2 ? qa[kk][2 * (HR - 1) + 1] : 0u;
+          Half<T>::mma(s0, qa[kk][0], a1, qa[kk][1], a3, b0, b1);
+          Half<T>::mma(s1, qa[kk][0], a1, qa[kk][1], a3, b2, b3);
+        }
+        // This thread's keys of a row: c0, c0 + 1, c0 + 8, c0 + 9.
+        const int c0 = key0 + 2 * (lane & 3);
+        uint32_t pa[2 * HR];
+        float alpha[HR];
+#pragma unroll
+        for (int r = 0; r < HR; ++r) {
+          float x[4];
+          x[0] = c0 <= pos[r] ? s0[2 * r] * p.scale_log2 : -INFINITY;
+          x[1] = c0 + 1 <= pos[r] ? s0[2 * r + 1] * p.scale_log2 : -INFINITY;
+          x[2] = c0 + 8 <= pos[r] ? s1[2 * r] * p.scale_log2 : -INFINITY;
+          x[3] = c0 + 9 <= pos[r] ? s1[2 * r + 1] * p.scale_log2 : -INFINITY;
+          float mb = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+          mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
+          const float m_new = fmaxf(m_run[r], mb);
+          const float mu = m_new == -INFINITY ? 0.f : m_new;
+          alpha[r] = ex2(m_run[r] - mu);
+          m_run[r] = m_new;
+          // P is rounded to the cache's type for the product; the sum takes the
+          // rounded values, so that a row ruled by few keys loses nothing by it.
+          pa[2 * r] = Half<T>::pack(ex2(x[0] - mu), ex2(x[1] - mu));
+          pa[2 * r + 1] = Half<T>::pack(ex2(x[2] - mu), ex2(x[3] - mu));
+          const float2 u = Half<T>::unpack(pa[2 * r]), v = Half<T>::unpack(pa[2 * r + 1]);
+          l_run[r] = l_run[r] * alpha[r] + (u.x + u.y) + (v.x + v.y);
+        }
+        const int vr = k_lo + (lane & 7) + (((lane >> 3) & 1) << 3);
+#pragma unroll
+        for (int j = 0; j < NT; j += 2) {
+          const int dch = j + (lane >> 4);
+          uint32_t v0, v1, v2, v3;
+          ldsm_x4_t(sw128(sv + (dch >> 3) * kRowKeys * 128, vr, dch & 7), v0, v1, v2, v3);
+          float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < 2 * HR; ++e) {
+            d0[e] = o_acc[j][e] * alpha[e >> 1];
+            d1[e] = o_acc[j + 1][e] * alpha[e >> 1];
+          }
+          const uint32_t a1 = HR == 2 ? pa[2 * (HR - 1)] : 0u, a3 = HR == 2 ? pa[2 * (HR - 1) + 1] : 0u;
+          Half<T>::mma(d0, pa[0], a1, pa[1], a3, v0, v1);
+          Half<T>::mma(d1, pa[0], a1, pa[1], a3, v2, v3);
+#pragma unroll
+          for (int e = 0; e < 2 * HR; ++e) {
+            o_acc[j][e] = d0[e];
+            o_acc[j + 1][e] = d1[e];
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_empty[slot]));
+    }
+  }
+  __syncthreads();  // ring idle (producer drained): reuse it for the warps' partial outputs
+  if (warp < kRowConsumers) {
+#pragma unroll
+    for (int r = 0; r < HR; ++r) {
+      float l = l_run[r];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if ((lane & 3) == 0) {
+        s_m[warp][row + 8 * r] = m_run[r];
+        s_l[warp][row + 8 * r] = l;
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        *reinterpret_cast<float2*>(&s_o[warp][row + 8 * r][j * 8 + 2 * (lane & 3)]) =
+            make_float2(o_acc[j][2 * r], o_acc[j][2 * r + 1]);
+    }
+  }
+  __syncthreads();
+  for (int idx = tid; idx < rows * (D / 2); idx += kRowThreads) {
+    const int r = idx / (D / 2), d = idx % (D / 2) * 2;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kRowConsumers; ++w) mx = fmaxf(mx, s_m[w][r]);
+    const float mu = mx == -INFINITY ? 0.f : mx;
+    float lsum = 0.f, acc0 = 0.f, acc1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowConsumers; ++w) {
+      const float c = ex2(s_m[w][r] - mu);
+      const float2 o = *reinterpret_cast<const float2*>(&s_o[w][r][d]);
+      lsum += s_l[w][r] * c;
+      acc0 += o.x * c;
+      acc1 += o.y * c;
+    }
+    const int tok = ut.t0 + r / nh, h = h0 + r % nh;
+    if (p.n_split == 1) {
+      const float inv = lsum > 0.f ? 1.0f / lsum : (lsum == 0.f ? 0.f : lsum);
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.o_strides[0] +
+                                   (int64_t)h * a.o_strides[1] + d) = Half<T>::pack(acc0 * inv, acc1 * inv);
+    } else {
+      const int64_t at = ((int64_t)tok * a.Hq + h) * p.n_split + split;
+      *reinterpret_cast<float2*>(p.part_o + at * D + d) = make_float2(acc0, acc1);
+      if (d == 0) {
+        p.part_ml[at * 2] = mx;
+        p.part_ml[at * 2 + 1] = lsum;
+      }
+    }
+  }
+}
+
+// Joins the splits of one (token, head) per warp.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedRowParams p, bool sparse) {
+  constexpr int E = D / 32;
+  const sa_paged_attn_args& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int h = (int)(w % a.Hq);
+  const int64_t t = w / a.Hq;
+  if (t >= a.batch.N) return;
+  UnitTokens ut;
+  if (!unit_tokens(a.batch, t, 1, nullptr, ut)) return;
+  int n = p.n_split;
+  if (!sparse) {
+    // The splits that the token's unit ran: as far as its last token sees.
+    const int c0 = __ldg(a.batch.cu_q + ut.b), c1 = __ldg(a.batch.cu_q + ut.b + 1);
+    const int in = (ut.t0 - c0) % p.tq;
+    const int lead = min(p.tq - in, c1 - ut.t0);  // this token and those behind it in the unit
+    ut.n = lead;
+    n = min(n, unit_splits(unit_keys(ut, a.max_len), a.split_len));
+  }
+  const int64_t at = ((int64_t)t * a.Hq + h) * p.n_split;
+  const float* ml = p.part_ml + at * 2;
+  float mx = -INFINITY;
+  for (int s = lane; s < n; s += 32) mx = fmaxf(mx, ml[2 * s]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float mu = mx == -INFINITY ? 0.f : mx;
+  float lsum = 0.f, acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int s = 0; s < n; ++s) {
+    const float m = ml[2 * s], l = ml[2 * s + 1];
+    if (m == -INFINITY && l == 0.f) continue;  // a split without keys wrote no output
+    const float c = ex2(m - mu);
+    lsum += l * c;
+    const float* o = p.part_o + (at + s) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] += o[e] * c;
+  }
+  const float inv = lsum > 0.f ? 1.0f / lsum : (lsum == 0.f ? 0.f : lsum);
+  T* dst = reinterpret_cast<T*>(a.out) + t * a.o_strides[0] + (int64_t)h * a.o_strides[1] + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2)
+    *reinterpret_cast<uint32_t*>(dst + e) = Half<T>::pack(acc[e] * inv, acc[e + 1] * inv);
+}
+
+// Shape of the launch: tokens per unit, splits, workspace.
+struct RowPlan {
+  int tq, gh, nhg, n_split, split_len;
+  int64_t units;
+};
+
+static RowPlan row_plan(const sa_paged_attn_args& a, int sms) {
+  RowPlan r;
+  const int group = a.Hq / a.Hkv;
+  r.gh = group < kRowMax ? group : kRowMax;
+  r.nhg = (group + kRowMax - 1) / kRowMax;
+  r.tq = a.blocks ? 1 : (a.max_q < kRowMax / r.gh ? a.max_q : kRowMax / r.gh);
+  if (r.tq < 1) r.tq = 1;
+  r.units = unit_count(a.batch.N, a.batch.B, r.tq);
+  // Keys of the longest unit.
+  const int64_t cap = (int64_t)a.batch.max_pages * a.batch.page_size;
+  int64_t longest = a.max_len < cap ? a.max_len : cap;
+  if (a.blocks) {
+    const int64_t kept = (int64_t)a.n_blocks * a.batch.page_size;
+    // Every entry of the list takes its share of a 64-key stage.
+    if (kept < longest || a.batch.page_size < kRowKeys) longest = kept;
+  }
+  longest = (longest + kRowKeys - 1) / kRowKeys * kRowKeys;
+  int64_t len = ((int64_t)a.split_len + kRowKeys - 1) / kRowKeys * kRowKeys;
+  if (a.split_len <= 0) {
+    // About four CTAs per resident slot (two a SM), but at least 256 keys each.
+    const int64_t lines = (a.blocks ? r.units : a.batch.N / r.tq + 1) * a.Hkv * r.nhg;
+    const int64_t want = 8ll * sms;
+    const int64_t splits = lines >= want ? 1 : (want + lines - 1) / lines;
+    len = (longest + splits - 1) / splits;
+    len = (len + kRowKeys - 1) / kRowKeys * kRowKeys;
+    if (len < 256) len = 256;
+  }
+  if (len > longest) len = longest;
+  // The join reads every split: no more than 512 of them.
+  if ((longest + len - 1) / len > 512) len = ((longest + 511) / 512 + kRowKeys - 1) / kRowKeys * kRowKeys;
+  r.split_len = (int)len;
+  r.n_split = (int)((longest + len - 1) / len);
+  return r;
+}
+
+template <typename T, int D, bool SPARSE, int ROWS>
+static int launch_rows(const PagedRowParams& prm, const RowPlan& r, cudaStream_t stream) {
+  auto kern = paged_rows_kernel<T, D, SPARSE, ROWS>;
+  SA_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedRowCfg<D>::kSmemBytes));
+  const int64_t gx = r.units * r.n_split, gy = (int64_t)prm.a.Hkv * r.nhg;
+  if (gx > 0x7fffffff || gy > 65535) return sa_fail(SA_ERR_INVALID, "paged attention: batch too large");
+  kern<<<dim3((unsigned)gx, (unsigned)gy), kRowThreads, PagedRowCfg<D>::kSmemBytes, stream>>>(prm);
+  SA_CHECK_CUDA(cudaGetLastError());
+  if (r.n_split > 1) {
+    const int64_t warps = (int64_t)prm.a.batch.N * prm.a.Hq;
+    paged_join_kernel<T, D><<<(unsigned)((warps + 3) / 4), 128, 0, stream>>>(prm, SPARSE);
+    SA_CHECK_CUDA(cudaGetLastError());
+  }
+  return SA_OK;
+}
+
+template <typename T, int D>
+static int launch_rows_any(const PagedRowParams& prm, const RowPlan& r, cudaStream_t stream) {
+  const bool few = r.tq * r.gh <= 8;
+  if (prm.a.blocks)
+    return few ? launch_rows<T, D, true, 8>(prm, r, stream) : launch_rows<T, D, true, 16>(prm, r, stream);
+  return few ? launch_rows<T, D, false, 8>(prm, r, stream) : launch_rows<T, D, false, 16>(prm, r, stream);
+}
+
+static int check_paged_attn(const sa_paged_attn_args* a) {
+  if (!a) return sa_fail(SA_ERR_INVALID, "args is NULL");
+  int rc = sa_check_paged_batch(&a->batch, "paged attention");
+  if (rc) return rc;
+  if (!a->q || !a->out) return sa_fail(SA_ERR_INVALID, "NULL tensor pointer");
+  if (a->D != 64 && a->D != 128) return sa_fail(SA_ERR_UNSUPPORTED, "head_dim %d unsupported (64 or 128)", a->D);
+  if (a->dtype != SA_BF16 && a->dtype != SA_FP16) return sa_fail(SA_ERR_UNSUPPORTED, "dtype %d unknown", a->dtype);
+  if (a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv)
+    return sa_fail(SA_ERR_INVALID, "Hq=%d not a multiple of Hkv=%d", a->Hq, a->Hkv);
+  if (a->max_q < 1 || a->max_len < 1) return sa_fail(SA_ERR_INVALID, "max_q and max_len must be at least 1");
+  if (a->split_len < 0 || a->num_sms < 0) return sa_fail(SA_ERR_INVALID, "negative split_len or num_sms");
+  if ((rc = sa_check_pages(a->k_pages, a->k_strides, a->D, "k_pages"))) return rc;
+  if ((rc = sa_check_pages(a->v_pages, a->v_strides, a->D, "v_pages"))) return rc;
+  const int64_t* st[2] = {a->q_strides, a->o_strides};
+  for (int i = 0; i < 2; ++i)
+    if (st[i][0] < 0 || st[i][1] < 0 || st[i][0] % 8 || st[i][1] % 8)
+      return sa_fail(SA_ERR_INVALID, "q/out strides must be non-negative multiples of 8 elements (16 B)");
+  if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15u)
+    return sa_fail(SA_ERR_INVALID, "q/out must be 16-byte aligned");
+  if (a->blocks) {
+    if (a->n_blocks < 1) return sa_fail(SA_ERR_INVALID, "n_blocks must be at least 1");
+    if (a->blocks_strides[0] < 0 || a->blocks_strides[1] < 0)
+      return sa_fail(SA_ERR_INVALID, "blocks strides must be non-negative");
+  }
+  return SA_OK;
+}
+
+}  // namespace sa
+
+using namespace sa;
+
+extern "C" int sa_paged_attn_workspace(const sa_paged_attn_args* a, int64_t* floats) {
+  int rc = check_paged_attn(a);
+  if (rc) return rc;
+  if (!floats) return sa_fail(SA_ERR_INVALID, "floats is NULL");
+  const int sms = a->num_sms > 0 ? a->num_sms : sa_num_sms();
+  if (sms <= 0) return sa_fail(SA_ERR_CUDA, "cannot query SM count");
+  const RowPlan r = row_plan(*a, sms);
+  *floats = r.n_split > 1 ? (int64_t)a->batch.N * a->Hq * r.n_split * (a->D + 2) : 0;
+  return SA_OK;
+}
+
+extern "C" int sa_paged_attn(const sa_paged_attn_args* a, sa_stream_t stream_) {
+  int rc = check_paged_attn(a);
+  if (rc) return rc;
+  const int sms = a->num_sms > 0 ? a->num_sms : sa_num_sms();
+  if (sms <= 0) return sa_fail(SA_ERR_CUDA, "cannot query SM count");
+  const RowPlan r = row_plan(*a, sms);
+  if (r.n_split > 1 && !a->workspace) return sa_fail(SA_ERR_INVALID, "paged attention: workspace is NULL");
+  PagedRowParams prm;
+  memset(&prm, 0, sizeof(prm));
+  const int box = a->batch.page_size < kRowKeys ? a->batch.page_size : kRowKeys;
+  if ((rc = sa_make_map(&prm.tm_k, a->k_pages, a->batch.num_pages, a->Hkv, a->batch.page_size, a->D, a->k_strides,
+                        box, "k_pages")))
+    return rc;
+  if ((rc = sa_make_map(&prm.tm_v, a->v_pages, a->batch.num_pages, a->Hkv, a->batch.page_size, a->D, a->v_strides,
+                        box, "v_pages")))
+    return rc;
+  prm.a = *a;
+  prm.a.split_len = r.split_len;
+  prm.tq = r.tq;
+  prm.gh = r.gh;
+  prm.nhg = r.nhg;
+  prm.n_split = r.n_split;
+  prm.scale_log2 = a->scale * 1.4426950408889634f;
+  prm.part_o = a->workspace;
+  prm.part_ml = a->workspace ? a->workspace + (int64_t)a->batch.N * a->Hq * r.n_split * a->D : nullptr;
+  prm.err = sa_device_error_ptr();
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream_);
+  if (a->dtype == SA_BF16)
+    return a->D == 128 ? launch_rows_any<__nv_bfloat16, 128>(prm, r, st)
+                       : launch_rows_any<__nv_bfloat16, 64>(prm, r, st);
+  return a->D == 128 ? launch_rows_any<__half, 128>(prm, r, st) : launch_rows_any<__half, 64>(prm, r, st);
+}

@@ -1,0 +1,251 @@
+"""The paged-cache operators against their definitions in 64 bits (tests/_paged.py)."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import _paged as P
+from sparseattentioninfer_b200 import _capi, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def rope_tables(n, D, dtype, theta=1e6):
+    ang = torch.outer(torch.arange(n, dtype=torch.float64), theta ** (-torch.arange(0, D, 2, dtype=torch.float64) / D))
+    ang = torch.cat([ang, ang], -1)
+    return ang.cos().to(dtype), ang.sin().to(dtype)
+
+
+# --------------------------------------------------------------------- append
+@pytest.mark.parametrize("ctx,new,Hq,Hkv,D,page,dtype,layout,pad", [
+    ([0], [1], 4, 1, 64, 16, torch.bfloat16, "heads", 0),                                  # the very first token
+    ([5, 0, 31, 16], [1, 1, 1, 1], 8, 2, 128, 16, torch.bfloat16, "heads", 3),             # decode, page starts and ends
+    ([0, 7, 100, 3], [37, 0, 65, 1], 6, 2, 128, 32, torch.float16, "slots", 0),            # ragged, one without tokens
+    ([63, 64, 1], [130, 129, 300], 20, 4, 64, 64, torch.bfloat16, "wide", 5),
+    ([200] * 40, [2] * 40, 9, 3, 128, 128, torch.float16, "heads", 1),
+    ([10], [1000], 16, 16, 64, 128, torch.bfloat16, "slots", 0),
+])
+@pytest.mark.parametrize("normed", [True, False])
+def test_append(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, normed):
+    bt = P.Batch(ctx, new, Hq=Hq, Hkv=Hkv, D=D, page=page, dtype=dtype, device=DEV, seed=len(ctx), pad=pad,
+                 layout=layout)
+    g = bt.g
+    total = Hq + 2 * Hkv
+    qkv = (3 * torch.randn(bt.N, total, D, generator=g)).to(dtype)
+    qw, kw = ((1 + 0.1 * torch.randn(D, generator=g)).to(dtype) for _ in range(2))
+    cos, sin = rope_tables(max(bt.lens), D, dtype)
+    old = P.Batch(ctx, [0] * len(ctx), Hq=Hq, Hkv=Hkv, D=D, page=page, dtype=dtype)
+    old.table, old.pages, old.g = bt.table, bt.pages, g
+    k0, v0 = old.pool(), old.pool()
+    k_pages, v_pages = bt.place(k0), bt.place(v0)
+    bounds = P.bounds_of(bt, k0, lens=ctx, fill=float("nan")).to(DEV)
+    q_out = torch.full((bt.N, Hq, D), 7.0, dtype=dtype, device=DEV)
+    # (token rows of a wider buffer)
+    wide = torch.full((bt.N, total * D + 16), float("nan"), dtype=dtype, device=DEV)
+    wide[:, 8:8 + total * D] = qkv.to(DEV).view(bt.N, -1)
+    src = wide[:, 8:8 + total * D].view(bt.N, total, D)
+    got = ops.paged_qk_norm_rope_append(
+        src, qw.to(DEV) if normed else None, kw.to(DEV) if normed else None, cos.to(DEV), sin.to(DEV), k_pages,
+        v_pages, *bt.batch, Hq=Hq, Hkv=Hkv, eps=1e-6, k_bounds=bounds, q_out=q_out)
+    assert got is q_out and _capi.device_error() == 0
+    # q and k: |y c| + |y' s| carries the 32-bit errors (sum of D squares, rsqrt: below 2^-16), one rounding on top
+    x = qkv[:, :Hq + Hkv].double()
+    if normed:
+        x = x / torch.sqrt(x.pow(2).mean(-1, keepdim=True) + 1e-6)
+        x = torch.cat([x[:, :Hq] * qw.double(), x[:, Hq:] * kw.double()], 1)
+    u = torch.finfo(dtype).eps / 2
+    rows = torch.tensor([r for r, _, _ in bt.tokens()])
+    pos = torch.tensor([p for _, _, p in bt.tokens()])
+    c, s = cos.double()[pos][:, None], sin.double()[pos][:, None]
+    x = x[rows]
+    ref = x * c + torch.cat([-x[..., D // 2:], x[..., :D // 2]], -1) * s
+    size = (x * c).abs() + (torch.cat([x[..., D // 2:], x[..., :D // 2]], -1) * s).abs()
+    tol = u * ref.abs() + 2.0 ** -16 * size + torch.finfo(dtype).tiny
+    assert ((got.cpu().double()[rows] - ref[:, :Hq]).abs() <= tol[:, :Hq]).all()
+    if pad:
+        assert (got[bt.N - pad:] == 7.0).all()
+    kp, vp = k_pages.cpu(), v_pages.cpu()
+    k0, v0 = k0.clone(), v0.clone()
+    for i, (r, b, p) in enumerate(bt.tokens()):
+        page_, slot = int(bt.table[b, p // page]), p % page
+        assert ((kp[page_, :, slot].double() - ref[i, Hq:]).abs() <= tol[i, Hq:]).all()
+        k0[page_, :, slot] = kp[page_, :, slot]
+        v0[page_, :, slot] = qkv[r, Hq + Hkv:]
+    assert torch.equal(kp.view(torch.int16), k0.view(torch.int16))  # nothing else was written
+    assert torch.equal(vp.view(torch.int16), v0.view(torch.int16))
+    want = P.bounds_of(bt, kp, fill=float("nan"))
+    assert torch.equal(bounds.cpu().nan_to_num(77.0), want.nan_to_num(77.0))
+
+
+def test_append_in_pieces_gives_the_same_cache():
+    """One call and a token at a time: the same pages and bounds, bit for bit."""
+    Hq, Hkv, D, page, n = 4, 2, 128, 16, 50
+    bt = P.Batch([3], [n], Hq=Hq, Hkv=Hkv, D=D, page=page, device=DEV)
+    qkv = torch.randn(n, Hq + 2 * Hkv, D, generator=bt.g).to(torch.bfloat16).to(DEV)
+    w = torch.ones(D, dtype=torch.bfloat16, device=DEV)
+    cos, sin = (t.to(DEV) for t in rope_tables(64, D, torch.bfloat16))
+    res = []
+    for step in (n, 1, 7):
+        k, v = (torch.zeros(bt.pages, Hkv, page, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        bounds = torch.zeros(bt.pages, Hkv, 2, D, dtype=torch.bfloat16, device=DEV)
+        table = bt.table.to(DEV)
+        qs = []
+        for i in range(0, n, step):
+            m = min(step, n - i)
+            cu, ln = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, m], [3 + i + m]))
+            qs.append(ops.paged_qk_norm_rope_append(qkv[i:i + m], w, w, cos, sin, k, v, table, cu, ln, Hq=Hq,
+                                                    Hkv=Hkv, k_bounds=bounds))
+        res.append((torch.cat(qs), k, v, bounds))
+    for other in res[1:]:
+        for a, b in zip(res[0], other):
+            assert torch.equal(a, b)
+    assert _capi.device_error() == 0
+
+
+# ------------------------------------------------------------------ attention
+ATTN = [
+    # ctx, new, Hq, Hkv, D, page, dtype, layout, pad
+    ([0], [1], 1, 1, 64, 16, torch.bfloat16, "heads", 0),
+    ([0, 1, 14, 15, 16, 63, 64, 200], [1] * 8, 8, 2, 128, 16, torch.bfloat16, "heads", 2),
+    ([700, 3, 128, 255], [1, 1, 0, 1], 12, 4, 64, 32, torch.float16, "slots", 1),
+    ([100, 0, 600, 31], [3, 5, 0, 2], 8, 2, 128, 64, torch.bfloat16, "wide", 0),
+    ([129, 1000], [1, 4], 40, 2, 128, 128, torch.float16, "heads", 0),      # 20 heads a group
+    ([65, 0], [33, 70], 6, 2, 64, 16, torch.bfloat16, "slots", 3),
+    ([0, 300, 17], [200, 129, 1], 8, 8, 128, 32, torch.bfloat16, "heads", 0),
+    ([0], [260], 10, 2, 128, 64, torch.float16, "heads", 0),                # 5 heads a group
+    ([513], [140], 16, 1, 64, 128, torch.bfloat16, "wide", 4),
+    ([0, 0, 90], [1, 257, 40], 3, 1, 128, 128, torch.float16, "heads", 0),
+]
+
+
+def _qkv(bt, std=1.5):
+    q = (std * torch.randn(bt.N, bt.Hq, bt.D, generator=bt.g)).to(bt.dtype)
+    return q, bt.pool(), bt.pool()
+
+
+def _assert_attention(bt, got, q, k, v, scale, blocks=None, before=None):
+    ref, mag = P.attention(bt, q, k, v, scale, blocks)
+    n = sum(bt.new)
+    err = (got.cpu().double()[:n] - ref[:n]).abs()
+    tol = P.attention_tolerance(ref[:n], mag[:n], bt.dtype)
+    assert (err <= tol).all(), (err / tol).max()
+    if before is not None:
+        assert torch.equal(got[n:].cpu(), before[n:].cpu())
+    assert _capi.device_error() == 0
+
+
+@pytest.mark.parametrize("ctx,new,Hq,Hkv,D,page,dtype,layout,pad", ATTN)
+@pytest.mark.parametrize("hints", ["exact", "none", "wrong", "split"])
+def test_attention(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, hints):
+    """Slots behind a sequence's length hold NaN, table entries behind it -7."""
+    bt = P.Batch(ctx, new, Hq=Hq, Hkv=Hkv, D=D, page=page, dtype=dtype, device=DEV, seed=Hq + D, pad=pad,
+                 layout=layout)
+    q, k, v = _qkv(bt)
+    kw = {"exact": dict(max_q=max(new), max_len=max(bt.lens)), "none": {}, "wrong": dict(max_q=1),
+          "split": dict(max_q=max(new), split_len=64)}[hints]
+    out = torch.full((bt.N, Hq, D), 3.0, dtype=dtype, device=DEV)
+    before = out.clone()
+    got = ops.paged_attention(q.to(DEV), k, v, *bt.batch, out=out, **kw)
+    assert got is out
+    _assert_attention(bt, got, q, k, v, 1 / math.sqrt(D), before=before)
+
+
+def _random_blocks(bt, keep, seed=0, empty=False):
+    g = torch.Generator().manual_seed(seed)
+    out = torch.full((bt.N, bt.Hkv, keep), -1, dtype=torch.int32)
+    for r, b, pos in bt.tokens():
+        for h in range(bt.Hkv):
+            last = pos // bt.page
+            n = min(keep, int(torch.randint(0 if empty else 1, last + 2, (1,), generator=g)))
+            got = torch.randperm(last + 1, generator=g)[:n].sort().values
+            out[r, h, :n] = got.int()
+    return out
+
+
+@pytest.mark.parametrize("ctx,new,Hq,Hkv,D,page,dtype,layout,pad", ATTN)
+@pytest.mark.parametrize("keep,split_len", [(1, None), (5, 64), (9, None)])
+def test_sparse_attention(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, keep, split_len):
+    bt = P.Batch(ctx, new, Hq=Hq, Hkv=Hkv, D=D, page=page, dtype=dtype, device=DEV, seed=keep, pad=pad, layout=layout)
+    q, k, v = _qkv(bt)
+    blocks = _random_blocks(bt, keep, empty=True)  # some lists are empty: those rows are 0
+    out = torch.full((bt.N, Hq, D), 3.0, dtype=dtype, device=DEV)
+    before = out.clone()
+    ops.paged_attention(q.to(DEV), k, v, *bt.batch, blocks=blocks.to(DEV), split_len=split_len, out=out)
+    _assert_attention(bt, out, q, k, v, 1 / math.sqrt(D), blocks, before)
+
+
+def test_attention_scale_and_strided_rows():
+    bt = P.Batch([40, 3], [5, 9], Hq=4, Hkv=2, D=64, page=16, device=DEV)
+    q, k, v = _qkv(bt)
+    wide = torch.full((bt.N, 9, 64 + 16), float("nan"), dtype=torch.bfloat16, device=DEV)
+    wide[:, 2:6, 8:72] = q.to(DEV)
+    res = torch.zeros(6, bt.N, 64, dtype=torch.bfloat16, device=DEV)
+    ops.paged_attention(wide[:, 2:6, 8:72], k, v, *bt.batch, scale=0.3, out=res.transpose(0, 1)[:, 1:5])
+    _assert_attention(bt, res.transpose(0, 1)[:, 1:5], q, k, v, 0.3)
+    assert (res[0] == 0).all() and (res[5] == 0).all()
+
+
+# -------------------------------------------------------------------- select
+@pytest.mark.parametrize("ctx,new,Hq,Hkv,D,page,dtype,layout,pad", ATTN + [
+    ([9000, 40, 4111], [1, 1, 3], 8, 2, 128, 16, torch.bfloat16, "heads", 0),
+])
+@pytest.mark.parametrize("keep,first,recent", [(1, 0, 1), (4, 1, 2), (8, 0, 3), (70, 2, 5)])
+def test_select(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, keep, first, recent):
+    bt = P.Batch(ctx, new, Hq=Hq, Hkv=Hkv, D=D, page=page, dtype=dtype, device=DEV, seed=3, pad=pad)
+    q = torch.randn(bt.N, Hq, D, generator=bt.g).to(dtype)
+    bounds = P.bounds_of(bt, bt.pool(), fill=float("nan"))
+    out = torch.full((bt.N, Hkv, keep), 99, dtype=torch.int32, device=DEV)
+    ops.paged_block_select(q.to(DEV), bounds.to(DEV), *bt.batch, page_size=page, keep=keep, first=first,
+                           recent=recent, max_q=max(new), out=out)
+    n = sum(new)
+    assert torch.equal(out[:n].cpu(), P.select(bt, q, bounds, keep, first, recent)[:n])
+    assert (out[n:] == 99).all()
+    assert _capi.device_error() == 0
+
+
+def test_select_ties_nan_and_infinities():
+    """Equal pages go to the lower index; NaN scores rank with -infinity; 1 ulp decides."""
+    bt = P.Batch([64 * 16], [1], Hq=2, Hkv=1, D=64, page=16, device=DEV)
+    q = torch.randn(1, 2, 64, generator=bt.g).to(torch.bfloat16)
+    for case in range(4):
+        bounds = torch.ones(bt.pages, 1, 2, 64, dtype=torch.bfloat16)
+        if case == 1:  # every second page better by one unit in the last place of one channel
+            bounds[bt.table[0, ::2].long(), 0, :, 17] *= 1 + 2 ** -7
+        if case == 2:
+            bounds[bt.table[0, 3:40].long(), 0, 1, 5] = math.nan
+            bounds[bt.table[0, 50].long()] = -math.inf
+        if case == 3:
+            bounds[bt.table[0, 10].long(), 0, 1] = math.inf
+            bounds[bt.table[0, 11].long(), 0, 0] = -math.inf
+        got = ops.paged_block_select(q.to(DEV), bounds.to(DEV), *bt.batch, page_size=16, keep=20, first=1, recent=1)
+        assert torch.equal(got.cpu(), P.select(bt, q, bounds, 20, 1, 1)), case
+
+
+# -------------------------------------------------------------------- as used
+def test_prefill_then_decode_with_kept_pages():
+    """Append, select and attend over several steps of three sequences: whole
+    prompts, then single tokens over kept pages, against dense attention in 64
+    bits over what the cache then holds."""
+    Hq, Hkv, D, page, B = 8, 2, 128, 16, 3
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.full((64, Hkv, page, D), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    bounds = torch.full((64, Hkv, 2, D), float("nan"), dtype=torch.bfloat16, device=DEV)
+    w = torch.ones(D, dtype=torch.bfloat16, device=DEV)
+    cos, sin = (t.to(DEV) for t in rope_tables(400, D, torch.bfloat16))
+    table = torch.randperm(64, generator=g)[:B * 20].view(B, 20).int()
+    lens = [0] * B
+    for new in ([100, 33, 257], [1, 1, 1], [1, 0, 1], [4, 1, 2]):
+        bt = P.Batch(lens, new, Hq=Hq, Hkv=Hkv, D=D, page=page, device=DEV, width=20)
+        bt.table, bt.pages = table, 64
+        lens = bt.lens
+        qkv = torch.randn(bt.N, Hq + 2 * Hkv, D, generator=g).to(torch.bfloat16).to(DEV)
+        q = ops.paged_qk_norm_rope_append(qkv, w, w, cos, sin, k, v, *bt.batch, Hq=Hq, Hkv=Hkv, k_bounds=bounds)
+        out = ops.paged_attention(q, k, v, *bt.batch, max_q=max(new), max_len=max(lens))
+        _assert_attention(bt, out, q.cpu(), k, v, 1 / math.sqrt(D))
+        kept = ops.paged_block_select(q, bounds, *bt.batch, page_size=page, keep=5, first=1, recent=2)
+        assert torch.equal(kept.cpu(), P.select(bt, q, bounds, 5, 1, 2))
+        out = ops.paged_attention(q, k, v, *bt.batch, blocks=kept)
+        _assert_attention(bt, out, q.cpu(), k, v, 1 / math.sqrt(D), kept)
