@@ -23,6 +23,10 @@ int32_t* sa_device_error_ptr();
 int sa_make_map(CUtensorMap* m, const void* base, int B, int H, int T, int D, const int64_t strides[3],
                 int box_rows, const char* name);
 
+// The same with any box: dims and box innermost first, element strides of dims 1..3.
+int sa_make_map4(CUtensorMap* m, const void* base, const int64_t dims[4], const int64_t strides[3],
+                 const int box[4], const char* name);
+
 #define SA_CHECK_CUDA(call)                                   \
   do {                                                        \
     cudaError_t _e = (call);                                  \
@@ -284,6 +288,10 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo
   return d;
 }
 
+// Instruction descriptor, kind::f16, f16 x f16 -> f32 (the A and B format fields of bf16 are 1, of f16 0).
+__host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N, bool b_mn_major) {
+  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
 // Instruction descriptor, kind::f16, bf16 x bf16 -> f32.
 __host__ __device__ constexpr uint32_t idesc_bf16_f32(int M, int N, bool b_mn_major) {
   return (1u << 4)                        // D format f32

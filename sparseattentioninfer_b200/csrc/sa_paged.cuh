@@ -117,6 +117,28 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// One launch of the attention kernels.
+struct PagedAttnParams {
+  CUtensorMap tm_q;  // the chunk kernel's
+  CUtensorMap tm_k;
+  CUtensorMap tm_v;
+  sa_paged_attn_args a;
+  int32_t tq;       // tokens per unit
+  int32_t gh;       // heads per unit
+  int32_t nhg;      // units per kv head and token tile: ceil(group / gh)
+  int32_t n_split;  // grid splits: ceil(max_len / split_len)
+  float scale_log2;
+  float* part_o;    // [N, Hq, n_split, D]
+  float* part_ml;   // [N, Hq, n_split, 2]
+  int32_t* err;
+};
+
+// Keys that the unit's last token may see.
+__device__ __forceinline__ int unit_keys(const UnitTokens& ut, int max_len) {
+  return max(0, min(min(ut.pos0 + ut.n, ut.len), max_len));
+}
+__device__ __forceinline__ int unit_splits(int keys, int split_len) { return max(1, (keys + split_len - 1) / split_len); }
+
 }  // namespace sa
 
 // Host checks of a packed batch (sa_paged_append.cu).
@@ -124,3 +146,5 @@ int sa_check_paged_batch(const sa_paged_batch* b, const char* what);
 // Pages of 16-bit elements: 16-byte aligned base, strides (page, head, slot) that are multiples of 8
 // elements, below 2^36 elements, and at least D.
 int sa_check_pages(const void* base, const int64_t strides[3], int D, const char* name);
+// The kernel for many query rows (sa_paged_chunk_sm100.cu); maps of k and v are set.
+int sa_paged_chunk_launch(sa::PagedAttnParams& prm, int64_t units, cudaStream_t stream);

@@ -28,26 +28,6 @@ constexpr int kRowStages = 3;
 constexpr int kRowKeys = 64;  // keys per stage
 constexpr int kRowMax = 16;   // query rows per CTA
 
-struct PagedRowParams {
-  CUtensorMap tm_k;
-  CUtensorMap tm_v;
-  sa_paged_attn_args a;
-  int32_t tq;       // tokens per unit
-  int32_t gh;       // heads per unit: min(group, 16)
-  int32_t nhg;      // units per kv head: ceil(group / 16)
-  int32_t n_split;  // grid splits: ceil(max_len / split_len)
-  float scale_log2;
-  float* part_o;    // [N, Hq, n_split, D]
-  float* part_ml;   // [N, Hq, n_split, 2]
-  int32_t* err;
-};
-
-// Keys that the unit's last token may see.
-__device__ __forceinline__ int unit_keys(const UnitTokens& ut, int max_len) {
-  return max(0, min(min(ut.pos0 + ut.n, ut.len), max_len));
-}
-__device__ __forceinline__ int unit_splits(int keys, int split_len) { return max(1, (keys + split_len - 1) / split_len); }
-
 template <int D>
 struct PagedRowCfg {
   static constexpr int kRegions = D / 64;
@@ -60,7 +40,7 @@ struct PagedRowCfg {
 // ROWS 8: at most 8 query rows, half of the products' rows are padding that
 // costs nothing but tensor rate; ROWS 16 holds twice the accumulators.
 template <typename T, int D, bool SPARSE, int ROWS>
-__global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_constant__ PagedRowParams p) {
+__global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_constant__ PagedAttnParams p) {
   using Cfg = PagedRowCfg<D>;
   constexpr int R = Cfg::kRegions;
   constexpr int NT = D / 8;
@@ -384,7 +364,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
 
 // Joins the splits of one (token, head) per warp.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedRowParams p, bool sparse) {
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttnParams p, bool sparse) {
   constexpr int E = D / 32;
   const sa_paged_attn_args& a = p.a;
   const int lane = threadIdx.x & 31;
@@ -429,19 +409,29 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     *reinterpret_cast<uint32_t*>(dst + e) = Half<T>::pack(acc[e] * inv, acc[e + 1] * inv);
 }
 
-// Shape of the launch: tokens per unit, splits, workspace.
-struct RowPlan {
+// Shape of the launch.
+struct AttnPlan {
+  bool chunk;  // 128-row tiles on tcgen05 instead of 16-row units
   int tq, gh, nhg, n_split, split_len;
   int64_t units;
 };
 
-static RowPlan row_plan(const sa_paged_attn_args& a, int sms) {
-  RowPlan r;
+static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
+  AttnPlan r;
   const int group = a.Hq / a.Hkv;
-  r.gh = group < kRowMax ? group : kRowMax;
-  r.nhg = (group + kRowMax - 1) / kRowMax;
-  r.tq = a.blocks ? 1 : (a.max_q < kRowMax / r.gh ? a.max_q : kRowMax / r.gh);
-  if (r.tq < 1) r.tq = 1;
+  // One 16-row unit holds all rows of a sequence: the rows kernel reads the
+  // cache once, and nothing is gained by wider tiles.
+  r.chunk = !a.blocks && group <= 128 && (int64_t)a.max_q * group > kRowMax;
+  if (r.chunk) {
+    r.gh = group;
+    r.nhg = 1;
+    r.tq = 128 / group;
+  } else {
+    r.gh = group < kRowMax ? group : kRowMax;
+    r.nhg = (group + kRowMax - 1) / kRowMax;
+    r.tq = a.blocks ? 1 : (a.max_q < kRowMax / r.gh ? a.max_q : kRowMax / r.gh);
+    if (r.tq < 1) r.tq = 1;
+  }
   r.units = unit_count(a.batch.N, a.batch.B, r.tq);
   // Keys of the longest unit.
   const int64_t cap = (int64_t)a.batch.max_pages * a.batch.page_size;
@@ -454,13 +444,15 @@ static RowPlan row_plan(const sa_paged_attn_args& a, int sms) {
   longest = (longest + kRowKeys - 1) / kRowKeys * kRowKeys;
   int64_t len = ((int64_t)a.split_len + kRowKeys - 1) / kRowKeys * kRowKeys;
   if (a.split_len <= 0) {
-    // About four CTAs per resident slot (two a SM), but at least 256 keys each.
+    // About four CTAs per resident slot (two a SM), but at least 256 keys each
+    // (1,024 in 128-row tiles, whose partial results are larger).
     const int64_t lines = (a.blocks ? r.units : a.batch.N / r.tq + 1) * a.Hkv * r.nhg;
     const int64_t want = 8ll * sms;
     const int64_t splits = lines >= want ? 1 : (want + lines - 1) / lines;
     len = (longest + splits - 1) / splits;
     len = (len + kRowKeys - 1) / kRowKeys * kRowKeys;
-    if (len < 256) len = 256;
+    const int least = r.chunk ? 1024 : 256;
+    if (len < least) len = least;
   }
   if (len > longest) len = longest;
   // The join reads every split: no more than 512 of them.
@@ -470,28 +462,41 @@ static RowPlan row_plan(const sa_paged_attn_args& a, int sms) {
   return r;
 }
 
+template <typename T, int D>
+static int launch_join(const PagedAttnParams& prm, cudaStream_t stream) {
+  const int64_t warps = (int64_t)prm.a.batch.N * prm.a.Hq;
+  paged_join_kernel<T, D><<<(unsigned)((warps + 3) / 4), 128, 0, stream>>>(prm, prm.a.blocks != nullptr);
+  SA_CHECK_CUDA(cudaGetLastError());
+  return SA_OK;
+}
+
 template <typename T, int D, bool SPARSE, int ROWS>
-static int launch_rows(const PagedRowParams& prm, const RowPlan& r, cudaStream_t stream) {
+static int launch_rows(const PagedAttnParams& prm, const AttnPlan& r, cudaStream_t stream) {
   auto kern = paged_rows_kernel<T, D, SPARSE, ROWS>;
   SA_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedRowCfg<D>::kSmemBytes));
   const int64_t gx = r.units * r.n_split, gy = (int64_t)prm.a.Hkv * r.nhg;
   if (gx > 0x7fffffff || gy > 65535) return sa_fail(SA_ERR_INVALID, "paged attention: batch too large");
   kern<<<dim3((unsigned)gx, (unsigned)gy), kRowThreads, PagedRowCfg<D>::kSmemBytes, stream>>>(prm);
   SA_CHECK_CUDA(cudaGetLastError());
-  if (r.n_split > 1) {
-    const int64_t warps = (int64_t)prm.a.batch.N * prm.a.Hq;
-    paged_join_kernel<T, D><<<(unsigned)((warps + 3) / 4), 128, 0, stream>>>(prm, SPARSE);
-    SA_CHECK_CUDA(cudaGetLastError());
-  }
   return SA_OK;
 }
 
 template <typename T, int D>
-static int launch_rows_any(const PagedRowParams& prm, const RowPlan& r, cudaStream_t stream) {
+static int launch_rows_any(const PagedAttnParams& prm, const AttnPlan& r, cudaStream_t stream) {
   const bool few = r.tq * r.gh <= 8;
   if (prm.a.blocks)
     return few ? launch_rows<T, D, true, 8>(prm, r, stream) : launch_rows<T, D, true, 16>(prm, r, stream);
   return few ? launch_rows<T, D, false, 8>(prm, r, stream) : launch_rows<T, D, false, 16>(prm, r, stream);
+}
+
+template <typename T, int D>
+static int launch_any(PagedAttnParams& prm, const AttnPlan& r, cudaStream_t stream) {
+  int rc;
+  if (r.chunk)
+    rc = sa_paged_chunk_launch(prm, r.units, stream);
+  else
+    rc = launch_rows_any<T, D>(prm, r, stream);
+  return rc || r.n_split == 1 ? rc : launch_join<T, D>(prm, stream);
 }
 
 static int check_paged_attn(const sa_paged_attn_args* a) {
@@ -504,13 +509,14 @@ static int check_paged_attn(const sa_paged_attn_args* a) {
   if (a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv)
     return sa_fail(SA_ERR_INVALID, "Hq=%d not a multiple of Hkv=%d", a->Hq, a->Hkv);
   if (a->max_q < 1 || a->max_len < 1) return sa_fail(SA_ERR_INVALID, "max_q and max_len must be at least 1");
+  if (!(a->scale > 0.f) || a->scale > 3.0e38f) return sa_fail(SA_ERR_INVALID, "scale must be positive and finite");
   if (a->split_len < 0 || a->num_sms < 0) return sa_fail(SA_ERR_INVALID, "negative split_len or num_sms");
   if ((rc = sa_check_pages(a->k_pages, a->k_strides, a->D, "k_pages"))) return rc;
   if ((rc = sa_check_pages(a->v_pages, a->v_strides, a->D, "v_pages"))) return rc;
   const int64_t* st[2] = {a->q_strides, a->o_strides};
   for (int i = 0; i < 2; ++i)
-    if (st[i][0] < 0 || st[i][1] < 0 || st[i][0] % 8 || st[i][1] % 8)
-      return sa_fail(SA_ERR_INVALID, "q/out strides must be non-negative multiples of 8 elements (16 B)");
+    if (st[i][0] <= 0 || st[i][1] <= 0 || st[i][0] % 8 || st[i][1] % 8 || (st[i][0] | st[i][1]) >= (1ll << 36))
+      return sa_fail(SA_ERR_INVALID, "q/out strides must be positive multiples of 8 elements (16 B) below 2^36");
   if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15u)
     return sa_fail(SA_ERR_INVALID, "q/out must be 16-byte aligned");
   if (a->blocks) {
@@ -531,7 +537,7 @@ extern "C" int sa_paged_attn_workspace(const sa_paged_attn_args* a, int64_t* flo
   if (!floats) return sa_fail(SA_ERR_INVALID, "floats is NULL");
   const int sms = a->num_sms > 0 ? a->num_sms : sa_num_sms();
   if (sms <= 0) return sa_fail(SA_ERR_CUDA, "cannot query SM count");
-  const RowPlan r = row_plan(*a, sms);
+  const AttnPlan r = attn_plan(*a, sms);
   *floats = r.n_split > 1 ? (int64_t)a->batch.N * a->Hq * r.n_split * (a->D + 2) : 0;
   return SA_OK;
 }
@@ -541,9 +547,9 @@ extern "C" int sa_paged_attn(const sa_paged_attn_args* a, sa_stream_t stream_) {
   if (rc) return rc;
   const int sms = a->num_sms > 0 ? a->num_sms : sa_num_sms();
   if (sms <= 0) return sa_fail(SA_ERR_CUDA, "cannot query SM count");
-  const RowPlan r = row_plan(*a, sms);
+  const AttnPlan r = attn_plan(*a, sms);
   if (r.n_split > 1 && !a->workspace) return sa_fail(SA_ERR_INVALID, "paged attention: workspace is NULL");
-  PagedRowParams prm;
+  PagedAttnParams prm;
   memset(&prm, 0, sizeof(prm));
   const int box = a->batch.page_size < kRowKeys ? a->batch.page_size : kRowKeys;
   if ((rc = sa_make_map(&prm.tm_k, a->k_pages, a->batch.num_pages, a->Hkv, a->batch.page_size, a->D, a->k_strides,
@@ -564,7 +570,6 @@ extern "C" int sa_paged_attn(const sa_paged_attn_args* a, sa_stream_t stream_) {
   prm.err = sa_device_error_ptr();
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream_);
   if (a->dtype == SA_BF16)
-    return a->D == 128 ? launch_rows_any<__nv_bfloat16, 128>(prm, r, st)
-                       : launch_rows_any<__nv_bfloat16, 64>(prm, r, st);
-  return a->D == 128 ? launch_rows_any<__half, 128>(prm, r, st) : launch_rows_any<__half, 64>(prm, r, st);
+    return a->D == 128 ? launch_any<__nv_bfloat16, 128>(prm, r, st) : launch_any<__nv_bfloat16, 64>(prm, r, st);
+  return a->D == 128 ? launch_any<__half, 128>(prm, r, st) : launch_any<__half, 64>(prm, r, st);
 }

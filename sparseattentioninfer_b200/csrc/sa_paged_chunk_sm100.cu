@@ -1,0 +1,467 @@
+// sa_paged_chunk_sm100.cu — causal attention over a paged cache for many query
+// rows: chunks of prompts and whole prompts.
+//
+// One CTA is one tile of 128 query rows of one kv head over one split of the
+// keys: 128 / G consecutive tokens times the group's G heads (rows ordered token
+// by token), so each key is read once for the whole group and a chunk of a few
+// dozen tokens still fills the tile. Two CTAs fit on an SM: the softmax of one
+// runs while the other's products do. Six warps:
+//   warp 0     TMA producer: Q (one box of heads x tokens), then 64-key chunks of
+//              K and V, a box per page and 64 columns, into rings (SWIZZLE_128B).
+//              A page past the keys, or a bad one, is loaded from behind the last
+//              page of the map, which reads as zeros.
+//   warp 1     tcgen05.mma issuer: S = Q K^T into one of two TMEM buffers, then
+//              O += P V with P read from TMEM.
+//   warps 2-5  softmax, one thread a row: running maximum and sum in registers, P
+//              (16 bits) written over S, O rescaled in TMEM only when the maximum
+//              grew by more than 2^8 (the same stale maximum serves P, sum and O).
+// Slots behind the last key may hold anything: S there is masked, and V's rows
+// are set to zero in shared memory by the softmax warps before P is handed over.
+// Unsplit tiles write out = O / l; split ones their O, maximum and sum.
+#include <type_traits>
+
+#include "sa_paged.cuh"
+
+namespace sa {
+
+constexpr int kChM = 128;      // query rows
+constexpr int kChN = 64;       // keys per chunk
+constexpr int kChMeta = 16;    // ring of page masks; see kMetaRing of the block-sparse kernel
+constexpr int kChThreads = 192;
+
+template <typename T>
+constexpr uint32_t chunk_idesc(int N, bool b_mn_major) {
+  return std::is_same<T, __half>::value ? idesc_f16_f32(kChM, N, b_mn_major)
+                                                           : idesc_bf16_f32(kChM, N, b_mn_major);
+}
+
+template <int D>
+struct ChunkCfg {
+  static constexpr int kRegions = D / 64;
+  static constexpr int kQBytes = kChM * D * 2;
+  static constexpr int kKVBytes = kChN * D * 2;
+  static constexpr int kTmemCols = 256;  // O [0, D), S/P at D and D + 64; two CTAs share the SM's 512
+  static_assert(D + 2 * kChN <= kTmemCols, "TMEM over-subscribed");
+  // Two CTAs on an SM's 228 KB, less 1 KB each that the hardware keeps and 1 KB of static data.
+  static constexpr int kBufs = (233472 / 2 - 2048 - kQBytes) / kKVBytes;
+  // V is used a whole softmax later than K, so the odd buffer is V's.
+  static constexpr int kKStages = kBufs / 2 > 4 ? 4 : kBufs / 2;
+  static constexpr int kVStages = kBufs - kKStages > 4 ? 4 : kBufs - kKStages;
+  static constexpr int kSmemBytes = kQBytes + (kKStages + kVStages) * kKVBytes;
+  static_assert(kKStages >= 2 && kVStages >= 2, "not enough shared memory");
+  static_assert(kKStages + 3 < kChMeta, "mask ring too short");
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid_constant__ PagedAttnParams p,
+                                                                    int64_t units) {
+  using Cfg = ChunkCfg<D>;
+  constexpr int N = kChN, R = Cfg::kRegions, NSK = Cfg::kKStages, NSV = Cfg::kVStages;
+  constexpr uint32_t SB = D;  // first S/P column
+  __shared__ __align__(8) uint64_t bar_q, bar_drain;
+  __shared__ __align__(8) uint64_t bar_k_full[NSK], bar_k_empty[NSK], bar_v_full[NSV], bar_v_empty[NSV];
+  __shared__ __align__(8) uint64_t bar_p_full[2], bar_meta[kChMeta];
+  __shared__ uint32_t meta_mask[kChMeta];  // 16-key groups of the chunk that hold keys
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ int abort_flag;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const sa_paged_attn_args& a = p.a;
+  const sa_paged_batch& bt = a.batch;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.gh, ps = bt.page_size;
+  // Tiles of late tokens see the most keys: they come first, all heads of a
+  // token tile side by side.
+  const int kvh = blockIdx.x % a.Hkv;
+  const int64_t rest = blockIdx.x / a.Hkv;
+  const int split = (int)(rest % p.n_split);
+  UnitTokens ut;
+  if (!unit_tokens(bt, units - 1 - rest / p.n_split, p.tq, p.err, ut)) return;
+  const int keys = unit_keys(ut, a.max_len);
+  if (keys < min(ut.pos0 + ut.n, ut.len) && lane == 0) record_error(p.err, SA_DEV_ERR_INDEX);
+  if (split >= unit_splits(keys, a.split_len)) return;
+  const int c0 = split * (a.split_len / N);  // chunks [c0, c0 + nch)
+  const int nch = max(0, min((keys + N - 1) / N, c0 + a.split_len / N) - c0);
+  const int rows = ut.n * G;
+  const uint32_t sQ = smem_u32(smem_raw), sK = sQ + Cfg::kQBytes, sV = sK + NSK * Cfg::kKVBytes;
+
+  auto out_row = [&](int r) {
+    return reinterpret_cast<T*>(a.out) + (int64_t)(ut.t0 + r / G) * a.o_strides[0] +
+           (int64_t)(kvh * G + r % G) * a.o_strides[1];
+  };
+  auto part_at = [&](int r) {
+    return ((int64_t)(ut.t0 + r / G) * a.Hq + kvh * G + r % G) * p.n_split + split;
+  };
+  if (nch == 0 || (sQ & 1023u)) {  // block-uniform
+    if (threadIdx.x == 0 && (sQ & 1023u)) record_error(p.err, SA_DEV_ERR_INDEX);
+    for (int r = threadIdx.x; r < rows; r += kChThreads) {
+      if (p.n_split == 1) {
+        for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(out_row(r) + d) = make_uint4(0, 0, 0, 0);
+      } else {
+        p.part_ml[part_at(r) * 2] = -INFINITY;
+        p.part_ml[part_at(r) * 2 + 1] = 0.f;
+      }
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&bar_q), 1);
+    mbar_init(smem_u32(&bar_drain), 1);
+    for (int i = 0; i < NSK; ++i) {
+      mbar_init(smem_u32(&bar_k_full[i]), 1);
+      mbar_init(smem_u32(&bar_k_empty[i]), 1);
+    }
+    for (int i = 0; i < NSV; ++i) {
+      mbar_init(smem_u32(&bar_v_full[i]), 1);
+      mbar_init(smem_u32(&bar_v_empty[i]), 1);
+    }
+    for (int i = 0; i < kChMeta; ++i) mbar_init(smem_u32(&bar_meta[i]), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&bar_p_full[i]), 128);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&tmem_base_sh), Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;
+  volatile int* abort_v = &abort_flag;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ producer
+    // Lane j < pps loads page j of a chunk; page numbers are read 32 ahead.
+    if (lane == 0) {
+      mbar_arrive_expect_tx(smem_u32(&bar_q), (uint32_t)p.tq * G * D * 2);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        tma_load_4d(sQ + r * kChM * 128, &p.tm_q, smem_u32(&bar_q), r * 64, kvh * G, ut.t0, 0);
+    }
+    const int32_t* trow = bt.table + (int64_t)ut.b * bt.table_stride;
+    const int pps = ps < N ? N / ps : 1, spp = ps > N ? ps / N : 1, box = min(ps, N);
+    const int e0 = c0 / spp * pps;
+    int page = bt.num_pages, base = -32, kn = 0, vn = 0;  // chunks of K and V issued
+    bool ok = true, bad = false;
+    for (int g = 0; g < nch; ++g) {
+      const int first = (c0 + g) / spp * pps - e0;
+      if (first >= base + 32) {
+        base = first;
+        const int64_t blk = (int64_t)e0 + base + lane;
+        page = bt.num_pages;  // behind the last page: reads as zeros
+        if (blk * ps < keys) {
+          const int pg = __ldg(trow + blk);
+          if (pg < 0 || pg >= bt.num_pages)
+            bad = true;
+          else
+            page = pg;
+        }
+      }
+      const int pg = __shfl_sync(0xffffffffu, page, (first - base + (lane < pps ? lane : 0)) & 31);
+      const int off = spp > 1 ? ((c0 + g) % spp) * N : 0;
+      const unsigned have = __ballot_sync(0xffffffffu, lane < pps && pg < bt.num_pages);
+      const int ks = g % NSK, vs = g % NSV, ms = g % kChMeta;
+      if (g >= NSK) {
+        ok = mbar_wait(smem_u32(&bar_k_empty[ks]), ((g / NSK) - 1) & 1, abort_v, p.err);
+        if (!__all_sync(0xffffffffu, ok)) break;
+      }
+      if (lane == 0) {
+        uint32_t mask = 0;
+        for (int j = 0; j < pps; ++j)
+          if ((have >> j) & 1u) mask |= ((1u << (box / 16)) - 1) << (j * (box / 16));
+        meta_mask[ms] = mask;
+        mbar_arrive(smem_u32(&bar_meta[ms]));
+        mbar_arrive_expect_tx(smem_u32(&bar_k_full[ks]), Cfg::kKVBytes);
+      }
+      __syncwarp();
+      if (lane < pps) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          tma_load_4d(sK + ks * Cfg::kKVBytes + r * N * 128 + lane * box * 128, &p.tm_k, smem_u32(&bar_k_full[ks]),
+                      r * 64, off, kvh, pg);
+      }
+      ++kn;
+      if (g >= NSV) {
+        ok = mbar_wait(smem_u32(&bar_v_empty[vs]), ((g / NSV) - 1) & 1, abort_v, p.err);
+        if (!__all_sync(0xffffffffu, ok)) break;
+      }
+      if (lane == 0) mbar_arrive_expect_tx(smem_u32(&bar_v_full[vs]), Cfg::kKVBytes);
+      __syncwarp();
+      if (lane < pps) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          tma_load_4d(sV + vs * Cfg::kKVBytes + r * N * 128 + lane * box * 128, &p.tm_v, smem_u32(&bar_v_full[vs]),
+                      r * 64, off, kvh, pg);
+      }
+      ++vn;
+    }
+    if (__any_sync(0xffffffffu, bad) && lane == 0) record_error(p.err, SA_DEV_ERR_INDEX);
+    // Drain: wait (bounded, ignoring the abort flag) for copies still in flight.
+    int zero = 0;
+    volatile int* never = &zero;
+    for (int i = max(0, kn - NSK); i < kn; ++i)
+      mbar_wait(smem_u32(&bar_k_full[i % NSK]), (i / NSK) & 1, never, nullptr);
+    for (int i = max(0, vn - NSV); i < vn; ++i)
+      mbar_wait(smem_u32(&bar_v_full[i % NSV]), (i / NSV) & 1, never, nullptr);
+    mbar_wait(smem_u32(&bar_q), 0, never, nullptr);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = chunk_idesc<T>(N, false);
+      constexpr uint32_t idesc_pv = chunk_idesc<T>(D, true);
+      const uint64_t q_desc = smem_desc_sw128(sQ, 16, 1024);
+      const uint64_t k_desc = smem_desc_sw128(sK, 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(sV, N * 128, 1024);
+      // S = Q K^T of chunk g; its commit frees the K slot and tells the softmax.
+      auto next_s = [&](int g) -> bool {
+        const int ks = g % NSK;
+        if (!mbar_wait(smem_u32(&bar_k_full[ks]), (g / NSK) & 1, abort_v, p.err)) return false;
+        tc_fence_after();
+        const uint32_t d = tmem + SB + (g & 1) * N;
+        const uint64_t kst = k_desc + (uint64_t)((ks * Cfg::kKVBytes) >> 4);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const int r = k >> 2, kk = k & 3;
+          mma_ss(d, q_desc + ((r * kChM * 128 + kk * 32) >> 4), kst + ((r * N * 128 + kk * 32) >> 4), idesc_s,
+                 k > 0 ? 1u : 0u);
+        }
+        mma_commit(smem_u32(&bar_k_empty[ks]));
+        return true;
+      };
+      bool ok = mbar_wait(smem_u32(&bar_q), 0, abort_v, p.err) && next_s(0);
+      for (int g = 0; ok && g < nch; ++g) {
+        // S of the next chunk goes in before this chunk's PV.
+        if (g + 1 < nch && !(ok = next_s(g + 1))) break;
+        if (!(ok = mbar_wait(smem_u32(&bar_p_full[g & 1]), (g >> 1) & 1, abort_v, p.err))) break;
+        const int vs = g % NSV;
+        if (!(ok = mbar_wait(smem_u32(&bar_v_full[vs]), (g / NSV) & 1, abort_v, p.err))) break;
+        tc_fence_after();
+        const uint32_t pbuf = tmem + SB + (g & 1) * N;
+        const uint64_t vst = v_desc + (uint64_t)((vs * Cfg::kKVBytes) >> 4);
+#pragma unroll
+        for (int k = 0; k < N / 16; ++k)
+          mma_ts(tmem, pbuf + k * 8, vst + ((k * 2048) >> 4), idesc_pv, (k > 0 || g > 0) ? 1u : 0u);
+        mma_commit(smem_u32(&bar_v_empty[vs]));  // PV of chunk g retired: V slot free, O holds it
+      }
+      mma_commit(smem_u32(&bar_drain));
+      int zero = 0;
+      mbar_wait(smem_u32(&bar_drain), 0, &zero, nullptr);
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax
+    const int wr = warp & 3;  // TMEM lane quadrant this warp may access
+    const int row = wr * 32 + lane;
+    const uint32_t lane_base = (uint32_t)(wr * 32) << 16;
+    const unsigned FULL = 0xffffffffu;
+    const bool row_ok = row < rows;
+    const int pos = row_ok ? min(ut.pos0 + row / G, keys - 1) : -1;
+    float m_ref = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int g = 0; g < nch; ++g) {
+      const int ms = g % kChMeta;
+      ok = mbar_wait(smem_u32(&bar_meta[ms]), (g / kChMeta) & 1, abort_v, p.err);
+      if (!__all_sync(FULL, ok)) { ok = false; break; }
+      const uint32_t mask = meta_mask[ms];
+      ok = mbar_wait(smem_u32(&bar_k_empty[g % NSK]), (g / NSK) & 1, abort_v, p.err);  // S is in TMEM
+      if (!__all_sync(FULL, ok)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t sbuf = tmem + lane_base + SB + (g & 1) * N;
+      const int key0 = (c0 + g) * N;
+      float s[N];
+      {
+        uint32_t r32[2][32];
+        tmem_ld32(sbuf, r32[0]);
+        tmem_ld32(sbuf + 32, r32[1]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          reg_fence32(r32[cc]);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[cc * 32 + i] = __uint_as_float(r32[cc][i]);
+        }
+      }
+      const int lim = pos - key0;  // columns <= lim are seen
+      if (lim < N - 1 || mask != 0xfu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = (i <= lim && ((mask >> (i / 16)) & 1u)) ? s[i] : -INFINITY;
+      }
+      float mx8[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx8[i] = s[i];
+#pragma unroll
+      for (int i = 8; i < N; i += 2) mx8[(i >> 1) & 7] = max3(mx8[(i >> 1) & 7], s[i], s[i + 1]);
+      const float mraw = max3(fmaxf(max3(mx8[0], mx8[1], mx8[2]), mx8[3]), max3(mx8[4], mx8[5], mx8[6]), mx8[7]);
+      const float m_new = fmaxf(m_ref, mraw * p.scale_log2);
+      if (g == 0) {
+        m_ref = m_new;
+      } else {
+        const bool need = m_new > m_ref + 8.0f;
+        if (__any_sync(FULL, need)) {
+          // O still takes the previous chunk's PV: wait for it, then rescale.
+          ok = mbar_wait(smem_u32(&bar_v_empty[(g - 1) % NSV]), ((g - 1) / NSV) & 1, abort_v, p.err);
+          if (!__all_sync(FULL, ok)) { ok = false; break; }
+          tc_fence_after();
+          const float alpha = need ? ex2(m_ref - m_new) : 1.0f;
+#pragma unroll
+          for (int cc = 0; cc < D / 32; ++cc) {
+            uint32_t o32[32];
+            tmem_ld32(tmem + lane_base + cc * 32, o32);
+            tmem_wait_ld();
+            reg_fence32(o32);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o32[i] = __float_as_uint(__uint_as_float(o32[i]) * alpha);
+            tmem_st32(tmem + lane_base + cc * 32, o32);
+          }
+          tmem_wait_st();
+          if (need) {
+            l *= alpha;
+            m_ref = m_new;
+          }
+        }
+      }
+      const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
+      const uint64_t sc2 = f2pack(p.scale_log2, p.scale_log2), nm2 = f2pack(-m_use, -m_use);
+      uint64_t rs4[4] = {0ull, 0ull, 0ull, 0ull};
+      uint32_t pk[N / 2];
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        float x0, x1;
+        f2unpack(fma2(f2pack(s[2 * i], s[2 * i + 1]), sc2, nm2), x0, x1);
+        const float p0 = ex2(x0), p1 = ex2(x1);
+        rs4[i & 3] = add2(rs4[i & 3], f2pack(p0, p1));
+        pk[i] = Half<T>::pack(p0, p1);
+      }
+      tmem_st32(sbuf, pk);
+      {
+        float a0, a1, b0, b1;
+        f2unpack(add2(rs4[0], rs4[1]), a0, a1);
+        f2unpack(add2(rs4[2], rs4[3]), b0, b1);
+        l += (a0 + a1) + (b0 + b1);
+      }
+      if (key0 + N > keys) {
+        // V rows past the last key: zero, whatever the page holds there.
+        ok = mbar_wait(smem_u32(&bar_v_full[g % NSV]), (g / NSV) & 1, abort_v, p.err);
+        if (!__all_sync(FULL, ok)) { ok = false; break; }
+        const uint32_t v0 = sV + (g % NSV) * Cfg::kKVBytes;
+        const int first = keys - key0;
+        for (int i = row; i < (N - first) * 8 * R; i += 128) {
+          const int reg = i / ((N - first) * 8), in = i % ((N - first) * 8);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v0 + reg * N * 128 + first * 128 + in * 16),
+                       "r"(0u)
+                       : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&bar_p_full[g & 1]));
+    }
+    // ---------------------------------------------------------------- epilogue
+    if (ok) ok = mbar_wait(smem_u32(&bar_v_empty[(nch - 1) % NSV]), ((nch - 1) / NSV) & 1, abort_v, p.err);
+    if (__all_sync(FULL, ok)) {
+      tc_fence_after();
+      uint32_t o32[D / 32][32];
+#pragma unroll
+      for (int cc = 0; cc < D / 32; ++cc) tmem_ld32(tmem + lane_base + cc * 32, o32[cc]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int cc = 0; cc < D / 32; ++cc) reg_fence32(o32[cc]);
+      if (p.n_split > 1) {
+        if (row_ok) {
+          const int64_t at = part_at(row);
+          float4* dst = reinterpret_cast<float4*>(p.part_o + at * D);
+#pragma unroll
+          for (int cc = 0; cc < D / 32; ++cc)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dst[cc * 8 + i] = make_float4(__uint_as_float(o32[cc][4 * i]), __uint_as_float(o32[cc][4 * i + 1]),
+                                            __uint_as_float(o32[cc][4 * i + 2]), __uint_as_float(o32[cc][4 * i + 3]));
+          *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
+        }
+      } else {
+        // One thread owns one row: pack it to 16 bits, then transpose chunks of
+        // rows among 4 lanes (shfl_xor butterflies), so that a store instruction
+        // writes whole rows of the group and not 32-byte pieces of 32 rows.
+        constexpr int TG = 4, W = D / 2, CW = W / TG;
+        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+        uint32_t u[W];
+#pragma unroll
+        for (int cc = 0; cc < D / 32; ++cc)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            u[cc * 16 + i] = Half<T>::pack(__uint_as_float(o32[cc][2 * i]) * inv,
+                                           __uint_as_float(o32[cc][2 * i + 1]) * inv);
+        const int j = lane % TG;
+#pragma unroll
+        for (int m = 1; m < TG; m <<= 1) {
+          const bool jb = (j & m) != 0;
+#pragma unroll
+          for (int x0 = 0; x0 < TG; ++x0) {
+            if (x0 & m) continue;
+            const int x1 = x0 | m;
+#pragma unroll
+            for (int i = 0; i < CW; ++i) {
+              const uint32_t r = __shfl_xor_sync(FULL, jb ? u[x0 * CW + i] : u[x1 * CW + i], m);
+              if (jb)
+                u[x0 * CW + i] = r;
+              else
+                u[x1 * CW + i] = r;
+            }
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < TG; ++kk) {
+          const int r = wr * 32 + lane / TG * TG + kk;
+          if (r < rows) {
+            T* dst = out_row(r) + j * (2 * CW);
+            if ((reinterpret_cast<uintptr_t>(dst) & 31u) == 0) {
+#pragma unroll
+              for (int v8 = 0; v8 < CW / 8; ++v8) st_global_v8(dst + 16 * v8, u + kk * CW + 8 * v8);
+            } else {
+              uint4* d4 = reinterpret_cast<uint4*>(dst);
+#pragma unroll
+              for (int i = 0; i < CW / 4; ++i)
+                d4[i] = make_uint4(u[kk * CW + 4 * i], u[kk * CW + 4 * i + 1], u[kk * CW + 4 * i + 2],
+                                   u[kk * CW + 4 * i + 3]);
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, Cfg::kTmemCols);
+}
+
+template <typename T, int D>
+static int launch_chunk(const PagedAttnParams& prm, int64_t units, cudaStream_t stream) {
+  auto kern = paged_chunk_kernel<T, D>;
+  SA_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkCfg<D>::kSmemBytes));
+  SA_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+  const int64_t blocks = units * prm.n_split * prm.a.Hkv;
+  if (blocks > 0x7fffffff) return sa_fail(SA_ERR_INVALID, "paged attention: batch too large");
+  kern<<<(unsigned)blocks, kChThreads, ChunkCfg<D>::kSmemBytes, stream>>>(prm, units);
+  SA_CHECK_CUDA(cudaGetLastError());
+  return SA_OK;
+}
+
+}  // namespace sa
+
+using namespace sa;
+
+int sa_paged_chunk_launch(PagedAttnParams& prm, int64_t units, cudaStream_t stream) {
+  const sa_paged_attn_args& a = prm.a;
+  // Q: (64 columns) x (the group's heads) x (tq tokens), a row of the tile each.
+  const int64_t dims[4] = {a.D, a.Hq, a.batch.N, 1};
+  const int64_t strides[3] = {a.q_strides[1], a.q_strides[0], 8};
+  const int box[4] = {64, prm.gh, prm.tq, 1};
+  int rc = sa_make_map4(&prm.tm_q, a.q, dims, strides, box, "q");
+  if (rc) return rc;
+  if (a.dtype == SA_BF16)
+    return a.D == 128 ? launch_chunk<__nv_bfloat16, 128>(prm, units, stream)
+                      : launch_chunk<__nv_bfloat16, 64>(prm, units, stream);
+  return a.D == 128 ? launch_chunk<__half, 128>(prm, units, stream) : launch_chunk<__half, 64>(prm, units, stream);
+}
