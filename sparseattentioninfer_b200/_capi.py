@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -132,6 +133,14 @@ class PagedSelectArgs(ctypes.Structure):
                 ("recent", _c_i32), ("max_q", _c_i32)]
 
 
+# The same structures packed in one call (native alignment): filling a ctypes
+# structure field by field costs several microseconds, as much as a small launch.
+_PB = "PPPqiiiii4x"
+PAGED_APPEND = struct.Struct("@" + _PB + "PqPPPPP2qP3qP3qP3qiiiiif0q")
+PAGED_ATTN = struct.Struct("@" + _PB + "PP2q2qP3qP3qP2qiiiiifiiiiP0q")
+PAGED_SELECT = struct.Struct("@" + _PB + "P2qP3qP2qiiiiiiii0q")
+
+
 class ArPeers(ctypes.Structure):
     _fields_ = [("rank", _c_i32), ("world", _c_i32), ("data", _c_p * 8), ("flags", _c_p * 8), ("epoch", _c_p),
                 ("max_ctas", _c_i32)]
@@ -175,10 +184,11 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     lib.sa_silu_mul.argtypes = [_c_p, _c_p, _c_i64, _c_i32, _c_i64, _c_i64, _c_p]
     lib.sa_linear_m8.argtypes = [_c_p, _c_i32, _c_i32, _c_i64, _c_p, _c_i32, _c_i64, _c_p, _c_i64, _c_i32, _c_p]
     lib.sa_topk_softmax_pv.argtypes = [ctypes.POINTER(TopkArgs), _c_p]
-    lib.sa_paged_append.argtypes = [ctypes.POINTER(PagedAppendArgs), _c_p]
-    lib.sa_paged_attn_workspace.argtypes = [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(_c_i64)]
-    lib.sa_paged_attn.argtypes = [ctypes.POINTER(PagedAttnArgs), _c_p]
-    lib.sa_paged_select.argtypes = [ctypes.POINTER(PagedSelectArgs), _c_p]
+    # (argument structures as PAGED_*.pack() bytes or a pointer to the ctypes structure)
+    lib.sa_paged_append.argtypes = [_c_p, _c_p]
+    lib.sa_paged_attn_workspace.argtypes = [_c_p, ctypes.POINTER(_c_i64)]
+    lib.sa_paged_attn.argtypes = [_c_p, _c_p]
+    lib.sa_paged_select.argtypes = [_c_p, _c_p]
     lib.sa_ar_alloc.argtypes = [ctypes.c_size_t, ctypes.POINTER(_c_p)]
     lib.sa_ar_free.argtypes = [_c_p]
     lib.sa_ar_ipc_handle.argtypes = [_c_p, _c_p]

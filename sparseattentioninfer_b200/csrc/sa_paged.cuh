@@ -148,3 +148,5 @@ int sa_check_paged_batch(const sa_paged_batch* b, const char* what);
 int sa_check_pages(const void* base, const int64_t strides[3], int D, const char* name);
 // The kernel for many query rows (sa_paged_chunk_sm100.cu); maps of k and v are set.
 int sa_paged_chunk_launch(sa::PagedAttnParams& prm, int64_t units, cudaStream_t stream);
+// Raises a kernel's dynamic shared memory limit (and with it the SM's carve-out), once per device.
+int sa_smem_once(const void* kernel, int bytes, bool (&done)[64]);

@@ -211,6 +211,16 @@ int sa_check_paged_batch(const sa_paged_batch* b, const char* what) {
   return SA_OK;
 }
 
+int sa_smem_once(const void* kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  SA_CHECK_CUDA(cudaGetDevice(&dev));
+  if (dev >= 0 && dev < 64 && done[dev]) return SA_OK;
+  SA_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  SA_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+  if (dev >= 0 && dev < 64) done[dev] = true;
+  return SA_OK;
+}
+
 int sa_check_pages(const void* base, const int64_t strides[3], int D, const char* name) {
   if (!base) return sa_fail(SA_ERR_INVALID, "%s is NULL", name);
   if (reinterpret_cast<uintptr_t>(base) & 15u) return sa_fail(SA_ERR_INVALID, "%s must be 16-byte aligned", name);

@@ -473,7 +473,9 @@ static int launch_join(const PagedAttnParams& prm, cudaStream_t stream) {
 template <typename T, int D, bool SPARSE, int ROWS>
 static int launch_rows(const PagedAttnParams& prm, const AttnPlan& r, cudaStream_t stream) {
   auto kern = paged_rows_kernel<T, D, SPARSE, ROWS>;
-  SA_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedRowCfg<D>::kSmemBytes));
+  static bool done[64];
+  int rc = sa_smem_once(reinterpret_cast<const void*>(kern), PagedRowCfg<D>::kSmemBytes, done);
+  if (rc) return rc;
   const int64_t gx = r.units * r.n_split, gy = (int64_t)prm.a.Hkv * r.nhg;
   if (gx > 0x7fffffff || gy > 65535) return sa_fail(SA_ERR_INVALID, "paged attention: batch too large");
   kern<<<dim3((unsigned)gx, (unsigned)gy), kRowThreads, PagedRowCfg<D>::kSmemBytes, stream>>>(prm);

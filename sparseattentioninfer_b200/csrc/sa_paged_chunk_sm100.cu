@@ -439,8 +439,9 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
 template <typename T, int D>
 static int launch_chunk(const PagedAttnParams& prm, int64_t units, cudaStream_t stream) {
   auto kern = paged_chunk_kernel<T, D>;
-  SA_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkCfg<D>::kSmemBytes));
-  SA_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+  static bool done[64];
+  int rc = sa_smem_once(reinterpret_cast<const void*>(kern), ChunkCfg<D>::kSmemBytes, done);
+  if (rc) return rc;
   const int64_t blocks = units * prm.n_split * prm.a.Hkv;
   if (blocks > 0x7fffffff) return sa_fail(SA_ERR_INVALID, "paged attention: batch too large");
   kern<<<(unsigned)blocks, kChThreads, ChunkCfg<D>::kSmemBytes, stream>>>(prm, units);

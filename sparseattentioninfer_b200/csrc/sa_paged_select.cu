@@ -6,190 +6,440 @@
 // Q+ = sum_g max(q_g, 0), Q- = sum_g min(q_g, 0): the group's heads are summed
 // once, so a page costs 2 D multiply-adds however many heads share it.
 //
-// Which pages are kept goes by the order of near values, so the scores are
-// summed in 64 bits (16-bit factors: only the sums round) and each page in the
-// same order, so that equal pages tie exactly; ties go to the lower index.
-// One CTA per (token, kv head): scores to shared memory as order-preserving
-// 64-bit keys, the keep-th largest by radix select, the kept indexes out in
-// ascending order by a scan.
+// Which pages are kept goes by the order of near values: it has to be the order
+// of the scores in 64 bits, but only the pages near the border need them. One
+// CTA serves up to 8 tokens of a sequence and one kv head:
+//  1. Scores of all pages with mma.sync m16n8k16, 16 pages x 8 tokens, in 32
+//     bits: Q is scaled by a power of two (rank does not change) and split into
+//     two 16-bit parts hi + lo, and a third product sums the sizes
+//     A = sum |Q| |b|, by which every 32-bit score is within
+//       eps = 2^-14 max A  of the real one:
+//     the split leaves 2^-16 |Q| (bf16; fp16 less, and its subnormals at most
+//     2^-25 a channel, which the 2^-9 added to |Q| covers), and 16 chained MMAs
+//     of 16 products that each lose at most 17 * 2^-24 of the largest addend
+//     16 * 17 * 2^-24 < 2^-15.9.
+//  2. A warp a token (or the CTA, when it has one token) bisects for the 32-bit score t that fills the list. Pages
+//     above t + 2 eps are in, pages below t - 2 eps out; what lies between is
+//     summed again in 64 bits (16-bit factors, so only the sums round; every
+//     page in the same order, so equal pages tie exactly) and ranked, ties to the
+//     lower index. A row with scores that are not finite is summed again whole.
+//  3. The kept indexes are written in ascending order by ballots.
 #include "sa_paged.cuh"
 
 namespace sa {
 
 constexpr int kSelThreads = 256;
-constexpr int kSelMaxPages = 16384;  // 128 KB of keys
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelTokens = 8;
+constexpr int kSelMaxPages = 16384;
 constexpr int kSelMaxKeep = 4096;
+constexpr int kSelRegs = 16;  // keys a lane holds in registers
+constexpr int kSelMid = 32;
+constexpr unsigned kAll = 0xffffffffu;
 
 __device__ __forceinline__ uint64_t order_key(double x) {
   if (x != x) x = -INFINITY;  // NaN counts as the lowest score
   const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);  // -0 and 0 are equal
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
-
-// Exclusive prefix of the block's flags, and their number.
-__device__ __forceinline__ int block_rank(bool flag, int* warp_cnt, int& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned m = __ballot_sync(0xffffffffu, flag);
-  if (lane == 0) warp_cnt[warp] = __popc(m);
-  __syncthreads();
-  int before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kSelThreads / 32; ++w) {
-    const int c = warp_cnt[w];
-    if (w < warp) before += c;
-    all += c;
-  }
-  __syncthreads();
-  total = all;
-  return before + __popc(m & ((1u << lane) - 1));
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k);
 }
 
 template <typename T, int D>
+struct SelectCfg {
+  static constexpr int kRow = 4 * D + 64;                       // bytes of one token's Q part: 2 D values, padded
+  static constexpr int kPart = kSelTokens * kRow;               // hi, lo or |Q|
+  static constexpr int kQd = 3 * kPart;                         // Q in 64 bits: [token][2 D]
+  static constexpr int kKeys = kQd + kSelTokens * 2 * D * 8;    // keys: [token][pages], 64 bits each
+};
+
+// The score of one page in 64 bits, in every lane.
+template <typename T, int D>
+__device__ __forceinline__ double page_score(const T* low, int64_t to_high, const double* q, int lane) {
+  constexpr int E = D / 32;
+  double s = 0.;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int d = lane * E + e;
+    s = fma(q[d], (double)Half<T>::to(low[d]), s);
+    s = fma(q[D + d], (double)Half<T>::to(low[to_high + d]), s);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+  if (s != s) {
+    // An infinite bound met a factor of 0, which leaves it out of the maximum.
+    s = 0.;
+    for (int e = 0; e < E; ++e) {
+      const int d = lane * E + e;
+      if (q[d] != 0.) s = fma(q[d], (double)Half<T>::to(low[d]), s);
+      if (q[D + d] != 0.) s = fma(q[D + d], (double)Half<T>::to(low[to_high + d]), s);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+  }
+  return s;
+}
+
+// Pages whose order the 32-bit scores leave open.
+struct MidList {
+  int n;
+  int at[kSelMid];
+  uint64_t key[kSelMid];
+};
+
+// ONE: a token a CTA, whose warps share its selection.
+template <typename T, int D, bool ONE>
 __global__ void __launch_bounds__(kSelThreads)
-    paged_select_kernel(const __grid_constant__ sa_paged_select_args a, int32_t* err) {
-  extern __shared__ __align__(16) uint64_t keys[];  // [max_pages]
-  __shared__ double qs[2][D];                       // Q-, Q+
-  __shared__ int hist[256];
-  __shared__ int warp_cnt[kSelThreads / 32];
-  __shared__ int s_bucket, s_above;
+    paged_select_kernel(const __grid_constant__ sa_paged_select_args a, int tq, int32_t* err) {
+  using Cfg = SelectCfg<T, D>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int s_amax[kSelTokens];
+  __shared__ int s_wild[kSelTokens];  // the row has a score that is not finite
+  __shared__ MidList s_mid[ONE ? 1 : kSelWarps];
+  __shared__ uint32_t s_part[3][kSelWarps];
+  double* qd = reinterpret_cast<double*>(smem + Cfg::kQd);
+  uint64_t* keys = reinterpret_cast<uint64_t*>(smem + Cfg::kKeys);
   const sa_paged_batch& bt = a.batch;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int kvh = blockIdx.y, G = a.Hq / a.Hkv;
+  const int kvh = blockIdx.y, G = a.Hq / a.Hkv, ps = bt.page_size, W = bt.max_pages;
   UnitTokens ut;
-  if (!unit_tokens(bt, blockIdx.x, 1, err, ut)) return;
-  int32_t* out = a.out + (int64_t)ut.t0 * a.out_strides[0] + (int64_t)kvh * a.out_strides[1];
-  const int last = min(ut.pos0 / bt.page_size, bt.max_pages - 1);
-  const int nvis = last + 1;
-  if (nvis <= a.keep) {
-    for (int i = tid; i < a.keep; i += kSelThreads) out[i] = i < nvis ? i : -1;
-    return;
-  }
-  for (int d = tid; d < D; d += kSelThreads) {
-    const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)ut.t0 * a.q_strides[0] +
-                 (int64_t)kvh * G * a.q_strides[1] + d;
-    double lo = 0., hi = 0.;
-    for (int g = 0; g < G; ++g) {
-      const float x = Half<T>::to(q[(int64_t)g * a.q_strides[1]]);
-      if (x < 0.f)
-        lo += x;
-      else
-        hi += x;  // NaN too: every score becomes NaN
-    }
-    qs[0][d] = lo;
-    qs[1][d] = hi;
-  }
-  __syncthreads();
-  // Scores: 8 lanes a page, 4 pages a warp.
-  const int32_t* row = bt.table + (int64_t)ut.b * bt.table_stride;
-  const int sub = lane & 7;
-  for (int p0 = warp * 4; p0 < nvis; p0 += kSelThreads / 8) {
-    const int p = p0 + (lane >> 3);
-    const bool forced = p < a.first || p > last - a.recent;
-    int page = p < nvis && !forced ? __ldg(row + p) : -1;
-    if (page >= bt.num_pages || (page < 0 && p < nvis && !forced)) {
-      record_error(err, SA_DEV_ERR_INDEX);
-      page = -1;
-    }
-    double s = 0.;
-    const T* bp = reinterpret_cast<const T*>(a.bounds) + (int64_t)max(page, 0) * a.b_strides[0] +
-                  (int64_t)kvh * a.b_strides[1];
-    if (page >= 0) {
+  if (!unit_tokens(bt, blockIdx.x, tq, err, ut)) return;
+  const int nall = min((ut.pos0 + ut.n - 1) / ps, W - 1) + 1;  // pages that the last token sees
+  const int32_t* trow = bt.table + (int64_t)ut.b * bt.table_stride;
+  const T* bounds = reinterpret_cast<const T*>(a.bounds) + (int64_t)kvh * a.b_strides[1];
+  auto exact_key = [&](int p, int t) {  // page p's score for token t in 64 bits, as a key
+    const int page = __ldg(trow + p);
+    double s = -INFINITY;  // a bad page ranks lowest
+    if (page >= 0 && page < bt.num_pages)
+      s = page_score<T, D>(bounds + (int64_t)page * a.b_strides[0], a.b_strides[2], qd + t * 2 * D, lane);
+    return order_key(s);
+  };
+
+  if (nall > a.keep) {
+    // Q of the tile's tokens, a warp each.
+    for (int t = warp; t < kSelTokens; t += kSelWarps) {
+      double x[2 * D / 32];
+      float top = 0.f;
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        const int d0 = (c * 8 + sub) * 8;
-        const uint4 lo = *reinterpret_cast<const uint4*>(bp + d0);
-        const uint4 hi = *reinterpret_cast<const uint4*>(bp + a.b_strides[2] + d0);
-        const uint32_t lw[4] = {lo.x, lo.y, lo.z, lo.w}, hw[4] = {hi.x, hi.y, hi.z, hi.w};
+      for (int e = 0; e < D / 32; ++e) x[e] = x[D / 32 + e] = 0.;
+      if (t < ut.n) {
+        const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)(ut.t0 + t) * a.q_strides[0] +
+                     (int64_t)kvh * G * a.q_strides[1];
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 l = Half<T>::unpack(lw[i]), h = Half<T>::unpack(hw[i]);
-          s = fma(qs[0][d0 + 2 * i], (double)l.x, s);
-          s = fma(qs[1][d0 + 2 * i], (double)h.x, s);
-          s = fma(qs[0][d0 + 2 * i + 1], (double)l.y, s);
-          s = fma(qs[1][d0 + 2 * i + 1], (double)h.y, s);
-        }
-      }
-    }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (s != s) {
-      // An infinite bound met a factor of 0, which leaves it out of the maximum
-      // (uniform over the page's 8 lanes; every lane sums the whole page).
-      s = 0.;
-      for (int d = 0; d < D; ++d) {
-        if (qs[0][d] != 0.) s = fma(qs[0][d], (double)Half<T>::to(bp[d]), s);
-        if (qs[1][d] != 0.) s = fma(qs[1][d], (double)Half<T>::to(bp[a.b_strides[2] + d]), s);
-      }
-    }
-    if (sub == 0 && p < nvis) keys[p] = forced ? ~0ull : (page < 0 ? 0ull : order_key(s));
-  }
-  __syncthreads();
-  // The keep-th largest key: 8 bits a pass from the top. Keys whose top bits
-  // exceed `prefix` are in; `left` more come from those that equal it.
-  uint64_t prefix = 0;
-  int left = a.keep, shift = 64;
-  bool exact = false;
-  while (shift > 0 && !exact) {
-    shift -= 8;
-    hist[tid] = 0;
-    __syncthreads();
-    for (int p = tid; p < nvis; p += kSelThreads)
-      if (shift == 56 || (keys[p] >> (shift + 8)) == prefix) atomicAdd(&hist[(keys[p] >> shift) & 255], 1);
-    __syncthreads();
-    if (warp == 0) {
-      // Lane l holds buckets 255 - 8 l .. 248 - 8 l, from the top.
-      int c[8], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum += c[i] = hist[255 - 8 * lane - i];
-      int before = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += y;
-      }
-      before -= sum;
-      if (before < left && before + sum >= left) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (before < left && before + c[i] >= left) {
-            s_bucket = 255 - 8 * lane - i;
-            s_above = before;
+          for (int e = 0; e < D / 32; ++e) {
+            const float v = Half<T>::to(q[(int64_t)g * a.q_strides[1] + e * 32 + lane]);
+            if (v < 0.f)
+              x[e] += v;
+            else
+              x[D / 32 + e] += v;  // NaN too
           }
-          before += c[i];
+#pragma unroll
+        for (int e = 0; e < 2 * D / 32; ++e) {
+          qd[t * 2 * D + e * 32 + lane] = x[e];
+          top = max_nan(top, fabsf((float)x[e]));
         }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kAll, top, o));
+      // Scaled to a largest value in [2^13, 2^14).
+      const bool fine = top < 1e38f;
+      const int ex = fine && top > 0.f ? ilogbf(top) : 0;
+      if (lane == 0) {
+        s_amax[t] = 0;
+        s_wild[t] = !fine;
+      }
+#pragma unroll
+      for (int e = 0; e < 2 * D / 32; ++e) {
+        const float v = fine ? (float)ldexp(x[e], 13 - ex) : 0.f;
+        const T hi = Half<T>::from(v);
+        T* at = reinterpret_cast<T*>(smem + t * Cfg::kRow) + e * 32 + lane;
+        at[0] = hi;
+        at[Cfg::kPart / 2] = Half<T>::from(v - Half<T>::to(hi));
+        at[Cfg::kPart] = Half<T>::from(fabsf(v) + 0.001953125f);
       }
     }
     __syncthreads();
-    const int bucket = s_bucket;
-    left -= s_above;
-    exact = hist[bucket] == left;
-    prefix = (prefix << 8) | (uint64_t)bucket;
+    // Scores. Lane (r, j) = (lane / 4, lane % 4) loads 16 bytes of pages r and r + 8
+    // per 32 channels; the channels of a k-step are permuted alike in both operands.
+    const int j = lane & 3;
+    for (int p0 = warp * 16; p0 < nall; p0 += kSelWarps * 16) {
+      const T* src[2];
+      bool have[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int p = p0 + (lane >> 2) + 8 * i;
+        const int page = p < nall ? __ldg(trow + p) : -1;
+        have[i] = page >= 0 && page < bt.num_pages;
+        if (p < nall && !have[i]) record_error(err, SA_DEV_ERR_INDEX);
+        src[i] = bounds + (int64_t)(have[i] ? page : 0) * a.b_strides[0] + j * 8;
+      }
+      float hi[4] = {0.f, 0.f, 0.f, 0.f}, lo[4] = {0.f, 0.f, 0.f, 0.f}, ab[4] = {0.f, 0.f, 0.f, 0.f};
+      uint4 x[2][D / 32][2];
+#pragma unroll
+      for (int side = 0; side < 2; ++side)
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            x[side][c][i] = have[i] ? __ldg(reinterpret_cast<const uint4*>(src[i] + side * a.b_strides[2] + c * 32))
+                                    : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int side = 0; side < 2; ++side)
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          const uint8_t* qp = smem + (lane >> 2) * Cfg::kRow + (side * D + c * 32 + j * 8) * 2;
+          const uint4 qh = *reinterpret_cast<const uint4*>(qp);
+          const uint4 ql = *reinterpret_cast<const uint4*>(qp + Cfg::kPart);
+          const uint4 qa = *reinterpret_cast<const uint4*>(qp + 2 * Cfg::kPart);
+          const uint4 u = x[side][c][0], v = x[side][c][1];
+          constexpr uint32_t M = 0x7fff7fffu;
+          Half<T>::mma(hi, u.x, v.x, u.y, v.y, qh.x, qh.y);
+          Half<T>::mma(lo, u.x, v.x, u.y, v.y, ql.x, ql.y);
+          Half<T>::mma(ab, u.x & M, v.x & M, u.y & M, v.y & M, qa.x, qa.y);
+          Half<T>::mma(hi, u.z, v.z, u.w, v.w, qh.z, qh.w);
+          Half<T>::mma(lo, u.z, v.z, u.w, v.w, ql.z, ql.w);
+          Half<T>::mma(ab, u.z & M, v.z & M, u.w & M, v.w & M, qa.z, qa.w);
+        }
+      // Element 2 i + e: page r + 8 i, token 2 j + e.
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int t = 2 * j + e;
+        if (t >= ut.n) continue;
+        const int last = min((ut.pos0 + t) / ps, W - 1);
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int p = p0 + (lane >> 2) + 8 * i;
+          if (p > last) continue;
+          uint32_t k = 0;  // a bad page ranks lowest
+          if (p < a.first || p > last - a.recent) {
+            k = kAll;
+          } else if (have[i]) {
+            k = order_key(hi[2 * i + e] + lo[2 * i + e]);
+            top = max_nan(top, ab[2 * i + e]);
+          }
+          keys[(int64_t)t * W + p] = (uint64_t)k << 32;
+        }
+        if (!(top < 3e38f)) s_wild[t] = 1;
+        else atomicMax(&s_amax[t], __float_as_int(top));
+      }
+    }
     __syncthreads();
   }
-  // Kept indexes in ascending order; of equal keys the lowest `left`.
-  int base = 0, eq_base = 0;
-  for (int p0 = 0; p0 < nvis && base < a.keep; p0 += kSelThreads) {
-    const int p = p0 + tid;
-    const uint64_t top = p < nvis ? keys[p] >> shift : 0;
-    const bool eq = p < nvis && top == prefix;
-    int n_eq;
-    const int r_eq = block_rank(eq, warp_cnt, n_eq);
-    const bool in = p < nvis && (top > prefix || (eq && eq_base + r_eq < left));
-    int n_in;
-    const int r = block_rank(in, warp_cnt, n_in);
-    if (in) out[base + r] = p;
-    base += n_in;
-    eq_base += n_eq;
+  // Selection: a warp a token, or the CTA's warps together for a single one.
+  constexpr int GW = ONE ? kSelWarps : 1;  // warps per row
+  for (int t = ONE ? 0 : warp; t < ut.n; t += kSelWarps) {
+    int32_t* out = a.out + (int64_t)(ut.t0 + t) * a.out_strides[0] + (int64_t)kvh * a.out_strides[1];
+    const int last = min((ut.pos0 + t) / ps, W - 1), nvis = last + 1;
+    const int gl = ONE ? tid : lane;  // lane of the group
+    if (nvis <= a.keep) {
+      for (int i = gl; i < a.keep; i += 32 * GW) out[i] = i < nvis ? i : -1;
+      continue;
+    }
+    uint64_t* row = keys + (int64_t)t * W;
+    MidList& mid = s_mid[ONE ? 0 : warp];
+    const int need = a.keep - a.first - a.recent;  // of the pages that compete: [first, nvis - recent)
+    // This warp's part of the competing pages, the first kSelRegs * 32 in registers.
+    const int span = ((nvis - a.recent - a.first + GW * 32 - 1) / (GW * 32)) * 32;
+    const int b0 = a.first + (ONE ? warp * span : 0), b1 = min(nvis - a.recent, b0 + span);
+    auto key = [&](int p) { return (uint32_t)(row[p] >> 32); };
+    uint32_t kr[kSelRegs];
+#pragma unroll
+    for (int i = 0; i < kSelRegs; ++i) kr[i] = b0 + i * 32 + lane < b1 ? key(b0 + i * 32 + lane) : 0u;
+    // f(key) over the warp's pages.
+    auto each = [&](auto f) {
+#pragma unroll
+      for (int i = 0; i < kSelRegs; ++i)
+        if (b0 + i * 32 < b1) {
+          if (b0 + i * 32 + lane < b1) f(kr[i]);
+        }
+      for (int p = b0 + kSelRegs * 32 + lane; p < b1; p += 32) f(key(p));
+    };
+    int turn = 0;
+    auto join = [&](uint32_t v, auto op) {  // over the group's warps; s_part has three turns
+      if constexpr (ONE) {
+        uint32_t* part = s_part[turn];
+        turn = turn == 2 ? 0 : turn + 1;
+        if (lane == 0) part[warp] = v;
+        __syncthreads();
+        v = part[0];
+#pragma unroll
+        for (int w = 1; w < kSelWarps; ++w) v = op(v, part[w]);
+      }
+      return v;
+    };
+    auto sum = [&](int c) {
+      return (int)join(__reduce_add_sync(kAll, (unsigned)c), [](uint32_t x, uint32_t y) { return x + y; });
+    };
+    auto group_sync = [&]() {
+      if constexpr (ONE)
+        __syncthreads();
+      else
+        __syncwarp();
+    };
+
+    uint64_t bar = ~0ull;  // in: row[p] > bar, and the first `ties` that equal it
+    int ties = 0;
+    if (need > 0) {
+      uint32_t from = 0, above = kAll;  // keys above `above` are in, from..above have to be summed again
+      int n_from = 0;                   // keys >= from
+      if (!s_wild[t]) {
+        uint32_t kmax = 0, kmin = kAll;
+        each([&](uint32_t k) {
+          kmax = max(kmax, k);
+          kmin = min(kmin, k);
+        });
+        kmax = join(__reduce_max_sync(kAll, kmax), [](uint32_t x, uint32_t y) { return max(x, y); });
+        kmin = join(__reduce_min_sync(kAll, kmin), [](uint32_t x, uint32_t y) { return min(x, y); });
+        // The largest bound that `need` keys reach, from the first bit that differs on.
+        const int bits = 32 - __clz(kmax ^ kmin);
+        uint32_t v = bits == 32 ? 0u : (kmax >> bits) << bits;
+        for (int b = bits - 1; b >= 0; --b) {
+          const uint32_t cand = v | (1u << b);
+          int c = 0;
+          each([&](uint32_t k) { c += k >= cand ? 1 : 0; });
+          c = sum(c);
+          if (c >= need) v = cand;
+          if (c == need) break;
+        }
+        uint32_t kth = kAll;  // the smallest key that reaches it
+        each([&](uint32_t k) { kth = k >= v ? min(kth, k) : kth; });
+        kth = join(__reduce_min_sync(kAll, kth), [](uint32_t x, uint32_t y) { return min(x, y); });
+        const float th = key_value(kth), eps2 = __int_as_float(s_amax[t]) * (2.f / 16384.f);
+        from = kth ? order_key(th - eps2) : 0u;
+        above = kth ? order_key(th + eps2) : 0u;
+      }
+      int n_above = 0;
+      each([&](uint32_t k) {
+        n_from += k >= from ? 1 : 0;
+        n_above += k > above ? 1 : 0;
+      });
+      n_from = sum(n_from);
+      n_above = sum(n_above);
+      if (n_from == need) {
+        bar = (uint64_t)from << 32;
+        ties = 0x7fffffff;
+      } else {
+        const int n_mid = n_from - n_above;
+        const bool few = n_mid <= kSelMid;
+        if (gl == 0) mid.n = 0;
+        group_sync();
+        for (int p0 = b0; p0 < b1; p0 += 32) {
+          const int p = p0 + lane;
+          const uint32_t k = p < b1 ? key(p) : 0u;
+          const bool is_mid = p < b1 && k >= from && k <= above;
+          if (p < b1 && !is_mid) row[p] = k > above ? ~0ull : 0ull;
+          unsigned m = __ballot_sync(kAll, is_mid);
+          if (few) {
+            if (is_mid) mid.at[atomicAdd(&mid.n, 1)] = p;
+            continue;
+          }
+          while (m) {
+            const int q = p0 + __ffs(m) - 1;
+            m &= m - 1;
+            const uint64_t x = exact_key(q, t);
+            if (lane == 0) row[q] = x;
+          }
+        }
+        group_sync();
+        if (few) {
+          // Rank the candidates among themselves; ties to the lower index.
+          for (int i = ONE ? warp : 0; i < n_mid; i += GW) {
+            const uint64_t x = exact_key(mid.at[i], t);
+            if (lane == 0) mid.key[i] = x;
+          }
+          group_sync();
+          for (int i = gl; i < n_mid; i += 32 * GW) {
+            int rank = n_above;
+            const uint64_t x = mid.key[i];
+            const int p = mid.at[i];
+            for (int o = 0; o < n_mid; ++o) {
+              const uint64_t y = mid.key[o];
+              rank += y > x || (y == x && mid.at[o] < p) ? 1 : 0;
+            }
+            row[p] = rank < need ? ~0ull : 0ull;
+          }
+          group_sync();
+          bar = 1;
+        } else {
+          uint64_t v = 0;
+          bool whole = false;
+          auto count = [&](uint64_t x) {
+            int c = 0;
+            for (int p = b0 + lane; p < b1; p += 32) c += row[p] >= x ? 1 : 0;
+            return sum(c);
+          };
+          for (int b = 63; b >= 0 && !whole; --b) {
+            const uint64_t cand = v | (1ull << b);
+            const int c = count(cand);
+            if (c >= need) v = cand;
+            whole = c == need;
+          }
+          bar = v;
+          ties = whole ? 0x7fffffff : need - count(v + 1);
+        }
+      }
+    }
+    // Kept indexes in ascending order: the first pages, then each warp's, then the last.
+    const unsigned below = (1u << lane) - 1;
+    int base = a.first, eq_before = 0;
+    if constexpr (ONE) {
+      int c = 0, e = 0;
+      for (int p = b0 + lane; p < b1; p += 32) {
+        c += row[p] > bar ? 1 : 0;
+        e += row[p] == bar ? 1 : 0;
+      }
+      c = __reduce_add_sync(kAll, c);
+      e = __reduce_add_sync(kAll, e);
+      __syncthreads();  // the last join's part may still be read
+      if (lane == 0) {
+        s_part[0][warp] = c;
+        s_part[1][warp] = e;
+      }
+      __syncthreads();
+      for (int w = 0; w < warp; ++w) {
+        base += s_part[0][w] + min((int)s_part[1][w], max(0, ties - eq_before));
+        eq_before += s_part[1][w];
+      }
+    }
+    for (int i = gl; i < a.first + a.recent; i += 32 * GW)
+      out[i < a.first ? i : a.keep - a.recent + (i - a.first)] = i < a.first ? i : nvis - a.recent + (i - a.first);
+    if (need > 0)
+      for (int p0 = b0; p0 < b1; p0 += 32) {
+        const int p = p0 + lane;
+        const uint64_t k = p < b1 ? row[p] : 0ull;
+        const bool eq = p < b1 && k == bar;
+        const unsigned me = __ballot_sync(kAll, eq);
+        const bool in = p < b1 && (k > bar || (eq && eq_before + __popc(me & below) < ties));
+        const unsigned mi = __ballot_sync(kAll, in);
+        if (in) out[base + __popc(mi & below)] = p;
+        base += __popc(mi);
+        eq_before += __popc(me);
+      }
   }
 }
 
 template <typename T, int D>
 static int launch_select(const sa_paged_select_args& a, cudaStream_t stream) {
-  const int bytes = a.batch.max_pages * 8;
-  SA_CHECK_CUDA(cudaFuncSetAttribute(paged_select_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     kSelMaxPages * 8));
-  paged_select_kernel<T, D>
-      <<<dim3(a.batch.N, a.Hkv), kSelThreads, bytes, stream>>>(a, sa_device_error_ptr());
+  using Cfg = SelectCfg<T, D>;
+  // Tokens per CTA: the keys of all of them within 64 KB, so that three CTAs fit on an SM.
+  int tq = a.max_q < kSelTokens ? a.max_q : kSelTokens;
+  if ((int64_t)tq * a.batch.max_pages * 8 > 65536) tq = 65536 / (a.batch.max_pages * 8);
+  if (tq < 1) tq = 1;
+  const int64_t units = unit_count(a.batch.N, a.batch.B, tq);
+  if (units > 0x7fffffff) return sa_fail(SA_ERR_INVALID, "paged select: batch too large");
+  const int bytes = Cfg::kKeys + tq * a.batch.max_pages * 8;
+  static bool done[2][64];
+  auto kern = tq == 1 ? paged_select_kernel<T, D, true> : paged_select_kernel<T, D, false>;
+  int rc = sa_smem_once(reinterpret_cast<const void*>(kern), Cfg::kKeys + kSelMaxPages * 8, done[tq == 1]);
+  if (rc) return rc;
+  kern<<<dim3((unsigned)units, a.Hkv), kSelThreads, bytes, stream>>>(a, tq, sa_device_error_ptr());
   SA_CHECK_CUDA(cudaGetLastError());
   return SA_OK;
 }
@@ -207,6 +457,7 @@ extern "C" int sa_paged_select(const sa_paged_select_args* a, sa_stream_t stream
   if (a->dtype != SA_BF16 && a->dtype != SA_FP16) return sa_fail(SA_ERR_UNSUPPORTED, "dtype %d unknown", a->dtype);
   if (a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->Hkv > 65535)
     return sa_fail(SA_ERR_INVALID, "Hq=%d not a multiple of Hkv=%d", a->Hq, a->Hkv);
+  if (a->max_q < 1) return sa_fail(SA_ERR_INVALID, "max_q must be at least 1");
   if (a->first < 0 || a->recent < 1 || a->keep < 1 || a->keep > kSelMaxKeep ||
       (int64_t)a->first + a->recent > a->keep)
     return sa_fail(SA_ERR_INVALID, "need first >= 0, recent >= 1, first + recent <= keep <= %d (got %d, %d, %d)",

@@ -452,57 +452,61 @@ def topk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: int
 _HALF = {torch.bfloat16: _capi.SA_BF16, torch.float16: _capi.SA_FP16}
 
 
-def _paged_check(name: str, ref: torch.Tensor, halves, ints) -> int:
-    """Device, type and layout of a paged op's tensors; returns the type's code."""
-    dev = ref.device
-    if dev.type != "cuda":
+def _paged_check(name: str, dtype: torch.dtype, dev: int, halves, ints) -> None:
+    """Type, device and layout of a paged op's tensors: 16-bit ones of ``dtype``,
+    int32 ones, all on device ``dev`` with a contiguous last dimension."""
+    for want, ts in ((dtype, halves), (torch.int32, ints)):
+        for t in ts:
+            if t.dtype is not want or t.get_device() != dev:
+                raise TypeError(f"{name}: {want} on cuda:{dev} expected, got {t.dtype} on {t.device}")
+            if t.stride(-1) != 1 and t.shape[-1] > 1:
+                raise ValueError(f"{name}: the last dimension of every tensor must be contiguous, got strides "
+                                 f"{t.stride()} of {tuple(t.shape)}")
+
+
+def _paged_dtype(name: str, t: torch.Tensor) -> int:
+    if not t.is_cuda:
         raise RuntimeError("cuda_sparse_attention ops need CUDA tensors (there is no CPU path)")
-    code = _HALF.get(ref.dtype)
+    code = _HALF.get(t.dtype)
     if code is None:
-        raise TypeError(f"{name}: bf16 or fp16 tensors expected, got {ref.dtype}")
-    for n, t in halves:
-        if t.dtype != ref.dtype or t.device != dev:
-            raise TypeError(f"{name}: {n} must be {ref.dtype} on {dev}, got {t.dtype} on {t.device}")
-        if t.stride(-1) != 1:
-            raise ValueError(f"{name}: the last dimension of {n} must be contiguous")
-    for n, t in ints:
-        if t.dtype != torch.int32 or t.device != dev:
-            raise TypeError(f"{name}: {n} must be int32 on {dev}, got {t.dtype} on {t.device}")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
-            raise ValueError(f"{name}: the last dimension of {n} must be contiguous")
+        raise TypeError(f"{name}: bf16 or fp16 tensors expected, got {t.dtype}")
     return code
 
 
-def _paged_strides(dst, t: torch.Tensor, dims: Sequence[int]) -> None:
-    """Element strides of ``dims``; a dimension of one element gets the stride it
-    would have in a contiguous tensor (torch leaves any value there)."""
-    shape, strides = t.shape, t.stride()
-    for i, d in enumerate(dims):
-        s = strides[d]
-        if shape[d] == 1:
-            s = 1
-            for e in shape[d + 1:]:
-                s *= e
-        dst[i] = s
+def _outer(t: torch.Tensor, n: int) -> tuple[int, ...]:
+    """Element strides of the first n dimensions; one of a single element gets the
+    stride of a contiguous tensor (torch leaves any value there)."""
+    s, shape = t.stride(), t.shape
+    if 1 not in shape[:n]:
+        return s[:n]
+    return tuple(math.prod(shape[i + 1:]) if shape[i] == 1 else s[i] for i in range(n))
 
 
-def _fill_batch(b: _capi.PagedBatch, N: int, page_table, cu_q, seq_lens, num_pages: int, page_size: int) -> None:
-    if page_table.dim() != 2 or cu_q.dim() != 1 or seq_lens.dim() != 1:
-        raise ValueError("page_table [B, pages], cu_q [B + 1], seq_lens [B]")
-    B = seq_lens.shape[0]
-    if page_table.shape[0] != B or cu_q.shape[0] != B + 1:
-        raise ValueError(f"page_table {tuple(page_table.shape)} and cu_q {tuple(cu_q.shape)} do not fit "
-                         f"seq_lens {tuple(seq_lens.shape)}")
-    b.table, b.cu_q, b.seq_lens = page_table.data_ptr(), cu_q.data_ptr(), seq_lens.data_ptr()
-    b.max_pages = page_table.shape[1]
-    b.table_stride = page_table.stride(0) if B > 1 else page_table.shape[1]
-    b.B, b.N, b.num_pages, b.page_size = B, N, num_pages, page_size
+def _paged_batch(name: str, N: int, page_table, cu_q, seq_lens, num_pages: int, page_size: int) -> tuple:
+    B = seq_lens.numel()
+    if page_table.dim() != 2 or seq_lens.dim() != 1 or cu_q.shape != (B + 1,) or page_table.shape[0] != B:
+        raise ValueError(f"{name}: page_table [B, pages], cu_q [B + 1] and seq_lens [B] expected, got "
+                         f"{tuple(page_table.shape)}, {tuple(cu_q.shape)} and {tuple(seq_lens.shape)}")
+    width = page_table.shape[1]
+    return (page_table.data_ptr(), cu_q.data_ptr(), seq_lens.data_ptr(), page_table.stride(0) if B > 1 else width, B,
+            N, width, num_pages, page_size)
 
 
 def _check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, Hkv: int, D: int) -> None:
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or k_pages.shape[1] != Hkv or k_pages.shape[3] != D:
         raise ValueError(f"{name}: k_pages / v_pages must be [pages, {Hkv}, page_size, {D}], got "
                          f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+
+
+def _paged_call(fn, args: bytes, dev: int) -> None:
+    """fn(args, current stream of device dev), with that device current."""
+    if torch.cuda.current_device() == dev:
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _capi.check(rc)
 
 
 def paged_qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
@@ -526,44 +530,36 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor | None, 
     the call can be captured; what they must satisfy is stated in
     sparse_attn_b200.h, and a violation sets the device error word."""
     name = "paged_qk_norm_rope_append"
+    code = _paged_dtype(name, qkv)
     if qkv.dim() != 3 or qkv.shape[1] != Hq + 2 * Hkv:
         raise ValueError(f"{name}: qkv must be [N, {Hq}+2*{Hkv}, D], got {tuple(qkv.shape)}")
-    N, _, D = qkv.shape
+    N, heads, D = qkv.shape
+    dev = qkv.get_device()
     if q_out is None:
         q_out = torch.empty(N, Hq, D, dtype=qkv.dtype, device=qkv.device)
-    halves = [("qkv", qkv), ("cos", cos), ("sin", sin), ("k_pages", k_pages), ("v_pages", v_pages), ("q_out", q_out)]
-    halves += [(n, t) for n, t in (("q_weight", q_weight), ("k_weight", k_weight), ("k_bounds", k_bounds))
-               if t is not None]
-    code = _paged_check(name, qkv, halves,
-                        [("page_table", page_table), ("cu_q", cu_q), ("seq_lens", seq_lens)])
+    _paged_check(name, qkv.dtype, dev,
+                 [t for t in (qkv, cos, sin, k_pages, v_pages, q_out, q_weight, k_weight, k_bounds) if t is not None],
+                 (page_table, cu_q, seq_lens))
     _check_pages(name, k_pages, v_pages, Hkv, D)
     if qkv.stride(1) != D or q_out.shape != (N, Hq, D):
         raise ValueError(f"{name}: qkv heads must be contiguous and q_out [N, Hq, D]")
     if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != D or not cos.is_contiguous() or \
             not sin.is_contiguous():
         raise ValueError(f"{name}: cos / sin must be contiguous [positions, {D}]")
-    if any(w is not None and w.shape != (D,) for w in (q_weight, k_weight)):
+    if (q_weight is not None and q_weight.shape != (D,)) or (k_weight is not None and k_weight.shape != (D,)):
         raise ValueError(f"{name}: weights must be [{D}]")
-    if N == 0 or seq_lens.numel() == 0:
+    if k_bounds is not None and k_bounds.shape != (k_pages.shape[0], Hkv, 2, D):
+        raise ValueError(f"{name}: k_bounds must be [pages, {Hkv}, 2, {D}], got {tuple(k_bounds.shape)}")
+    batch = _paged_batch(name, N, page_table, cu_q, seq_lens, k_pages.shape[0], k_pages.shape[2])
+    if N == 0 or batch[4] == 0:
         return q_out
-    a = _capi.PagedAppendArgs()
-    _fill_batch(a.batch, N, page_table, cu_q, seq_lens, k_pages.shape[0], k_pages.shape[2])
-    a.qkv, a.qkv_st = qkv.data_ptr(), qkv.stride(0) if N > 1 else (Hq + 2 * Hkv) * D
-    a.q_weight = q_weight.data_ptr() if q_weight is not None else None
-    a.k_weight = k_weight.data_ptr() if k_weight is not None else None
-    a.cos, a.sin, a.q_out = cos.data_ptr(), sin.data_ptr(), q_out.data_ptr()
-    a.k_pages, a.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
-    _paged_strides(a.q_strides, q_out, (0, 1))
-    _paged_strides(a.k_strides, k_pages, (0, 1, 2))
-    _paged_strides(a.v_strides, v_pages, (0, 1, 2))
-    if k_bounds is not None:
-        if k_bounds.shape != (k_pages.shape[0], Hkv, 2, D):
-            raise ValueError(f"{name}: k_bounds must be [pages, {Hkv}, 2, {D}], got {tuple(k_bounds.shape)}")
-        a.bounds = k_bounds.data_ptr()
-        _paged_strides(a.b_strides, k_bounds, (0, 1, 2))
-    a.Hq, a.Hkv, a.D, a.positions, a.dtype, a.eps = Hq, Hkv, D, cos.shape[0], code, float(eps)
-    with torch.cuda.device(qkv.device):
-        _capi.check(_capi.load().sa_paged_append(ctypes.byref(a), _stream(qkv.device)))
+    args = _capi.PAGED_APPEND.pack(
+        *batch, qkv.data_ptr(), qkv.stride(0) if N > 1 else heads * D,
+        q_weight.data_ptr() if q_weight is not None else 0, k_weight.data_ptr() if k_weight is not None else 0,
+        cos.data_ptr(), sin.data_ptr(), q_out.data_ptr(), *_outer(q_out, 2), k_pages.data_ptr(), *_outer(k_pages, 3),
+        v_pages.data_ptr(), *_outer(v_pages, 3), k_bounds.data_ptr() if k_bounds is not None else 0,
+        *(_outer(k_bounds, 3) if k_bounds is not None else (0, 0, 0)), Hq, Hkv, D, cos.shape[0], code, eps)
+    _paged_call(_capi.load().sa_paged_append, args, dev)
     return q_out
 
 
@@ -581,31 +577,68 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, page_table: torc
     tensors as in paged_qk_norm_rope_append; ``max_q`` (most new tokens of one
     sequence) only steers the launch."""
     name = "paged_block_select"
+    code = _paged_dtype(name, q)
     if q.dim() != 3 or k_bounds.dim() != 4 or k_bounds.shape[2] != 2 or k_bounds.shape[3] != q.shape[2]:
         raise ValueError(f"{name}: q [N, Hq, D] and k_bounds [pages, Hkv, 2, D], got {tuple(q.shape)} and "
                          f"{tuple(k_bounds.shape)}")
     N, Hq, D = q.shape
-    Hkv = k_bounds.shape[1]
+    pages, Hkv = k_bounds.shape[:2]
+    dev = q.get_device()
     if out is None:
         out = torch.empty(N, Hkv, keep, dtype=torch.int32, device=q.device)
-    code = _paged_check(name, q, [("q", q), ("k_bounds", k_bounds)],
-                        [("page_table", page_table), ("cu_q", cu_q), ("seq_lens", seq_lens), ("out", out)])
+    _paged_check(name, q.dtype, dev, (q, k_bounds), (page_table, cu_q, seq_lens, out))
     if out.shape != (N, Hkv, keep):
         raise ValueError(f"{name}: out must be [{N}, {Hkv}, {keep}], got {tuple(out.shape)}")
-    if N == 0 or seq_lens.numel() == 0:
+    batch = _paged_batch(name, N, page_table, cu_q, seq_lens, pages, page_size)
+    if N == 0 or batch[4] == 0:
         return out
-    a = _capi.PagedSelectArgs()
-    _fill_batch(a.batch, N, page_table, cu_q, seq_lens, k_bounds.shape[0], page_size)
-    a.q, a.bounds, a.out = q.data_ptr(), k_bounds.data_ptr(), out.data_ptr()
-    _paged_strides(a.q_strides, q, (0, 1))
-    _paged_strides(a.b_strides, k_bounds, (0, 1, 2))
-    _paged_strides(a.out_strides, out, (0, 1))
-    a.Hq, a.Hkv, a.D, a.dtype = Hq, Hkv, D, code
-    a.keep, a.first, a.recent = keep, first, recent
-    a.max_q = int(max_q) if max_q is not None else N
-    with torch.cuda.device(q.device):
-        _capi.check(_capi.load().sa_paged_select(ctypes.byref(a), _stream(q.device)))
+    args = _capi.PAGED_SELECT.pack(*batch, q.data_ptr(), *_outer(q, 2), k_bounds.data_ptr(), *_outer(k_bounds, 3),
+                                   out.data_ptr(), *_outer(out, 2), Hq, Hkv, D, code, keep, first, recent,
+                                   N if max_q is None else max_q)
+    _paged_call(_capi.load().sa_paged_select, args, dev)
     return out
+
+
+def _paged_attn_args(name, q, k_pages, v_pages, page_table, cu_q, seq_lens, out, max_q, max_len, blocks, scale,
+                     split_len):
+    """Packed arguments of sa_paged_attn (workspace last), or None for an empty batch."""
+    code = _paged_dtype(name, q)
+    if q.dim() != 3 or k_pages.dim() != 4 or out.shape != q.shape:
+        raise ValueError(f"{name}: q and out [N, Hq, D] and pages of 4 dimensions expected, got {tuple(q.shape)}, "
+                         f"{tuple(out.shape)} and {tuple(k_pages.shape)}")
+    N, Hq, D = q.shape
+    pages, Hkv, page_size = k_pages.shape[:3]
+    dev = q.get_device()
+    _paged_check(name, q.dtype, dev, (q, k_pages, v_pages, out),
+                 (page_table, cu_q, seq_lens) if blocks is None else (page_table, cu_q, seq_lens, blocks))
+    _check_pages(name, k_pages, v_pages, Hkv, D)
+    if blocks is not None and (blocks.dim() != 3 or blocks.shape[:2] != (N, Hkv)):
+        raise ValueError(f"{name}: blocks must be [{N}, {Hkv}, n], got {tuple(blocks.shape)}")
+    batch = _paged_batch(name, N, page_table, cu_q, seq_lens, pages, page_size)
+    if N == 0 or batch[4] == 0:
+        return None
+    return (*batch, q.data_ptr(), out.data_ptr(), *_outer(q, 2), *_outer(out, 2), k_pages.data_ptr(),
+            *_outer(k_pages, 3), v_pages.data_ptr(), *_outer(v_pages, 3),
+            *((0, 0, 0, 0) if blocks is None else (blocks.data_ptr(), *_outer(blocks, 2), blocks.shape[2])),
+            Hq, Hkv, D, code, 1.0 / math.sqrt(D) if scale is None else scale, N if max_q is None else max_q,
+            page_table.shape[1] * page_size if max_len is None else max_len, 0 if split_len is None else split_len,
+            _num_sms(q.device))
+
+
+def _paged_workspace(args, dev: int) -> int:
+    n = ctypes.c_int64(0)
+    _capi.check(_capi.load().sa_paged_attn_workspace(_capi.PAGED_ATTN.pack(*args, 0), ctypes.byref(n)))
+    return n.value
+
+
+def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                              page_table: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor, *,
+                              max_q: int | None = None, max_len: int | None = None,
+                              blocks: torch.Tensor | None = None, split_len: int | None = None) -> int:
+    """float32 elements of workspace that paged_attention with these arguments needs."""
+    args = _paged_attn_args("paged_attention_workspace", q, k_pages, v_pages, page_table, cu_q, seq_lens, q, max_q,
+                            max_len, blocks, None, split_len)
+    return 0 if args is None else _paged_workspace(args, q.get_device())
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -626,75 +659,24 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     buffer of at least paged_attention_workspace(...) elements that a captured
     call keeps to itself (allocated per call when None)."""
     name = "paged_attention"
-    if q.dim() != 3:
-        raise ValueError(f"{name}: q must be [N, Hq, D], got {tuple(q.shape)}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    a = _paged_attn_args(name, q, k_pages, v_pages, page_table, cu_q, seq_lens, out, max_q, max_len, blocks, scale,
-                         split_len)
-    if a is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    args = _paged_attn_args(name, q, k_pages, v_pages, page_table, cu_q, seq_lens, out, max_q, max_len, blocks, scale,
+                            split_len)
+    if args is None:
         return out
-    lib = _capi.load()
-    with torch.cuda.device(q.device):
-        n = ctypes.c_int64(0)
-        _capi.check(lib.sa_paged_attn_workspace(ctypes.byref(a), ctypes.byref(n)))
-        if n.value:
-            if workspace is None:
-                workspace = torch.empty(n.value, dtype=torch.float32, device=q.device)
-            elif workspace.dtype != torch.float32 or workspace.device != q.device or \
-                    not workspace.is_contiguous() or workspace.numel() < n.value:
-                raise ValueError(f"{name}: workspace must be {n.value} contiguous float32 on {q.device}")
-            a.workspace = workspace.data_ptr()
-        _capi.check(lib.sa_paged_attn(ctypes.byref(a), _stream(q.device)))
+    dev = q.get_device()
+    need = _paged_workspace(args, dev)
+    ptr = 0
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.float32, device=q.device)
+        elif workspace.dtype != torch.float32 or workspace.get_device() != dev or not workspace.is_contiguous() or \
+                workspace.numel() < need:
+            raise ValueError(f"{name}: workspace must be {need} contiguous float32 on cuda:{dev}")
+        ptr = workspace.data_ptr()
+    _paged_call(_capi.load().sa_paged_attn, _capi.PAGED_ATTN.pack(*args, ptr), dev)
     return out
-
-
-def _paged_attn_args(name, q, k_pages, v_pages, page_table, cu_q, seq_lens, out, max_q, max_len, blocks, scale,
-                     split_len):
-    N, Hq, D = q.shape
-    ints = [("page_table", page_table), ("cu_q", cu_q), ("seq_lens", seq_lens)]
-    if blocks is not None:
-        ints.append(("blocks", blocks))
-    code = _paged_check(name, q, [("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("out", out)], ints)
-    Hkv = k_pages.shape[1] if k_pages.dim() == 4 else 0
-    _check_pages(name, k_pages, v_pages, Hkv, D)
-    if out.shape != q.shape:
-        raise ValueError(f"{name}: out must be {tuple(q.shape)}, got {tuple(out.shape)}")
-    if blocks is not None and (blocks.dim() != 3 or blocks.shape[:2] != (N, Hkv)):
-        raise ValueError(f"{name}: blocks must be [{N}, {Hkv}, n], got {tuple(blocks.shape)}")
-    if N == 0 or seq_lens.numel() == 0:
-        return None
-    a = _capi.PagedAttnArgs()
-    _fill_batch(a.batch, N, page_table, cu_q, seq_lens, k_pages.shape[0], k_pages.shape[2])
-    a.q, a.out, a.k_pages, a.v_pages = q.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr()
-    _paged_strides(a.q_strides, q, (0, 1))
-    _paged_strides(a.o_strides, out, (0, 1))
-    _paged_strides(a.k_strides, k_pages, (0, 1, 2))
-    _paged_strides(a.v_strides, v_pages, (0, 1, 2))
-    if blocks is not None:
-        a.blocks, a.n_blocks = blocks.data_ptr(), blocks.shape[2]
-        _paged_strides(a.blocks_strides, blocks, (0, 1))
-    a.Hq, a.Hkv, a.D, a.dtype = Hq, Hkv, D, code
-    a.scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    a.max_q = int(max_q) if max_q is not None else N
-    a.max_len = int(max_len) if max_len is not None else page_table.shape[1] * k_pages.shape[2]
-    a.split_len = int(split_len) if split_len is not None else 0
-    a.num_sms = _num_sms(q.device)
-    return a
-
-
-def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                              page_table: torch.Tensor, cu_q: torch.Tensor, seq_lens: torch.Tensor, *,
-                              max_q: int | None = None, max_len: int | None = None,
-                              blocks: torch.Tensor | None = None, split_len: int | None = None) -> int:
-    """float32 elements of workspace that paged_attention with these arguments needs."""
-    a = _paged_attn_args("paged_attention_workspace", q, k_pages, v_pages, page_table, cu_q, seq_lens, q, max_q,
-                         max_len, blocks, None, split_len)
-    if a is None:
-        return 0
-    n = ctypes.c_int64(0)
-    _capi.check(_capi.load().sa_paged_attn_workspace(ctypes.byref(a), ctypes.byref(n)))
-    return n.value
 
 
 def sparse_attn(q, k, v, block_pairs, block_pair_offsets, block_size: int, *, scale: float | None = None):

@@ -206,10 +206,11 @@ def test_select(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, keep, first, rec
     assert _capi.device_error() == 0
 
 
-def test_select_ties_nan_and_infinities():
+@pytest.mark.parametrize("new,ctx", [(1, 64 * 16), (6, 64 * 16), (1, 10000), (3, 10000)])
+def test_select_ties_nan_and_infinities(new, ctx):
     """Equal pages go to the lower index; NaN scores rank with -infinity; 1 ulp decides."""
-    bt = P.Batch([64 * 16], [1], Hq=2, Hkv=1, D=64, page=16, device=DEV)
-    q = torch.randn(1, 2, 64, generator=bt.g).to(torch.bfloat16)
+    bt = P.Batch([ctx], [new], Hq=2, Hkv=1, D=64, page=16, device=DEV)
+    q = torch.randn(new, 2, 64, generator=bt.g).to(torch.bfloat16)
     for case in range(4):
         bounds = torch.ones(bt.pages, 1, 2, 64, dtype=torch.bfloat16)
         if case == 1:  # every second page better by one unit in the last place of one channel
