@@ -94,7 +94,7 @@ struct MidList {
 
 // ONE: a token a CTA, whose warps share its selection.
 template <typename T, int D, bool ONE>
-__global__ void __launch_bounds__(kSelThreads)
+__global__ void __launch_bounds__(kSelThreads, 3)
     paged_select_kernel(const __grid_constant__ sa_paged_select_args a, int tq, int32_t* err) {
   using Cfg = SelectCfg<T, D>;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -150,13 +150,14 @@ __global__ void __launch_bounds__(kSelThreads)
       // Scaled to a largest value in [2^13, 2^14).
       const bool fine = top < 1e38f;
       const int ex = fine && top > 0.f ? ilogbf(top) : 0;
+      const double scale = __longlong_as_double((int64_t)(1023 + 13 - ex) << 52);
       if (lane == 0) {
         s_amax[t] = 0;
         s_wild[t] = !fine;
       }
 #pragma unroll
       for (int e = 0; e < 2 * D / 32; ++e) {
-        const float v = fine ? (float)ldexp(x[e], 13 - ex) : 0.f;
+        const float v = fine ? (float)(x[e] * scale) : 0.f;
         const T hi = Half<T>::from(v);
         T* at = reinterpret_cast<T*>(smem + t * Cfg::kRow) + e * 32 + lane;
         at[0] = hi;
@@ -168,36 +169,40 @@ __global__ void __launch_bounds__(kSelThreads)
     // Scores. Lane (r, j) = (lane / 4, lane % 4) loads 16 bytes of pages r and r + 8
     // per 32 channels; the channels of a k-step are permuted alike in both operands.
     const int j = lane & 3;
+    int page[2];  // read a round ahead
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int p = warp * 16 + (lane >> 2) + 8 * i;
+      page[i] = p < nall ? __ldg(trow + p) : -1;
+    }
     for (int p0 = warp * 16; p0 < nall; p0 += kSelWarps * 16) {
       const T* src[2];
       bool have[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int p = p0 + (lane >> 2) + 8 * i;
-        const int page = p < nall ? __ldg(trow + p) : -1;
-        have[i] = page >= 0 && page < bt.num_pages;
+        const int p = p0 + (lane >> 2) + 8 * i, next = p + kSelWarps * 16;
+        have[i] = page[i] >= 0 && page[i] < bt.num_pages;
         if (p < nall && !have[i]) record_error(err, SA_DEV_ERR_INDEX);
-        src[i] = bounds + (int64_t)(have[i] ? page : 0) * a.b_strides[0] + j * 8;
+        src[i] = bounds + (int64_t)(have[i] ? page[i] : 0) * a.b_strides[0] + j * 8;
+        page[i] = next < nall ? __ldg(trow + next) : -1;
       }
       float hi[4] = {0.f, 0.f, 0.f, 0.f}, lo[4] = {0.f, 0.f, 0.f, 0.f}, ab[4] = {0.f, 0.f, 0.f, 0.f};
-      uint4 x[2][D / 32][2];
 #pragma unroll
-      for (int side = 0; side < 2; ++side)
+      for (int side = 0; side < 2; ++side) {
+        uint4 x[D / 32][2];
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            x[side][c][i] = have[i] ? __ldg(reinterpret_cast<const uint4*>(src[i] + side * a.b_strides[2] + c * 32))
-                                    : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-      for (int side = 0; side < 2; ++side)
+            x[c][i] = have[i] ? __ldg(reinterpret_cast<const uint4*>(src[i] + side * a.b_strides[2] + c * 32))
+                              : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           const uint8_t* qp = smem + (lane >> 2) * Cfg::kRow + (side * D + c * 32 + j * 8) * 2;
           const uint4 qh = *reinterpret_cast<const uint4*>(qp);
           const uint4 ql = *reinterpret_cast<const uint4*>(qp + Cfg::kPart);
           const uint4 qa = *reinterpret_cast<const uint4*>(qp + 2 * Cfg::kPart);
-          const uint4 u = x[side][c][0], v = x[side][c][1];
+          const uint4 u = x[c][0], v = x[c][1];
           constexpr uint32_t M = 0x7fff7fffu;
           Half<T>::mma(hi, u.x, v.x, u.y, v.y, qh.x, qh.y);
           Half<T>::mma(lo, u.x, v.x, u.y, v.y, ql.x, ql.y);
@@ -206,6 +211,7 @@ __global__ void __launch_bounds__(kSelThreads)
           Half<T>::mma(lo, u.z, v.z, u.w, v.w, ql.z, ql.w);
           Half<T>::mma(ab, u.z & M, v.z & M, u.w & M, v.w & M, qa.z, qa.w);
         }
+      }
       // Element 2 i + e: page r + 8 i, token 2 j + e.
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -217,12 +223,10 @@ __global__ void __launch_bounds__(kSelThreads)
         for (int i = 0; i < 2; ++i) {
           const int p = p0 + (lane >> 2) + 8 * i;
           if (p > last) continue;
-          uint32_t k = 0;  // a bad page ranks lowest
-          if (p < a.first || p > last - a.recent) {
-            k = kAll;
-          } else if (have[i]) {
+          uint32_t k = kAll;
+          if (p >= a.first && p <= last - a.recent) {
             k = order_key(hi[2 * i + e] + lo[2 * i + e]);
-            top = max_nan(top, ab[2 * i + e]);
+            top = max_nan(top, have[i] ? ab[2 * i + e] : INFINITY);  // a bad page: the row is summed again whole
           }
           keys[(int64_t)t * W + p] = (uint64_t)k << 32;
         }
@@ -249,15 +253,19 @@ __global__ void __launch_bounds__(kSelThreads)
     const int span = ((nvis - a.recent - a.first + GW * 32 - 1) / (GW * 32)) * 32;
     const int b0 = a.first + (ONE ? warp * span : 0), b1 = min(nvis - a.recent, b0 + span);
     auto key = [&](int p) { return (uint32_t)(row[p] >> 32); };
-    uint32_t kr[kSelRegs];
+    uint32_t kr[kSelRegs];  // 0 behind the part's end; no score's key is 0
+    const int groups = min(kSelRegs / 4, (b1 - b0 + 127) / 128);
 #pragma unroll
     for (int i = 0; i < kSelRegs; ++i) kr[i] = b0 + i * 32 + lane < b1 ? key(b0 + i * 32 + lane) : 0u;
-    // f(key) over the warp's pages.
+    // f(key) over the warp's pages, and over zeros that fill up the registers.
     auto each = [&](auto f) {
 #pragma unroll
-      for (int i = 0; i < kSelRegs; ++i)
-        if (b0 + i * 32 < b1) {
-          if (b0 + i * 32 + lane < b1) f(kr[i]);
+      for (int g = 0; g < kSelRegs / 4; ++g)
+        if (g < groups) {
+          f(kr[4 * g]);
+          f(kr[4 * g + 1]);
+          f(kr[4 * g + 2]);
+          f(kr[4 * g + 3]);
         }
       for (int p = b0 + kSelRegs * 32 + lane; p < b1; p += 32) f(key(p));
     };
@@ -287,16 +295,17 @@ __global__ void __launch_bounds__(kSelThreads)
     uint64_t bar = ~0ull;  // in: row[p] > bar, and the first `ties` that equal it
     int ties = 0;
     if (need > 0) {
-      uint32_t from = 0, above = kAll;  // keys above `above` are in, from..above have to be summed again
-      int n_from = 0;                   // keys >= from
+      // Keys above `above` are in, from..above have to be summed again.
+      uint32_t from = 0, above = kAll;
+      int n_from = nvis - a.recent - a.first, n_above = 0;  // keys >= from, and > above
       if (!s_wild[t]) {
         uint32_t kmax = 0, kmin = kAll;
         each([&](uint32_t k) {
           kmax = max(kmax, k);
-          kmin = min(kmin, k);
+          kmin = min(kmin, k - 1);  // (the zeros go to the top)
         });
         kmax = join(__reduce_max_sync(kAll, kmax), [](uint32_t x, uint32_t y) { return max(x, y); });
-        kmin = join(__reduce_min_sync(kAll, kmin), [](uint32_t x, uint32_t y) { return min(x, y); });
+        kmin = join(__reduce_min_sync(kAll, kmin), [](uint32_t x, uint32_t y) { return min(x, y); }) + 1;
         // The largest bound that `need` keys reach, from the first bit that differs on.
         const int bits = 32 - __clz(kmax ^ kmin);
         uint32_t v = bits == 32 ? 0u : (kmax >> bits) << bits;
@@ -308,20 +317,20 @@ __global__ void __launch_bounds__(kSelThreads)
           if (c >= need) v = cand;
           if (c == need) break;
         }
-        uint32_t kth = kAll;  // the smallest key that reaches it
-        each([&](uint32_t k) { kth = k >= v ? min(kth, k) : kth; });
+        uint32_t kth = kAll;  // the smallest key that reaches it (v > 0: no key is 0)
+        each([&](uint32_t k) { kth = k >= max(v, 1u) ? min(kth, k) : kth; });
         kth = join(__reduce_min_sync(kAll, kth), [](uint32_t x, uint32_t y) { return min(x, y); });
         const float th = key_value(kth), eps2 = __int_as_float(s_amax[t]) * (2.f / 16384.f);
-        from = kth ? order_key(th - eps2) : 0u;
-        above = kth ? order_key(th + eps2) : 0u;
+        from = order_key(th - eps2);
+        above = order_key(th + eps2);
+        n_from = 0;
+        each([&](uint32_t k) {
+          n_from += k >= from ? 1 : 0;
+          n_above += k > above ? 1 : 0;
+        });
+        n_from = sum(n_from);
+        n_above = sum(n_above);
       }
-      int n_above = 0;
-      each([&](uint32_t k) {
-        n_from += k >= from ? 1 : 0;
-        n_above += k > above ? 1 : 0;
-      });
-      n_from = sum(n_from);
-      n_above = sum(n_above);
       if (n_from == need) {
         bar = (uint64_t)from << 32;
         ties = 0x7fffffff;
