@@ -385,7 +385,7 @@ SA_API int sa_paged_append(const sa_paged_append_args* args, sa_stream_t stream)
  * kv head h / (Hq / Hkv). With blocks [N, Hkv, n_blocks] (logical page indexes,
  * strictly ascending, -1 behind the last) token t of a kv head sees only the
  * listed pages; an index that does not ascend or lies behind the token sets
- * SA_DEV_ERR_INDEX and is left out. A row that sees no key is 0. Slots past a
+ * SA_DEV_ERR_INDEX, and entries of its list may be left out. A row that sees no key is 0. Slots past a
  * sequence's length are never used, whatever they hold.
  * max_q (most new tokens of one sequence) and max_len (most keys) only steer the
  * choice of kernel and the split of long sequences: any value >= 1 is correct

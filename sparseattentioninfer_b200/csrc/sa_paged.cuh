@@ -130,6 +130,9 @@ struct PagedAttnParams {
   float scale_log2;
   float* part_o;    // [N, Hq, n_split, D]
   float* part_ml;   // [N, Hq, n_split, 2]
+  int32_t* pages;   // chunk kernel with kept pages: each tile's pages [units, Hkv, page_cap],
+  int32_t* n_pages; // and their numbers [units, Hkv]
+  int32_t page_cap;
   int32_t* err;
 };
 
@@ -148,5 +151,7 @@ int sa_check_paged_batch(const sa_paged_batch* b, const char* what);
 int sa_check_pages(const void* base, const int64_t strides[3], int D, const char* name);
 // The kernel for many query rows (sa_paged_chunk_sm100.cu); maps of k and v are set.
 int sa_paged_chunk_launch(sa::PagedAttnParams& prm, int64_t units, cudaStream_t stream);
+// Largest page table of the chunk kernel with kept pages (a bit each in shared memory).
+constexpr int kChunkMaxPages = 262144;
 // Raises a kernel's dynamic shared memory limit (and with it the SM's carve-out), once per device.
 int sa_smem_once(const void* kernel, int bytes, bool (&done)[64]);

@@ -414,6 +414,9 @@ struct AttnPlan {
   bool chunk;  // 128-row tiles on tcgen05 instead of 16-row units
   int tq, gh, nhg, n_split, split_len;
   int64_t units;
+  int64_t part;      // floats of the split results
+  int64_t page_cap;  // entries of a tile's page list; 0: none
+  int64_t workspace(const sa_paged_attn_args& a) const { return part + units * a.Hkv * (page_cap + (page_cap > 0)); }
 };
 
 static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
@@ -421,7 +424,21 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   const int group = a.Hq / a.Hkv;
   // One 16-row unit holds all rows of a sequence: the rows kernel reads the
   // cache once, and nothing is gained by wider tiles.
-  r.chunk = !a.blocks && group <= 128 && (int64_t)a.max_q * group > kRowMax;
+  const int64_t cap = (int64_t)a.batch.max_pages * a.batch.page_size;
+  int64_t longest = a.max_len < cap ? a.max_len : cap;  // keys of the longest unit
+  r.chunk = group <= 128 && (int64_t)a.max_q * group > kRowMax;
+  r.page_cap = 0;
+  if (a.blocks && r.chunk) {
+    // A tile reads the union of its tokens' pages once, the rows kernel every
+    // token's pages. Lists that may well cover the table make the union pay.
+    const int64_t tokens = a.max_q < 128 / group ? a.max_q : 128 / group;
+    const int64_t seen = (longest + a.batch.page_size - 1) / a.batch.page_size;
+    r.chunk = tokens * a.n_blocks >= seen && a.batch.max_pages <= kChunkMaxPages;
+    if (r.chunk) {
+      r.page_cap = (int64_t)(128 / group) * a.n_blocks;
+      if (r.page_cap > a.batch.max_pages) r.page_cap = a.batch.max_pages;
+    }
+  }
   if (r.chunk) {
     r.gh = group;
     r.nhg = 1;
@@ -433,11 +450,8 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
     if (r.tq < 1) r.tq = 1;
   }
   r.units = unit_count(a.batch.N, a.batch.B, r.tq);
-  // Keys of the longest unit.
-  const int64_t cap = (int64_t)a.batch.max_pages * a.batch.page_size;
-  int64_t longest = a.max_len < cap ? a.max_len : cap;
   if (a.blocks) {
-    const int64_t kept = (int64_t)a.n_blocks * a.batch.page_size;
+    const int64_t kept = (r.chunk ? r.page_cap : (int64_t)a.n_blocks) * a.batch.page_size;
     // Every entry of the list takes its share of a 64-key stage.
     if (kept < longest || a.batch.page_size < kRowKeys) longest = kept;
   }
@@ -459,6 +473,7 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   if ((longest + len - 1) / len > 512) len = ((longest + 511) / 512 + kRowKeys - 1) / kRowKeys * kRowKeys;
   r.split_len = (int)len;
   r.n_split = (int)((longest + len - 1) / len);
+  r.part = r.n_split > 1 ? (int64_t)a.batch.N * a.Hq * r.n_split * (a.D + 2) : 0;
   return r;
 }
 
@@ -540,7 +555,7 @@ extern "C" int sa_paged_attn_workspace(const sa_paged_attn_args* a, int64_t* flo
   const int sms = a->num_sms > 0 ? a->num_sms : sa_num_sms();
   if (sms <= 0) return sa_fail(SA_ERR_CUDA, "cannot query SM count");
   const AttnPlan r = attn_plan(*a, sms);
-  *floats = r.n_split > 1 ? (int64_t)a->batch.N * a->Hq * r.n_split * (a->D + 2) : 0;
+  *floats = r.workspace(*a);
   return SA_OK;
 }
 
@@ -550,7 +565,7 @@ extern "C" int sa_paged_attn(const sa_paged_attn_args* a, sa_stream_t stream_) {
   const int sms = a->num_sms > 0 ? a->num_sms : sa_num_sms();
   if (sms <= 0) return sa_fail(SA_ERR_CUDA, "cannot query SM count");
   const AttnPlan r = attn_plan(*a, sms);
-  if (r.n_split > 1 && !a->workspace) return sa_fail(SA_ERR_INVALID, "paged attention: workspace is NULL");
+  if (r.workspace(*a) > 0 && !a->workspace) return sa_fail(SA_ERR_INVALID, "paged attention: workspace is NULL");
   PagedAttnParams prm;
   memset(&prm, 0, sizeof(prm));
   const int box = a->batch.page_size < kRowKeys ? a->batch.page_size : kRowKeys;
@@ -569,6 +584,9 @@ extern "C" int sa_paged_attn(const sa_paged_attn_args* a, sa_stream_t stream_) {
   prm.scale_log2 = a->scale * 1.4426950408889634f;
   prm.part_o = a->workspace;
   prm.part_ml = a->workspace ? a->workspace + (int64_t)a->batch.N * a->Hq * r.n_split * a->D : nullptr;
+  prm.pages = reinterpret_cast<int32_t*>(a->workspace) + r.part;
+  prm.n_pages = prm.pages + r.units * a->Hkv * r.page_cap;
+  prm.page_cap = (int32_t)r.page_cap;
   prm.err = sa_device_error_ptr();
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream_);
   if (a->dtype == SA_BF16)

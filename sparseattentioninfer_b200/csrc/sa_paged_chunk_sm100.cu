@@ -18,6 +18,13 @@
 // Slots behind the last key may hold anything: S there is masked, and V's rows
 // are set to zero in shared memory by the softmax warps before P is handed over.
 // Unsplit tiles write out = O / l; split ones their O, maximum and sum.
+//
+// With kept pages a tile walks the union of its tokens' lists (a small kernel
+// before writes it, ascending) and each row follows its own list along: the next
+// entry and the one behind it wait in registers, and a chunk whose page is not the
+// next entry is masked for the row. Neighbouring tokens keep much the same pages,
+// and even lists drawn at random share them: of 32 lists of 16 out of 170 pages
+// the union holds some 140, read once instead of 512 pages read one by one.
 #include <type_traits>
 
 #include "sa_paged.cuh"
@@ -52,7 +59,72 @@ struct ChunkCfg {
   static_assert(kKStages + 3 < kChMeta, "mask ring too short");
 };
 
-template <typename T, int D>
+// The ascending union of the lists of one tile's tokens. Entries behind the first
+// -1 are nobody's; one that does not ascend or that its token does not see is
+// left out here, and with it what its row's walk would not reach.
+__global__ void __launch_bounds__(256) paged_union_kernel(const __grid_constant__ PagedAttnParams p, int64_t units) {
+  extern __shared__ uint32_t bits[];
+  __shared__ int s_cnt[8];
+  const sa_paged_attn_args& a = p.a;
+  const sa_paged_batch& bt = a.batch;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y;
+  const int64_t at = (int64_t)blockIdx.x * a.Hkv + kvh;
+  UnitTokens ut;
+  if (!unit_tokens(bt, blockIdx.x, p.tq, p.err, ut)) return;
+  const int ps = bt.page_size, keys = unit_keys(ut, a.max_len);
+  const int words = ((keys + ps - 1) / ps + 31) >> 5;
+  for (int w = tid; w < words; w += 256) bits[w] = 0u;
+  __syncthreads();
+  bool bad = false;
+  for (int t = warp; t < ut.n; t += 8) {
+    const int32_t* list = a.blocks + (int64_t)(ut.t0 + t) * a.blocks_strides[0] + (int64_t)kvh * a.blocks_strides[1];
+    const int own = min(ut.pos0 + t, keys - 1) / ps;  // (a negative position sees nothing)
+    int before = -1;
+    for (int i0 = 0; i0 < a.n_blocks; i0 += 32) {
+      const int i = i0 + lane;
+      const int e = i < a.n_blocks ? __ldg(list + i) : -1;
+      int prev = __shfl_up_sync(0xffffffffu, e, 1);
+      if (lane == 0) prev = before;
+      before = __shfl_sync(0xffffffffu, e, 31);
+      const unsigned end = __ballot_sync(0xffffffffu, e < 0);
+      if (end == 0 || lane < __ffs(end) - 1) {
+        if (e > prev && e <= own && keys > 0)
+          atomicOr(&bits[e >> 5], 1u << (e & 31));
+        else
+          bad = true;
+      }
+      if (end) break;
+    }
+  }
+  if (bad) record_error(p.err, SA_DEV_ERR_INDEX);
+  __syncthreads();
+  // Compact: thread t owns words [t * per, (t + 1) * per).
+  const int per = (words + 255) / 256;
+  int cnt = 0;
+  for (int w = tid * per; w < min(words, (tid + 1) * per); ++w) cnt += __popc(bits[w]);
+  int incl = cnt;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) s_cnt[warp] = incl;
+  __syncthreads();
+  int pos = incl - cnt, all = 0;
+  for (int w = 0; w < 8; ++w) {
+    if (w < warp) pos += s_cnt[w];
+    all += s_cnt[w];
+  }
+  int32_t* out = p.pages + at * p.page_cap;
+  for (int w = tid * per; w < min(words, (tid + 1) * per); ++w)
+    for (uint32_t m = bits[w]; m; m &= m - 1) {
+      if (pos < p.page_cap) out[pos] = w * 32 + __ffs(m) - 1;
+      ++pos;
+    }
+  if (tid == 0) p.n_pages[at] = min(all, p.page_cap);
+}
+
+template <typename T, int D, bool SPARSE>
 __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid_constant__ PagedAttnParams p,
                                                                     int64_t units) {
   using Cfg = ChunkCfg<D>;
@@ -62,6 +134,7 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   __shared__ __align__(8) uint64_t bar_k_full[NSK], bar_k_empty[NSK], bar_v_full[NSV], bar_v_empty[NSV];
   __shared__ __align__(8) uint64_t bar_p_full[2], bar_meta[kChMeta];
   __shared__ uint32_t meta_mask[kChMeta];  // 16-key groups of the chunk that hold keys
+  __shared__ int meta_blk[SPARSE ? kChMeta : 1][4];  // logical pages of the chunk, -1: none
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_flag;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -74,13 +147,24 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   const int kvh = blockIdx.x % a.Hkv;
   const int64_t rest = blockIdx.x / a.Hkv;
   const int split = (int)(rest % p.n_split);
+  const int64_t unit = units - 1 - rest / p.n_split;
   UnitTokens ut;
-  if (!unit_tokens(bt, units - 1 - rest / p.n_split, p.tq, p.err, ut)) return;
+  if (!unit_tokens(bt, unit, p.tq, p.err, ut)) return;
   const int keys = unit_keys(ut, a.max_len);
   if (keys < min(ut.pos0 + ut.n, ut.len) && lane == 0) record_error(p.err, SA_DEV_ERR_INDEX);
-  if (split >= unit_splits(keys, a.split_len)) return;
+  const int pps = ps < N ? N / ps : 1, spp = ps > N ? ps / N : 1, box = min(ps, N);  // pages per chunk, chunks per page
+  const int32_t* union_at = nullptr;
+  int n_union = 0, chunks;
+  if constexpr (SPARSE) {
+    union_at = p.pages + (unit * a.Hkv + kvh) * p.page_cap;
+    n_union = __ldg(p.n_pages + unit * a.Hkv + kvh);
+    chunks = (n_union + pps - 1) / pps * spp;
+  } else {
+    chunks = (keys + N - 1) / N;
+    if (split >= unit_splits(keys, a.split_len)) return;
+  }
   const int c0 = split * (a.split_len / N);  // chunks [c0, c0 + nch)
-  const int nch = max(0, min((keys + N - 1) / N, c0 + a.split_len / N) - c0);
+  const int nch = max(0, (split == p.n_split - 1 ? chunks : min(chunks, c0 + a.split_len / N)) - c0);
   const int rows = ut.n * G;
   const uint32_t sQ = smem_u32(smem_raw), sK = sQ + Cfg::kQBytes, sV = sK + NSK * Cfg::kKVBytes;
 
@@ -140,17 +224,20 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         tma_load_4d(sQ + r * kChM * 128, &p.tm_q, smem_u32(&bar_q), r * 64, kvh * G, ut.t0, 0);
     }
     const int32_t* trow = bt.table + (int64_t)ut.b * bt.table_stride;
-    const int pps = ps < N ? N / ps : 1, spp = ps > N ? ps / N : 1, box = min(ps, N);
     const int e0 = c0 / spp * pps;
-    int page = bt.num_pages, base = -32, kn = 0, vn = 0;  // chunks of K and V issued
+    int page = bt.num_pages, entry = -1, base = -32, kn = 0, vn = 0;  // chunks of K and V issued
     bool ok = true, bad = false;
     for (int g = 0; g < nch; ++g) {
       const int first = (c0 + g) / spp * pps - e0;
       if (first >= base + 32) {
         base = first;
-        const int64_t blk = (int64_t)e0 + base + lane;
+        int64_t blk = (int64_t)e0 + base + lane;
         page = bt.num_pages;  // behind the last page: reads as zeros
-        if (blk * ps < keys) {
+        if constexpr (SPARSE) {
+          blk = blk < n_union ? __ldg(union_at + blk) : -1;
+          entry = (int)blk;
+        }
+        if (blk >= 0 && blk * ps < keys) {
           const int pg = __ldg(trow + blk);
           if (pg < 0 || pg >= bt.num_pages)
             bad = true;
@@ -158,13 +245,19 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
             page = pg;
         }
       }
-      const int pg = __shfl_sync(0xffffffffu, page, (first - base + (lane < pps ? lane : 0)) & 31);
+      const int src = (first - base + (lane < pps ? lane : 0)) & 31;
+      const int pg = __shfl_sync(0xffffffffu, page, src);
+      const int blk_of = SPARSE ? __shfl_sync(0xffffffffu, entry, src) : 0;
       const int off = spp > 1 ? ((c0 + g) % spp) * N : 0;
       const unsigned have = __ballot_sync(0xffffffffu, lane < pps && pg < bt.num_pages);
       const int ks = g % NSK, vs = g % NSV, ms = g % kChMeta;
       if (g >= NSK) {
         ok = mbar_wait(smem_u32(&bar_k_empty[ks]), ((g / NSK) - 1) & 1, abort_v, p.err);
         if (!__all_sync(0xffffffffu, ok)) break;
+      }
+      if constexpr (SPARSE) {
+        if (lane < pps) meta_blk[ms][lane] = blk_of;
+        __syncwarp();
       }
       if (lane == 0) {
         uint32_t mask = 0;
@@ -258,6 +351,30 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
     const int pos = row_ok ? min(ut.pos0 + row / G, keys - 1) : -1;
     float m_ref = -INFINITY, l = 0.f;
     bool ok = true;
+    // The row's walk along its list: entry `ptr` is the next wanted, `ahead` the one behind it.
+    constexpr int kNone = 0x7fffffff;
+    const int32_t* list = nullptr;
+    int ptr = 0, want = kNone, ahead = kNone;
+    auto entry_at = [&](int i) {
+      const int e = i < a.n_blocks ? __ldg(list + i) : -1;
+      return e < 0 ? kNone : e;
+    };
+    if constexpr (SPARSE) {
+      if (row_ok) {
+        list = a.blocks + (int64_t)(ut.t0 + row / G) * a.blocks_strides[0] + (int64_t)kvh * a.blocks_strides[1];
+        const int from = __ldg(union_at + c0 / spp * pps);  // first page of this split
+        int hi = c0 > 0 ? a.n_blocks : 0;
+        while (ptr < hi) {
+          const int mid = (ptr + hi) >> 1;
+          if (entry_at(mid) < from)
+            ptr = mid + 1;
+          else
+            hi = mid;
+        }
+        want = entry_at(ptr);
+        ahead = want == kNone ? kNone : entry_at(ptr + 1);
+      }
+    }
     for (int g = 0; g < nch; ++g) {
       const int ms = g % kChMeta;
       ok = mbar_wait(smem_u32(&bar_meta[ms]), (g / kChMeta) & 1, abort_v, p.err);
@@ -267,36 +384,63 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
       if (!__all_sync(FULL, ok)) { ok = false; break; }
       tc_fence_after();
       const uint32_t sbuf = tmem + lane_base + SB + (g & 1) * N;
-      const int key0 = (c0 + g) * N;
-      float s[N];
-      {
-        uint32_t r32[2][32];
-        tmem_ld32(sbuf, r32[0]);
-        tmem_ld32(sbuf + 32, r32[1]);
-        tmem_wait_ld();
+      const int off = SPARSE ? (c0 + g) % spp * N : (c0 + g) * N;  // first key, in its page or of all
+      int lim[4];  // column i of the chunk is seen when i % 16 <= lim[i / 16]
+      bool plain = true, skip = false, tail = false;
+      if constexpr (SPARSE) {
+        bool any = false;
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          reg_fence32(r32[cc]);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) s[cc * 32 + i] = __uint_as_float(r32[cc][i]);
+        for (int q = 0; q < 4; ++q) {
+          const int jp = q * 16 / box, blk = meta_blk[ms][jp];
+          const int key0 = blk * ps + off + q * 16 - jp * box;
+          lim[q] = blk == want && ((mask >> q) & 1u) ? min(pos - key0, 15) : -1;
+          plain &= lim[q] == 15;
+          any |= lim[q] >= 0;
+          tail |= blk >= 0 && key0 + 16 > keys;
+          if ((q + 1) * 16 % box == 0 && blk == want && (c0 + g) % spp == spp - 1) {
+            ++ptr;
+            want = ahead;
+            ahead = want == kNone ? kNone : entry_at(ptr + 1);
+          }
         }
-      }
-      const int lim = pos - key0;  // columns <= lim are seen
-      if (lim < N - 1 || mask != 0xfu) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = (i <= lim && ((mask >> (i / 16)) & 1u)) ? s[i] : -INFINITY;
-      }
-      float mx8[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) mx8[i] = s[i];
-#pragma unroll
-      for (int i = 8; i < N; i += 2) mx8[(i >> 1) & 7] = max3(mx8[(i >> 1) & 7], s[i], s[i + 1]);
-      const float mraw = max3(fmaxf(max3(mx8[0], mx8[1], mx8[2]), mx8[3]), max3(mx8[4], mx8[5], mx8[6]), mx8[7]);
-      const float m_new = fmaxf(m_ref, mraw * p.scale_log2);
-      if (g == 0) {
-        m_ref = m_new;
+        skip = !__any_sync(FULL, any);  // no row of the warp sees the chunk
       } else {
-        const bool need = m_new > m_ref + 8.0f;
+        plain = pos - off >= N - 1 && mask == 0xfu;
+        tail = off + N > keys;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) lim[q] = ((mask >> q) & 1u) ? min(pos - off - q * 16, 15) : -1;
+      }
+      uint32_t pk[N / 2];
+      if (skip) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) pk[i] = 0u;
+      } else {
+        float s[N];
+        {
+          uint32_t r32[2][32];
+          tmem_ld32(sbuf, r32[0]);
+          tmem_ld32(sbuf + 32, r32[1]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            reg_fence32(r32[cc]);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[cc * 32 + i] = __uint_as_float(r32[cc][i]);
+          }
+        }
+        if (!plain) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) s[i] = i % 16 <= lim[i / 16] ? s[i] : -INFINITY;
+        }
+        float mx8[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx8[i] = s[i];
+#pragma unroll
+        for (int i = 8; i < N; i += 2) mx8[(i >> 1) & 7] = max3(mx8[(i >> 1) & 7], s[i], s[i + 1]);
+        const float mraw = max3(fmaxf(max3(mx8[0], mx8[1], mx8[2]), mx8[3]), max3(mx8[4], mx8[5], mx8[6]), mx8[7]);
+        const float m_new = fmaxf(m_ref, mraw * p.scale_log2);
+        // (a row that has seen no key yet has nothing in O to rescale)
+        const bool need = m_ref > -INFINITY && m_new > m_ref + 8.0f;
         if (__any_sync(FULL, need)) {
           // O still takes the previous chunk's PV: wait for it, then rescale.
           ok = mbar_wait(smem_u32(&bar_v_empty[(g - 1) % NSV]), ((g - 1) / NSV) & 1, abort_v, p.err);
@@ -314,42 +458,40 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
             tmem_st32(tmem + lane_base + cc * 32, o32);
           }
           tmem_wait_st();
-          if (need) {
-            l *= alpha;
-            m_ref = m_new;
-          }
+          if (need) l *= alpha;
         }
-      }
-      const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
-      const uint64_t sc2 = f2pack(p.scale_log2, p.scale_log2), nm2 = f2pack(-m_use, -m_use);
-      uint64_t rs4[4] = {0ull, 0ull, 0ull, 0ull};
-      uint32_t pk[N / 2];
+        if (need || m_ref == -INFINITY) m_ref = m_new;
+        const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
+        const uint64_t sc2 = f2pack(p.scale_log2, p.scale_log2), nm2 = f2pack(-m_use, -m_use);
+        uint64_t rs4[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        float x0, x1;
-        f2unpack(fma2(f2pack(s[2 * i], s[2 * i + 1]), sc2, nm2), x0, x1);
-        const float p0 = ex2(x0), p1 = ex2(x1);
-        rs4[i & 3] = add2(rs4[i & 3], f2pack(p0, p1));
-        pk[i] = Half<T>::pack(p0, p1);
-      }
-      tmem_st32(sbuf, pk);
-      {
+        for (int i = 0; i < N / 2; ++i) {
+          float x0, x1;
+          f2unpack(fma2(f2pack(s[2 * i], s[2 * i + 1]), sc2, nm2), x0, x1);
+          const float p0 = ex2(x0), p1 = ex2(x1);
+          rs4[i & 3] = add2(rs4[i & 3], f2pack(p0, p1));
+          pk[i] = Half<T>::pack(p0, p1);
+        }
         float a0, a1, b0, b1;
         f2unpack(add2(rs4[0], rs4[1]), a0, a1);
         f2unpack(add2(rs4[2], rs4[3]), b0, b1);
         l += (a0 + a1) + (b0 + b1);
       }
-      if (key0 + N > keys) {
+      tmem_st32(sbuf, pk);
+      if (tail) {
         // V rows past the last key: zero, whatever the page holds there.
         ok = mbar_wait(smem_u32(&bar_v_full[g % NSV]), (g / NSV) & 1, abort_v, p.err);
         if (!__all_sync(FULL, ok)) { ok = false; break; }
         const uint32_t v0 = sV + (g % NSV) * Cfg::kKVBytes;
-        const int first = keys - key0;
-        for (int i = row; i < (N - first) * 8 * R; i += 128) {
-          const int reg = i / ((N - first) * 8), in = i % ((N - first) * 8);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v0 + reg * N * 128 + first * 128 + in * 16),
-                       "r"(0u)
-                       : "memory");
+        for (int i = row; i < N * 8 * R; i += 128) {
+          const int r = (i >> 3) % N;
+          int key = off + r;
+          if constexpr (SPARSE) {
+            const int blk = meta_blk[ms][r / box];
+            key = blk < 0 ? 0 : blk * ps + off + r % box;  // (none: read as zeros)
+          }
+          if (key >= keys)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v0 + i * 16), "r"(0u) : "memory");
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
@@ -436,17 +578,29 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   if (warp == 1) tmem_dealloc(tmem, Cfg::kTmemCols);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool SPARSE>
 static int launch_chunk(const PagedAttnParams& prm, int64_t units, cudaStream_t stream) {
-  auto kern = paged_chunk_kernel<T, D>;
-  static bool done[64];
+  auto kern = paged_chunk_kernel<T, D, SPARSE>;
+  static bool done[64], union_done[64];
   int rc = sa_smem_once(reinterpret_cast<const void*>(kern), ChunkCfg<D>::kSmemBytes, done);
   if (rc) return rc;
   const int64_t blocks = units * prm.n_split * prm.a.Hkv;
-  if (blocks > 0x7fffffff) return sa_fail(SA_ERR_INVALID, "paged attention: batch too large");
+  if (blocks > 0x7fffffff || prm.a.Hkv > 65535) return sa_fail(SA_ERR_INVALID, "paged attention: batch too large");
+  if constexpr (SPARSE) {
+    rc = sa_smem_once(reinterpret_cast<const void*>(paged_union_kernel), kChunkMaxPages / 8, union_done);
+    if (rc) return rc;
+    paged_union_kernel<<<dim3((unsigned)units, prm.a.Hkv), 256, (prm.a.batch.max_pages + 31) / 32 * 4, stream>>>(
+        prm, units);
+    SA_CHECK_CUDA(cudaGetLastError());
+  }
   kern<<<(unsigned)blocks, kChThreads, ChunkCfg<D>::kSmemBytes, stream>>>(prm, units);
   SA_CHECK_CUDA(cudaGetLastError());
   return SA_OK;
+}
+
+template <typename T, int D>
+static int launch_chunk_any(const PagedAttnParams& prm, int64_t units, cudaStream_t stream) {
+  return prm.a.blocks ? launch_chunk<T, D, true>(prm, units, stream) : launch_chunk<T, D, false>(prm, units, stream);
 }
 
 }  // namespace sa
@@ -462,7 +616,8 @@ int sa_paged_chunk_launch(PagedAttnParams& prm, int64_t units, cudaStream_t stre
   int rc = sa_make_map4(&prm.tm_q, a.q, dims, strides, box, "q");
   if (rc) return rc;
   if (a.dtype == SA_BF16)
-    return a.D == 128 ? launch_chunk<__nv_bfloat16, 128>(prm, units, stream)
-                      : launch_chunk<__nv_bfloat16, 64>(prm, units, stream);
-  return a.D == 128 ? launch_chunk<__half, 128>(prm, units, stream) : launch_chunk<__half, 64>(prm, units, stream);
+    return a.D == 128 ? launch_chunk_any<__nv_bfloat16, 128>(prm, units, stream)
+                      : launch_chunk_any<__nv_bfloat16, 64>(prm, units, stream);
+  return a.D == 128 ? launch_chunk_any<__half, 128>(prm, units, stream)
+                    : launch_chunk_any<__half, 64>(prm, units, stream);
 }

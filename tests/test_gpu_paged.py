@@ -166,14 +166,16 @@ def _random_blocks(bt, keep, seed=0, empty=False):
 
 
 @pytest.mark.parametrize("ctx,new,Hq,Hkv,D,page,dtype,layout,pad", ATTN)
-@pytest.mark.parametrize("keep,split_len", [(1, None), (5, 64), (9, None)])
-def test_sparse_attention(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, keep, split_len):
+@pytest.mark.parametrize("keep,split_len", [(1, None), (5, 64), (9, None), (30, 128)])
+@pytest.mark.parametrize("max_q", [1, None])
+def test_sparse_attention(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, keep, split_len, max_q):
     bt = P.Batch(ctx, new, Hq=Hq, Hkv=Hkv, D=D, page=page, dtype=dtype, device=DEV, seed=keep, pad=pad, layout=layout)
     q, k, v = _qkv(bt)
     blocks = _random_blocks(bt, keep, empty=True)  # some lists are empty: those rows are 0
     out = torch.full((bt.N, Hq, D), 3.0, dtype=dtype, device=DEV)
     before = out.clone()
-    ops.paged_attention(q.to(DEV), k, v, *bt.batch, blocks=blocks.to(DEV), split_len=split_len, out=out)
+    ops.paged_attention(q.to(DEV), k, v, *bt.batch, blocks=blocks.to(DEV), split_len=split_len, max_q=max_q,
+                        out=out)
     _assert_attention(bt, out, q, k, v, 1 / math.sqrt(D), blocks, before)
 
 
