@@ -64,20 +64,20 @@ static PFN_encodeTiled_t get_encode_fn() {
   return fn;
 }
 
-// 4-D map of 16-bit elements (dims and box innermost first, strides in elements of dims 1..3),
-// SWIZZLE_128B, zero fill out of range.
-int sa_make_map4(CUtensorMap* m, const void* base, const int64_t dims[4], const int64_t strides[3],
-                 const int box[4], const char* name) {
+// Map of 16-bit elements of n <= 5 dimensions (dims and box innermost first, strides in elements of
+// dims 1..n-1), SWIZZLE_128B, zero fill out of range.
+int sa_make_map_nd(CUtensorMap* m, const void* base, int n, const int64_t* dims, const int64_t* strides,
+                   const int* box, const char* name) {
   PFN_encodeTiled_t enc = get_encode_fn();
   if (!enc) return sa_fail(SA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  cuuint64_t d[4], g[3];
-  cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
-  for (int i = 0; i < 4; ++i) {
+  cuuint64_t d[5], g[4];
+  cuuint32_t b[5], estr[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < n; ++i) {
     d[i] = (cuuint64_t)dims[i];
     b[i] = (cuuint32_t)box[i];
+    if (i + 1 < n) g[i] = (cuuint64_t)strides[i] * 2;
   }
-  for (int i = 0; i < 3; ++i) g[i] = (cuuint64_t)strides[i] * 2;
-  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, g, b, estr,
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, n, const_cast<void*>(base), d, g, b, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return sa_fail(SA_ERR_INVALID, "tensor map for %s rejected (CUresult %d)", name, (int)r);
@@ -89,7 +89,7 @@ int sa_make_map(CUtensorMap* m, const void* base, int B, int H, int T, int D,
                     const int64_t strides[3], int box_rows, const char* name) {
   const int64_t dims[4] = {D, T, H, B}, st[3] = {strides[2], strides[1], strides[0]};
   const int box[4] = {64, box_rows, 1, 1};
-  return sa_make_map4(m, base, dims, st, box, name);
+  return sa_make_map_nd(m, base, 4, dims, st, box, name);
 }
 
 extern "C" const char* sa_version(void) { return SA_VERSION_STRING; }

@@ -23,9 +23,9 @@ int32_t* sa_device_error_ptr();
 int sa_make_map(CUtensorMap* m, const void* base, int B, int H, int T, int D, const int64_t strides[3],
                 int box_rows, const char* name);
 
-// The same with any box: dims and box innermost first, element strides of dims 1..3.
-int sa_make_map4(CUtensorMap* m, const void* base, const int64_t dims[4], const int64_t strides[3],
-                 const int box[4], const char* name);
+// The same of n <= 5 dimensions and any box: dims and box innermost first, element strides of dims 1..n-1.
+int sa_make_map_nd(CUtensorMap* m, const void* base, int n, const int64_t* dims, const int64_t* strides,
+                   const int* box, const char* name);
 
 #define SA_CHECK_CUDA(call)                                   \
   do {                                                        \
@@ -138,6 +138,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int32_t c0, int32_t c1, int32_t c2, int32_t c3, int32_t c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
 }
 

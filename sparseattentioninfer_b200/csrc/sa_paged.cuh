@@ -44,16 +44,14 @@ __device__ __forceinline__ bool unit_tokens(const sa_paged_batch& bt, int64_t u,
                                             UnitTokens& r) {
   const int32_t* cu = bt.cu_q;
   if (tq == 1) {
-    if (u >= __ldg(cu + bt.B)) return false;  // rows behind the last sequence
     r.b = last_start(bt.B, u, [&](int b) { return (int64_t)__ldg(cu + b); });
   } else {
     r.b = last_start(bt.B, u, [&](int b) { return (int64_t)__ldg(cu + b) / tq + b; });
   }
-  const int c0 = __ldg(cu + r.b), c1 = __ldg(cu + r.b + 1);
+  const int c0 = __ldg(cu + r.b), c1 = __ldg(cu + r.b + 1), full = __ldg(bt.seq_lens + r.b);
   const int64_t first = tq == 1 ? u : c0 + (u - (c0 / tq + r.b)) * (int64_t)tq;
-  if (first < c0 || first >= c1) return false;
+  if (first < c0 || first >= c1) return false;  // an empty unit, or rows behind the last sequence
   const int cap = (int)min((int64_t)bt.max_pages * bt.page_size, (int64_t)0x7fffffff);
-  const int full = __ldg(bt.seq_lens + r.b);
   if (c0 < 0 || c1 > bt.N || full < c1 - c0 || full > cap) {
     record_error(err, SA_DEV_ERR_INDEX);
     if (c0 < 0 || c1 > bt.N || full < c1 - c0) return false;
@@ -65,8 +63,57 @@ __device__ __forceinline__ bool unit_tokens(const sa_paged_batch& bt, int64_t u,
   return true;
 }
 
+// Unit number of the u-th tile when tiles are taken longest sequence first and,
+// of one sequence, last tokens (the most keys) first; -1 behind the last tile.
+// One lane a sequence: for up to 32 of them. Longer batches keep their order,
+// from the end: among many sequences the long ones spread by themselves.
+__device__ __forceinline__ int64_t longest_first(const sa_paged_batch& bt, int64_t u, int64_t units, int tq) {
+  if (bt.B > 32) return units - 1 - u;
+  constexpr unsigned A = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  int len = -1, tiles = 0;
+  int64_t start = 0;
+  if (lane < bt.B) {
+    const int c0 = __ldg(bt.cu_q + lane), c1 = __ldg(bt.cu_q + lane + 1);
+    tiles = max(0, (c1 - c0 + tq - 1) / tq);
+    len = __ldg(bt.seq_lens + lane);
+    start = tq == 1 ? c0 : c0 / tq + lane;
+  }
+  int before = 0;  // tiles of longer sequences
+  for (int i = 0; i < bt.B; ++i) {
+    const int li = __shfl_sync(A, len, i), ti = __shfl_sync(A, tiles, i);
+    if (li > len || (li == len && i < lane)) before += ti;
+  }
+  const bool mine = lane < bt.B && u >= before && u < before + tiles;
+  const unsigned m = __ballot_sync(A, mine);
+  if (!m) return -1;
+  return __shfl_sync(A, start + (before + tiles - 1 - u), __ffs(m) - 1);
+}
+
 // Units that cover any batch of N tokens in B sequences.
 inline int64_t unit_count(int64_t N, int64_t B, int tq) { return tq == 1 ? N : N / tq + B; }
+
+// Thread-block clusters: barrier halves, and a peer's shared memory.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ uint32_t cluster_map(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
 
 // 16-bit element types of the cache.
 template <typename T>

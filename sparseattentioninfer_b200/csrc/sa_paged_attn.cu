@@ -15,39 +15,48 @@
 // visible key hold anything: their scores are masked and their V rows set to
 // zero in shared memory before the product (0 * NaN is NaN).
 // Splits are split_len keys long whatever the sequence's length, so that a
-// ragged batch still makes equal CTAs; a second kernel joins them.
+// ragged batch still makes equal CTAs. In grids that are resident at once up to 8
+// splits of a unit are a thread-block cluster and join through its shared memory
+// (2,048 keys of 8 kv heads: 11.8 -> 7.6 us); others go through the workspace and
+// a second kernel.
 #include <cstring>
 
 #include "sa_paged.cuh"
 
 namespace sa {
 
-constexpr int kRowConsumers = 4;
-constexpr int kRowThreads = 32 * (kRowConsumers + 1);
-constexpr int kRowStages = 3;
 constexpr int kRowKeys = 64;  // keys per stage
 constexpr int kRowMax = 16;   // query rows per CTA
 
-template <int D>
+// WIDE: one CTA on an SM, for grids that leave no second one for it: a ring of
+// 192 KB and two groups of consumer warps, which take the stages in turn.
+template <int D, int ROWS, bool WIDE>
 struct PagedRowCfg {
   static constexpr int kRegions = D / 64;
   static constexpr int kHalfBytes = kRowKeys * D * 2;
   static constexpr int kStageBytes = 2 * kHalfBytes;
-  static constexpr int kSmemBytes = kRowStages * kStageBytes;
-  static_assert(kRowConsumers * kRowMax * D * 4 <= kSmemBytes, "ring too small for the partial outputs");
+  static constexpr int kGroups = WIDE ? 2 : 1;
+  static constexpr int kConsumers = 4 * kGroups;  // warps
+  static constexpr int kThreads = 32 * (kConsumers + 1);
+  // Otherwise two CTAs on an SM, four where the registers and 64-wide heads allow it.
+  static constexpr int kStages = WIDE ? 196608 / kStageBytes : (D == 64 && ROWS == 16) ? 6 : 3;
+  static constexpr int kSmemBytes = kStages * kStageBytes;
+  static_assert(kConsumers * ROWS * D * 4 <= kSmemBytes, "ring too small for the partial outputs");
 };
 
 // ROWS 8: at most 8 query rows, half of the products' rows are padding that
 // costs nothing but tensor rate; ROWS 16 holds twice the accumulators.
-template <typename T, int D, bool SPARSE, int ROWS>
-__global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_constant__ PagedAttnParams p) {
-  using Cfg = PagedRowCfg<D>;
-  constexpr int R = Cfg::kRegions;
+template <typename T, int D, bool SPARSE, int ROWS, bool WIDE>
+__global__ void __launch_bounds__(PagedRowCfg<D, ROWS, WIDE>::kThreads) paged_rows_kernel(const __grid_constant__ PagedAttnParams p) {
+  using Cfg = PagedRowCfg<D, ROWS, WIDE>;
+  constexpr int R = Cfg::kRegions, kRowStages = Cfg::kStages, kRowGroups = Cfg::kGroups;
+  constexpr int kRowConsumers = Cfg::kConsumers, kRowThreads = Cfg::kThreads;
   constexpr int NT = D / 8;
   constexpr int HR = ROWS / 8;  // rows per thread
   __shared__ __align__(8) uint64_t bar_full[kRowStages], bar_empty[kRowStages];
   __shared__ int s_key0[kRowStages][4];  // first key of each 16-key group, -1: none
   __shared__ float s_m[kRowConsumers][ROWS], s_l[kRowConsumers][ROWS];
+  __shared__ float2 s_ml[ROWS];  // the CTA's maximum and sum of each row
   __shared__ int abort_flag;
   extern __shared__ __align__(1024) uint8_t dsmem[];
   const uint32_t sbase = smem_u32(dsmem);
@@ -69,9 +78,9 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
   const int rows = ut.n * nh;
   // Stages [st0, st1) of this split: 64 keys each, or with kept pages the list's
   // entries (64 / ps of them, or a part of one).
-  const int pps = ps < kRowKeys ? kRowKeys / ps : 1;  // pages per stage
-  const int spp = ps > kRowKeys ? ps / kRowKeys : 1;  // stages per page
-  const int box = min(ps, kRowKeys);
+  const int box = min(ps, kRowKeys), lbox = 31 - __clz(box);
+  const int lpps = 6 - lbox, pps = 1 << lpps;             // pages per stage
+  const int spp = max(1, ps / kRowKeys), lspp = spp >> 1;  // stages per page: 1 or 2
   const int32_t* list = nullptr;
   int st0, st1, n_used, n_list = 0x7fffffff;  // entries of the list
   if constexpr (SPARSE) {
@@ -84,14 +93,14 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
       if (m != 0xffffffffu) break;
     }
     n_list = cnt;
-    const int nst = (cnt + pps - 1) / pps * spp;
+    const int nst = (cnt + pps - 1) >> lpps << lspp;
     n_used = max(1, (nst + per - 1) / per);
     st0 = split * per;
     st1 = min(nst, st0 + per);
     n_used = min(n_used, p.n_split);
     if (split == p.n_split - 1) st1 = nst;
-    if (split >= n_used) {
-      // The join reads every split of the row: this one has nothing.
+    if (split >= n_used && !WIDE) {
+      // The join kernel reads every split of the row: this one has nothing.
       if (p.n_split > 1)
         for (int r = tid; r < rows; r += kRowThreads) {
           const int64_t at = ((int64_t)(ut.t0 + r / nh) * a.Hq + h0 + r % nh) * p.n_split + split;
@@ -102,17 +111,19 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
     }
   } else {
     n_used = unit_splits(keys, a.split_len);
-    if (split >= n_used) return;
+    if (split >= n_used && !WIDE) return;
     st0 = split * (a.split_len / kRowKeys);
     st1 = min((keys + kRowKeys - 1) / kRowKeys, st0 + a.split_len / kRowKeys);
   }
   const int nst = max(0, st1 - st0);
 
   if (tid == 0) {
+    tma_prefetch_desc(&p.tm_k);
+    tma_prefetch_desc(&p.tm_v);
     if (sbase & 1023u) record_error(p.err, SA_DEV_ERR_INDEX);
     for (int i = 0; i < kRowStages; ++i) {
       mbar_init(smem_u32(&bar_full[i]), 1);
-      mbar_init(smem_u32(&bar_empty[i]), kRowConsumers);
+      mbar_init(smem_u32(&bar_empty[i]), 4);
     }
     abort_flag = 0;
     fence_mbar_init();
@@ -135,11 +146,10 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
 
   if (warp == kRowConsumers) {
     // ------------------------------------------------------------ producer
-    // Lane j < pps loads page j of the stage; the page numbers of the next 32
-    // pages are read ahead, one a lane.
+    // The page numbers of the next 32 pages are read ahead, one a lane.
     const int32_t* trow = bt.table + (int64_t)ut.b * bt.table_stride;
-    const int e0 = st0 / spp * pps;                        // first entry of the split
-    const int ne = min((st1 + spp - 1) / spp * pps, n_list) - e0;  // entries of the split
+    const int e0 = st0 >> lspp << lpps;                                   // first entry of the split
+    const int ne = min((st1 + spp - 1) >> lspp << lpps, n_list) - e0;  // entries of the split
     int blk = -1, page = -1, bad = 0;
     auto fetch = [&](int i) {  // entry e0 + i: logical block and page, -1: none
       blk = -1;
@@ -165,43 +175,42 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
         }
       }
     };
-    bool ok = true;
-    int base = -32;
+    // Lane j < 8 of a stage: 16-key group j & 3, of K (j < 4) or V. The group that
+    // begins a page loads all of it with one copy.
+    const int group16 = lane & 3, side = (lane >> 2) & 1;
+    const int jp = (group16 * 16) >> lbox, in_page = (group16 * 16) & (box - 1);
+    const bool leads = lane < 8 && in_page == 0;
+    const CUtensorMap* map = side ? &p.tm_v : &p.tm_k;
+    const uint32_t dst0 = sbase + side * Cfg::kHalfBytes + jp * box * (D * 2);
+    int base = -32, slot = 0;
+    uint32_t parity = 1;  // of the slot's last use
     for (int i = 0; i < nst; ++i) {
-      const int slot = i % kRowStages;
-      const int first = (st0 + i) / spp * pps - e0;  // entry of the stage's first page
+      const int first = ((st0 + i) >> lspp << lpps) - e0;  // entry of the stage's first page
       if (first >= base + 32) {
         base = first;
         fetch(base + lane);
       }
-      const int src = (first - base + (lane < pps ? lane : 0)) & 31;
+      const int src = (first - base + jp) & 31;
       const int pg = __shfl_sync(0xffffffffu, page, src);
       const int bk = __shfl_sync(0xffffffffu, blk, src);
-      const int off = spp > 1 ? ((st0 + i) % spp) * kRowKeys : 0;
-      const bool mine = lane < pps && pg >= 0 && (int64_t)bk * ps + off < keys;
+      const int off = ((st0 + i) & (spp - 1)) * kRowKeys;
+      const int key0 = bk * ps + off + in_page;  // (bk * ps < keys)
+      const bool have = pg >= 0 && bk * ps + off < keys;
+      const bool mine = leads && have;
       const int n = __popc(__ballot_sync(0xffffffffu, mine));
-      if (i >= kRowStages) {
-        ok = mbar_wait(smem_u32(&bar_empty[slot]), ((i / kRowStages) - 1) & 1, abort_v, p.err);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          // stages from i on were not loaded
-          st1 = st0 + i;
-          break;
-        }
+      const bool ok = i < kRowStages || mbar_wait(smem_u32(&bar_empty[slot]), parity, abort_v, p.err);
+      if (!__all_sync(0xffffffffu, ok)) {
+        st1 = st0 + i;  // stages from i on were not loaded
+        break;
       }
-      if (lane < pps)
-        for (int g = 0; g < box / 16; ++g) s_key0[slot][lane * (box / 16) + g] = mine ? bk * ps + off + 16 * g : -1;
-      __syncwarp();
+      if (lane < 4) s_key0[slot][lane] = have ? key0 : -1;
       const uint32_t bar = smem_u32(&bar_full[slot]);
-      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)n * box * D * 4);
+      if (mine) tma_load_5d(dst0 + slot * Cfg::kStageBytes, map, bar, 0, off, 0, kvh, pg);
       __syncwarp();
-      if (mine) {
-        const uint32_t dst = sbase + slot * Cfg::kStageBytes + lane * box * 128;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          tma_load_4d(dst + r * kRowKeys * 128, &p.tm_k, bar, r * 64, off, kvh, pg);
-          tma_load_4d(dst + Cfg::kHalfBytes + r * kRowKeys * 128, &p.tm_v, bar, r * 64, off, kvh, pg);
-        }
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)n * box * D * 2);
+      if (++slot == kRowStages) {
+        slot = 0;
+        parity ^= 1;
       }
     }
     if (__any_sync(0xffffffffu, bad) && lane == 0) record_error(p.err, SA_DEV_ERR_INDEX);
@@ -228,14 +237,18 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
         qa[kk][2 * r + 1] = live ? *reinterpret_cast<const uint32_t*>(qrow + d + 8) : 0u;
       }
     }
-    const int k_lo = warp * 16;
-    for (int i = 0; i < nst; ++i) {
-      const int slot = i % kRowStages;
-      const bool ok = mbar_wait(smem_u32(&bar_full[slot]), (i / kRowStages) & 1, abort_v, p.err);
+    // This warp's 16 keys of a stage: rows of 128 bytes, a page's 64-column
+    // regions one behind the other.
+    const uint32_t keys_at = ((warp & 3) * 16 >> lbox) * box * (D * 2) + ((warp & 3) * 16 & (box - 1)) * 128;
+    const uint32_t region = box * 128;
+    int slot = WIDE ? warp >> 2 : 0;
+    uint32_t parity = 0;
+    for (int i = slot; i < nst; i += kRowGroups) {
+      const bool ok = mbar_wait(smem_u32(&bar_full[slot]), parity, abort_v, p.err);
       if (!__all_sync(0xffffffffu, ok)) break;
-      const int key0 = s_key0[slot][warp];
+      const int key0 = s_key0[slot][warp & 3];
       if (key0 >= 0 && key0 < keys) {
-        const uint32_t sk = sbase + slot * Cfg::kStageBytes;
+        const uint32_t sk = sbase + slot * Cfg::kStageBytes + keys_at;
         const uint32_t sv = sk + Cfg::kHalfBytes;
         if (key0 + 16 > keys) {
           // V rows past the last key: zero, whatever the page holds there.
@@ -243,24 +256,31 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
           for (int r = first + (lane >> 3); r < 16; r += 4)
 #pragma unroll
             for (int reg = 0; reg < R; ++reg)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + reg * kRowKeys * 128 +
-                                                                           (k_lo + r) * 128 + (lane & 7) * 16),
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + reg * region + r * 128 +
+                                                                           (lane & 7) * 16),
                            "r"(0u)
                            : "memory");
           // (the next TMA load into this slot is ordered behind these stores)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         }
+        // (two accumulators a tile, so that the chain of products is half as long)
         float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-        const int kr = k_lo + (lane & 7) + ((lane >> 4) << 3);
+        float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
+        const int kr = (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const int ch = ((kk & 3) << 1) + ((lane >> 3) & 1);
           uint32_t b0, b1, b2, b3;
-          ldsm_x4(sw128(sk + (kk >> 2) * kRowKeys * 128, kr, ch), b0, b1, b2, b3);
+          ldsm_x4(sw128(sk + (kk >> 2) * region, kr, ch), b0, b1, b2, b3);
           const uint32_t a1 = HR == 2 ? qa[kk][2 * (HR - 1)] : 0u, a3 = HR == 2 ? qa[kk][2 * (HR - 1) + 1] : 0u;
-          Half<T>::mma(s0, qa[kk][0], a1, qa[kk][1], a3, b0, b1);
-          Half<T>::mma(s1, qa[kk][0], a1, qa[kk][1], a3, b2, b3);
+          Half<T>::mma(kk & 1 ? t0 : s0, qa[kk][0], a1, qa[kk][1], a3, b0, b1);
+          Half<T>::mma(kk & 1 ? t1 : s1, qa[kk][0], a1, qa[kk][1], a3, b2, b3);
+        }
+#pragma unroll
+        for (int e = 0; e < 2 * HR; ++e) {
+          s0[e] += t0[e];
+          s1[e] += t1[e];
         }
         // This thread's keys of a row: c0, c0 + 1, c0 + 8, c0 + 9.
         const int c0 = key0 + 2 * (lane & 3);
@@ -287,12 +307,12 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
           const float2 u = Half<T>::unpack(pa[2 * r]), v = Half<T>::unpack(pa[2 * r + 1]);
           l_run[r] = l_run[r] * alpha[r] + (u.x + u.y) + (v.x + v.y);
         }
-        const int vr = k_lo + (lane & 7) + (((lane >> 3) & 1) << 3);
+        const int vr = (lane & 7) + (((lane >> 3) & 1) << 3);
 #pragma unroll
         for (int j = 0; j < NT; j += 2) {
           const int dch = j + (lane >> 4);
           uint32_t v0, v1, v2, v3;
-          ldsm_x4_t(sw128(sv + (dch >> 3) * kRowKeys * 128, vr, dch & 7), v0, v1, v2, v3);
+          ldsm_x4_t(sw128(sv + (dch >> 3) * region, vr, dch & 7), v0, v1, v2, v3);
           float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int e = 0; e < 2 * HR; ++e) {
@@ -311,6 +331,11 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&bar_empty[slot]));
+      slot += kRowGroups;
+      if (slot >= kRowStages) {
+        slot -= kRowStages;
+        parity ^= 1;
+      }
     }
   }
   __syncthreads();  // ring idle (producer drained): reuse it for the warps' partial outputs
@@ -331,34 +356,83 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
     }
   }
   __syncthreads();
-  for (int idx = tid; idx < rows * (D / 2); idx += kRowThreads) {
-    const int r = idx / (D / 2), d = idx % (D / 2) * 2;
+  auto out_at = [&](int r) {
+    return reinterpret_cast<T*>(a.out) + (int64_t)(ut.t0 + r / nh) * a.o_strides[0] +
+           (int64_t)(h0 + r % nh) * a.o_strides[1];
+  };
+  for (int idx = tid; idx < rows * (D / 4); idx += kRowThreads) {
+    const int r = idx / (D / 4), d = idx % (D / 4) * 4;
     float mx = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kRowConsumers; ++w) mx = fmaxf(mx, s_m[w][r]);
     const float mu = mx == -INFINITY ? 0.f : mx;
-    float lsum = 0.f, acc0 = 0.f, acc1 = 0.f;
+    float lsum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kRowConsumers; ++w) {
       const float c = ex2(s_m[w][r] - mu);
-      const float2 o = *reinterpret_cast<const float2*>(&s_o[w][r][d]);
+      const float4 o = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
       lsum += s_l[w][r] * c;
-      acc0 += o.x * c;
-      acc1 += o.y * c;
+      acc.x += o.x * c;
+      acc.y += o.y * c;
+      acc.z += o.z * c;
+      acc.w += o.w * c;
     }
-    const int tok = ut.t0 + r / nh, h = h0 + r % nh;
     if (p.n_split == 1) {
       const float inv = lsum > 0.f ? 1.0f / lsum : (lsum == 0.f ? 0.f : lsum);
-      *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + (int64_t)tok * a.o_strides[0] +
-                                   (int64_t)h * a.o_strides[1] + d) = Half<T>::pack(acc0 * inv, acc1 * inv);
+      *reinterpret_cast<uint2*>(out_at(r) + d) =
+          make_uint2(Half<T>::pack(acc.x * inv, acc.y * inv), Half<T>::pack(acc.z * inv, acc.w * inv));
+    } else if (WIDE) {
+      *reinterpret_cast<float4*>(&s_o[0][r][d]) = acc;  // (this thread's own element)
+      if (d == 0) s_ml[r] = make_float2(mx, lsum);
     } else {
-      const int64_t at = ((int64_t)tok * a.Hq + h) * p.n_split + split;
-      *reinterpret_cast<float2*>(p.part_o + at * D + d) = make_float2(acc0, acc1);
-      if (d == 0) {
-        p.part_ml[at * 2] = mx;
-        p.part_ml[at * 2 + 1] = lsum;
-      }
+      const int64_t at = ((int64_t)(ut.t0 + r / nh) * a.Hq + h0 + r % nh) * p.n_split + split;
+      *reinterpret_cast<float4*>(p.part_o + at * D + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mx, lsum);
     }
+  }
+  if constexpr (WIDE) {
+    if (p.n_split == 1) return;
+    // Join over the cluster: the results stay in shared memory, and each CTA
+    // reads its share of the rows from all of them. Every thread of every CTA
+    // comes to both barriers, those of splits without keys too.
+    cluster_arrive();
+    cluster_wait();
+    const uint32_t o_at = sbase, ml_at = smem_u32(s_ml);
+    for (int idx = split * kRowThreads + tid; idx < rows * (D / 4); idx += p.n_split * kRowThreads) {
+      const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+      float2 ml[8];
+      float4 o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.f);
+        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < p.n_split) {
+          ml[i] = ld_cluster2(cluster_map(ml_at + r * 8, i));
+          o[i] = ld_cluster4(cluster_map(o_at + (r * D + d) * 4, i));
+        }
+      }
+      float mx = -INFINITY, lsum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, ml[i].x);
+      const float mu = mx == -INFINITY ? 0.f : mx;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;  // saw no key
+        const float c = ex2(ml[i].x - mu);
+        lsum += ml[i].y * c;
+        acc.x += o[i].x * c;
+        acc.y += o[i].y * c;
+        acc.z += o[i].z * c;
+        acc.w += o[i].w * c;
+      }
+      const float inv = lsum > 0.f ? 1.0f / lsum : (lsum == 0.f ? 0.f : lsum);
+      *reinterpret_cast<uint2*>(out_at(r) + d) =
+          make_uint2(Half<T>::pack(acc.x * inv, acc.y * inv), Half<T>::pack(acc.z * inv, acc.w * inv));
+    }
+    cluster_arrive();  // nobody leaves while its shared memory is read
+    cluster_wait();
   }
 }
 
@@ -411,6 +485,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 
 // Shape of the launch.
 struct AttnPlan {
+  bool wide;   // one CTA a SM, splits join inside a thread-block cluster
   bool chunk;  // 128-row tiles on tcgen05 instead of 16-row units
   int tq, gh, nhg, n_split, split_len;
   int64_t units;
@@ -457,23 +532,41 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   }
   longest = (longest + kRowKeys - 1) / kRowKeys * kRowKeys;
   int64_t len = ((int64_t)a.split_len + kRowKeys - 1) / kRowKeys * kRowKeys;
+  const int64_t slots = 2ll * sms;  // resident CTAs of either kernel
+  const int64_t lines = (a.blocks ? r.units : a.batch.N / r.tq + 1) * a.Hkv * r.nhg;
   if (a.split_len <= 0) {
-    // About four CTAs per resident slot (two a SM), but at least 256 keys each
-    // (1,024 in 128-row tiles, whose partial results are larger).
-    const int64_t lines = (a.blocks ? r.units : a.batch.N / r.tq + 1) * a.Hkv * r.nhg;
-    const int64_t want = 8ll * sms;
-    const int64_t splits = lines >= want ? 1 : (want + lines - 1) / lines;
-    len = (longest + splits - 1) / splits;
+    if (r.chunk) {
+      // Tiles are split only to fill the slots, and not below 1,024 keys: a split
+      // costs its tile's start, end and partial results again.
+      const int64_t splits = lines >= slots ? 1 : slots / lines;
+      len = (longest + splits - 1) / splits;
+      if (len < 1024) len = 1024;
+    } else {
+      // Half a wave of lines or more: only the longest are cut, so that a ragged
+      // batch ends together. Fewer: as many splits as a cluster joins with an SM
+      // for each CTA, where that leaves a CTA 2,048 keys at most; else enough for
+      // one wave. 256 keys each at least.
+      len = 4096;
+      if (2 * lines < slots) {
+        const int64_t fit = sms / lines < 8 ? sms / lines : 8;
+        const int64_t splits = fit >= 2 && longest <= fit * 2048 ? fit : (slots + lines - 1) / lines;
+        len = (longest + splits - 1) / splits;
+        if (len < 256) len = 256;
+        if (len > 4096) len = 4096;
+      }
+    }
     len = (len + kRowKeys - 1) / kRowKeys * kRowKeys;
-    const int least = r.chunk ? 1024 : 256;
-    if (len < least) len = least;
   }
   if (len > longest) len = longest;
   // The join reads every split: no more than 512 of them.
   if ((longest + len - 1) / len > 512) len = ((longest + 511) / 512 + kRowKeys - 1) / kRowKeys * kRowKeys;
   r.split_len = (int)len;
   r.n_split = (int)((longest + len - 1) / len);
-  r.part = r.n_split > 1 ? (int64_t)a.batch.N * a.Hq * r.n_split * (a.D + 2) : 0;
+  // A cluster's CTAs take an SM each and wait for one another: only where the
+  // whole grid is resident at once.
+  const int64_t grid = r.units * r.n_split * a.Hkv * r.nhg;
+  r.wide = !r.chunk && r.n_split <= 8 && grid <= sms;
+  r.part = r.n_split > 1 && !r.wide ? (int64_t)a.batch.N * a.Hq * r.n_split * (a.D + 2) : 0;
   return r;
 }
 
@@ -485,17 +578,34 @@ static int launch_join(const PagedAttnParams& prm, cudaStream_t stream) {
   return SA_OK;
 }
 
-template <typename T, int D, bool SPARSE, int ROWS>
+template <typename T, int D, bool SPARSE, int ROWS, bool WIDE>
 static int launch_rows(const PagedAttnParams& prm, const AttnPlan& r, cudaStream_t stream) {
-  auto kern = paged_rows_kernel<T, D, SPARSE, ROWS>;
+  using Cfg = PagedRowCfg<D, ROWS, WIDE>;
+  auto kern = paged_rows_kernel<T, D, SPARSE, ROWS, WIDE>;
   static bool done[64];
-  int rc = sa_smem_once(reinterpret_cast<const void*>(kern), PagedRowCfg<D>::kSmemBytes, done);
+  int rc = sa_smem_once(reinterpret_cast<const void*>(kern), Cfg::kSmemBytes, done);
   if (rc) return rc;
   const int64_t gx = r.units * r.n_split, gy = (int64_t)prm.a.Hkv * r.nhg;
   if (gx > 0x7fffffff || gy > 65535) return sa_fail(SA_ERR_INVALID, "paged attention: batch too large");
-  kern<<<dim3((unsigned)gx, (unsigned)gy), kRowThreads, PagedRowCfg<D>::kSmemBytes, stream>>>(prm);
-  SA_CHECK_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)gx, (unsigned)gy);
+  cfg.blockDim = dim3(Cfg::kThreads);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = WIDE ? (unsigned)r.n_split : 1u;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = WIDE ? 1 : 0;
+  SA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, prm));
   return SA_OK;
+}
+
+template <typename T, int D, bool SPARSE, int ROWS>
+static int launch_rows(const PagedAttnParams& prm, const AttnPlan& r, cudaStream_t stream) {
+  return r.wide ? launch_rows<T, D, SPARSE, ROWS, true>(prm, r, stream)
+                   : launch_rows<T, D, SPARSE, ROWS, false>(prm, r, stream);
 }
 
 template <typename T, int D>
@@ -513,7 +623,21 @@ static int launch_any(PagedAttnParams& prm, const AttnPlan& r, cudaStream_t stre
     rc = sa_paged_chunk_launch(prm, r.units, stream);
   else
     rc = launch_rows_any<T, D>(prm, r, stream);
-  return rc || r.n_split == 1 ? rc : launch_join<T, D>(prm, stream);
+  return rc || r.n_split == 1 || r.wide ? rc : launch_join<T, D>(prm, stream);
+}
+
+// Map over a page pool, box at most 64 slots of one head of one page: all D
+// columns as 64-column regions one behind the other (5-D: column, slot, region,
+// head, page), or 64 columns (4-D: column, slot, head, page).
+static int sa_page_map(CUtensorMap* m, const sa_paged_attn_args& a, const void* base, const int64_t strides[3],
+                       bool whole, const char* name) {
+  const int box = a.batch.page_size < kRowKeys ? a.batch.page_size : kRowKeys;
+  if (!whole)
+    return sa_make_map(m, base, a.batch.num_pages, a.Hkv, a.batch.page_size, a.D, strides, box, name);
+  const int64_t dims[5] = {64, a.batch.page_size, a.D / 64, a.Hkv, a.batch.num_pages};
+  const int64_t st[4] = {strides[2], 64, strides[1], strides[0]};
+  const int b[5] = {64, box, a.D / 64, 1, 1};
+  return sa_make_map_nd(m, base, 5, dims, st, b, name);
 }
 
 static int check_paged_attn(const sa_paged_attn_args* a) {
@@ -568,13 +692,8 @@ extern "C" int sa_paged_attn(const sa_paged_attn_args* a, sa_stream_t stream_) {
   if (r.workspace(*a) > 0 && !a->workspace) return sa_fail(SA_ERR_INVALID, "paged attention: workspace is NULL");
   PagedAttnParams prm;
   memset(&prm, 0, sizeof(prm));
-  const int box = a->batch.page_size < kRowKeys ? a->batch.page_size : kRowKeys;
-  if ((rc = sa_make_map(&prm.tm_k, a->k_pages, a->batch.num_pages, a->Hkv, a->batch.page_size, a->D, a->k_strides,
-                        box, "k_pages")))
-    return rc;
-  if ((rc = sa_make_map(&prm.tm_v, a->v_pages, a->batch.num_pages, a->Hkv, a->batch.page_size, a->D, a->v_strides,
-                        box, "v_pages")))
-    return rc;
+  if ((rc = sa_page_map(&prm.tm_k, *a, a->k_pages, a->k_strides, !r.chunk, "k_pages"))) return rc;
+  if ((rc = sa_page_map(&prm.tm_v, *a, a->v_pages, a->v_strides, true, "v_pages"))) return rc;
   prm.a = *a;
   prm.a.split_len = r.split_len;
   prm.tq = r.tq;

@@ -7,7 +7,8 @@
 // dozen tokens still fills the tile. Two CTAs fit on an SM: the softmax of one
 // runs while the other's products do. Six warps:
 //   warp 0     TMA producer: Q (one box of heads x tokens), then 64-key chunks of
-//              K and V, a box per page and 64 columns, into rings (SWIZZLE_128B).
+//              K and V into rings (SWIZZLE_128B): a box per page, for K also per 64
+//              columns, since its rows are the product's N and have to lie evenly.
 //              A page past the keys, or a bad one, is loaded from behind the last
 //              page of the map, which reads as zeros.
 //   warp 1     tcgen05.mma issuer: S = Q K^T into one of two TMEM buffers, then
@@ -142,14 +143,14 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   const sa_paged_batch& bt = a.batch;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.gh, ps = bt.page_size;
-  // Tiles of late tokens see the most keys: they come first, all heads of a
-  // token tile side by side.
+  // The tiles that see the most keys come first (448 tiles of 3.2k to 11.2k keys:
+  // 299 -> 282 us), all heads of a token tile side by side.
   const int kvh = blockIdx.x % a.Hkv;
   const int64_t rest = blockIdx.x / a.Hkv;
   const int split = (int)(rest % p.n_split);
-  const int64_t unit = units - 1 - rest / p.n_split;
+  const int64_t unit = longest_first(bt, rest / p.n_split, units, p.tq);
   UnitTokens ut;
-  if (!unit_tokens(bt, unit, p.tq, p.err, ut)) return;
+  if (unit < 0 || !unit_tokens(bt, unit, p.tq, p.err, ut)) return;
   const int keys = unit_keys(ut, a.max_len);
   if (keys < min(ut.pos0 + ut.n, ut.len) && lane == 0) record_error(p.err, SA_DEV_ERR_INDEX);
   const int pps = ps < N ? N / ps : 1, spp = ps > N ? ps / N : 1, box = min(ps, N);  // pages per chunk, chunks per page
@@ -281,12 +282,9 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
       }
       if (lane == 0) mbar_arrive_expect_tx(smem_u32(&bar_v_full[vs]), Cfg::kKVBytes);
       __syncwarp();
-      if (lane < pps) {
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-          tma_load_4d(sV + vs * Cfg::kKVBytes + r * N * 128 + lane * box * 128, &p.tm_v, smem_u32(&bar_v_full[vs]),
-                      r * 64, off, kvh, pg);
-      }
+      if (lane < pps)
+        tma_load_5d(sV + vs * Cfg::kKVBytes + lane * box * (D * 2), &p.tm_v, smem_u32(&bar_v_full[vs]), 0, off, 0, kvh,
+                    pg);
       ++vn;
     }
     if (__any_sync(0xffffffffu, bad) && lane == 0) record_error(p.err, SA_DEV_ERR_INDEX);
@@ -305,7 +303,9 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
       constexpr uint32_t idesc_pv = chunk_idesc<T>(D, true);
       const uint64_t q_desc = smem_desc_sw128(sQ, 16, 1024);
       const uint64_t k_desc = smem_desc_sw128(sK, 16, 1024);
-      const uint64_t v_desc = smem_desc_sw128(sV, N * 128, 1024);
+      // V lies page by page, a page's 64-column regions one behind the other.
+      const uint64_t v_desc = smem_desc_sw128(sV, box * 128, 1024);
+      const int lks = 31 - __clz(box) - 4;  // log2 of the 16-key steps per page
       // S = Q K^T of chunk g; its commit frees the K slot and tells the softmax.
       auto next_s = [&](int g) -> bool {
         const int ks = g % NSK;
@@ -334,7 +334,9 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         const uint64_t vst = v_desc + (uint64_t)((vs * Cfg::kKVBytes) >> 4);
 #pragma unroll
         for (int k = 0; k < N / 16; ++k)
-          mma_ts(tmem, pbuf + k * 8, vst + ((k * 2048) >> 4), idesc_pv, (k > 0 || g > 0) ? 1u : 0u);
+          mma_ts(tmem, pbuf + k * 8,
+                 vst + (uint64_t)(((k >> lks) * box * (D * 2) + (k & ((1 << lks) - 1)) * 2048) >> 4), idesc_pv,
+                 (k > 0 || g > 0) ? 1u : 0u);
         mma_commit(smem_u32(&bar_v_empty[vs]));  // PV of chunk g retired: V slot free, O holds it
       }
       mma_commit(smem_u32(&bar_drain));
@@ -484,11 +486,12 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         if (!__all_sync(FULL, ok)) { ok = false; break; }
         const uint32_t v0 = sV + (g % NSV) * Cfg::kKVBytes;
         for (int i = row; i < N * 8 * R; i += 128) {
-          const int r = (i >> 3) % N;
+          // 16-byte piece i: page, region, row
+          const int jp = i / (box * 8 * R), r = jp * box + ((i >> 3) & (box - 1));
           int key = off + r;
           if constexpr (SPARSE) {
-            const int blk = meta_blk[ms][r / box];
-            key = blk < 0 ? 0 : blk * ps + off + r % box;  // (none: read as zeros)
+            const int blk = meta_blk[ms][jp];
+            key = blk < 0 ? 0 : blk * ps + off + r - jp * box;  // (none: read as zeros)
           }
           if (key >= keys)
             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v0 + i * 16), "r"(0u) : "memory");
@@ -613,7 +616,7 @@ int sa_paged_chunk_launch(PagedAttnParams& prm, int64_t units, cudaStream_t stre
   const int64_t dims[4] = {a.D, a.Hq, a.batch.N, 1};
   const int64_t strides[3] = {a.q_strides[1], a.q_strides[0], 8};
   const int box[4] = {64, prm.gh, prm.tq, 1};
-  int rc = sa_make_map4(&prm.tm_q, a.q, dims, strides, box, "q");
+  int rc = sa_make_map_nd(&prm.tm_q, a.q, 4, dims, strides, box, "q");
   if (rc) return rc;
   if (a.dtype == SA_BF16)
     return a.D == 128 ? launch_chunk_any<__nv_bfloat16, 128>(prm, units, stream)
