@@ -174,6 +174,7 @@ struct PagedAttnParams {
   int32_t gh;       // heads per unit
   int32_t nhg;      // units per kv head and token tile: ceil(group / gh)
   int32_t n_split;  // grid splits: ceil(max_len / split_len)
+  int32_t cluster;  // the splits of a tile are one thread-block cluster and join in it (chunk kernel)
   float scale_log2;
   float* part_o;    // [N, Hq, n_split, D]
   float* part_ml;   // [N, Hq, n_split, 2]

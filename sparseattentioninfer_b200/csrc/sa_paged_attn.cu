@@ -485,7 +485,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
 
 // Shape of the launch.
 struct AttnPlan {
-  bool wide;   // one CTA a SM, splits join inside a thread-block cluster
+  bool cluster;  // chunk kernel: splits join inside a cluster
+  bool wide;   // rows kernel: one CTA a SM, splits join inside a thread-block cluster
   bool chunk;  // 128-row tiles on tcgen05 instead of 16-row units
   int tq, gh, nhg, n_split, split_len;
   int64_t units;
@@ -494,14 +495,23 @@ struct AttnPlan {
   int64_t workspace(const sa_paged_attn_args& a) const { return part + units * a.Hkv * (page_cap + (page_cap > 0)); }
 };
 
+// The largest power of two that is at most n and at most `most`, 1 at least.
+static int64_t pow2_below(int64_t n, int64_t most) {
+  int64_t r = 1;
+  while (2 * r <= n && 2 * r <= most) r *= 2;
+  return r;
+}
+
 static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   AttnPlan r;
   const int group = a.Hq / a.Hkv;
-  // One 16-row unit holds all rows of a sequence: the rows kernel reads the
-  // cache once, and nothing is gained by wider tiles.
   const int64_t cap = (int64_t)a.batch.max_pages * a.batch.page_size;
   int64_t longest = a.max_len < cap ? a.max_len : cap;  // keys of the longest unit
-  r.chunk = group <= 128 && (int64_t)a.max_q * group > kRowMax;
+  // Up to three 16-row units a sequence the rows kernel, above the chunk kernel:
+  // 16 sequences of 16k keys, 8 kv heads of 128: 32 rows 217 us against 180, 64
+  // rows 367 against 178; of 2k keys 34 against 37 and 61 against 40; one sequence
+  // of 2k keys 11 against 13 and 14 against 14.
+  r.chunk = group <= 128 && (int64_t)a.max_q * group > 48;
   r.page_cap = 0;
   if (a.blocks && r.chunk) {
     // A tile reads the union of its tokens' pages once, the rows kernel every
@@ -533,14 +543,27 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   longest = (longest + kRowKeys - 1) / kRowKeys * kRowKeys;
   int64_t len = ((int64_t)a.split_len + kRowKeys - 1) / kRowKeys * kRowKeys;
   const int64_t slots = 2ll * sms;  // resident CTAs of either kernel
-  const int64_t lines = (a.blocks ? r.units : a.batch.N / r.tq + 1) * a.Hkv * r.nhg;
+  // Those of a grid of clusters: up to 8 CTAs have to fit in one GPC, which leaves
+  // some of its SMs over (18 clusters of 8 CTAs that take an SM each, 144 in all,
+  // ran in two waves on 148 SMs, 16 in one).
+  const int64_t resident = slots * 7 / 8;
+  // Tiles that the batch has at least: full ones, and one a sequence.
+  const int64_t full = a.batch.N / r.tq + 1, some = a.batch.B < a.batch.N ? a.batch.B : a.batch.N;
+  const int64_t lines = (r.tq == 1 ? r.units : full > some ? full : some) * a.Hkv * r.nhg;
   if (a.split_len <= 0) {
     if (r.chunk) {
-      // Tiles are split only to fill the slots, and not below 1,024 keys: a split
-      // costs its tile's start, end and partial results again.
-      const int64_t splits = lines >= slots ? 1 : slots / lines;
+      // Tiles are split only to fill the slots: a split costs its tile's start, end
+      // and partial results again. Up to 8 splits join in a cluster, 256 keys each
+      // at least; more of them, of 1,024 keys, only where 8 would leave over 1,280
+      // (one sequence of 16k keys, 32 rows: 38 us with 8, 29 with 16).
+      int64_t splits = pow2_below(resident / (lines < 1 ? 1 : lines), 8);
+      int least = 256;
+      if (splits == 8 && longest > 8 * 1280) {
+        splits = slots / lines;
+        least = 1024;
+      }
       len = (longest + splits - 1) / splits;
-      if (len < 1024) len = 1024;
+      if (len < least) len = least;
     } else {
       // Half a wave of lines or more: only the longest are cut, so that a ragged
       // batch ends together. Fewer: as many splits as a cluster joins with an SM
@@ -548,7 +571,7 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
       // one wave. 256 keys each at least.
       len = 4096;
       if (2 * lines < slots) {
-        const int64_t fit = sms / lines < 8 ? sms / lines : 8;
+        const int64_t fit = pow2_below(resident / 2 / lines, 8);
         const int64_t splits = fit >= 2 && longest <= fit * 2048 ? fit : (slots + lines - 1) / lines;
         len = (longest + splits - 1) / splits;
         if (len < 256) len = 256;
@@ -562,11 +585,11 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   if ((longest + len - 1) / len > 512) len = ((longest + 511) / 512 + kRowKeys - 1) / kRowKeys * kRowKeys;
   r.split_len = (int)len;
   r.n_split = (int)((longest + len - 1) / len);
-  // A cluster's CTAs take an SM each and wait for one another: only where the
-  // whole grid is resident at once.
+  // A cluster's CTAs wait for one another: only where the whole grid is resident at once.
   const int64_t grid = r.units * r.n_split * a.Hkv * r.nhg;
-  r.wide = !r.chunk && r.n_split <= 8 && grid <= sms;
-  r.part = r.n_split > 1 && !r.wide ? (int64_t)a.batch.N * a.Hq * r.n_split * (a.D + 2) : 0;
+  r.wide = !r.chunk && r.n_split <= 8 && grid <= (r.n_split > 1 ? resident / 2 : sms);
+  r.cluster = r.chunk && r.n_split > 1 && r.n_split <= 8 && grid <= resident;
+  r.part = r.n_split > 1 && !r.wide && !r.cluster ? (int64_t)a.batch.N * a.Hq * r.n_split * (a.D + 2) : 0;
   return r;
 }
 
@@ -623,7 +646,7 @@ static int launch_any(PagedAttnParams& prm, const AttnPlan& r, cudaStream_t stre
     rc = sa_paged_chunk_launch(prm, r.units, stream);
   else
     rc = launch_rows_any<T, D>(prm, r, stream);
-  return rc || r.n_split == 1 || r.wide ? rc : launch_join<T, D>(prm, stream);
+  return rc || r.part == 0 ? rc : launch_join<T, D>(prm, stream);
 }
 
 // Map over a page pool, box at most 64 slots of one head of one page: all D
@@ -700,6 +723,7 @@ extern "C" int sa_paged_attn(const sa_paged_attn_args* a, sa_stream_t stream_) {
   prm.gh = r.gh;
   prm.nhg = r.nhg;
   prm.n_split = r.n_split;
+  prm.cluster = r.cluster;
   prm.scale_log2 = a->scale * 1.4426950408889634f;
   prm.part_o = a->workspace;
   prm.part_ml = a->workspace ? a->workspace + (int64_t)a->batch.N * a->Hq * r.n_split * a->D : nullptr;

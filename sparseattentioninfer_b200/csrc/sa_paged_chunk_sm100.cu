@@ -145,9 +145,11 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   const int G = p.gh, ps = bt.page_size;
   // The tiles that see the most keys come first (448 tiles of 3.2k to 11.2k keys:
   // 299 -> 282 us), all heads of a token tile side by side.
-  const int kvh = blockIdx.x % a.Hkv;
-  const int64_t rest = blockIdx.x / a.Hkv;
-  const int split = (int)(rest % p.n_split);
+  // (The splits of a cluster are neighbours.)
+  const int64_t tile = p.cluster ? blockIdx.x / p.n_split : blockIdx.x;
+  const int kvh = (int)(tile % a.Hkv);
+  const int64_t rest = p.cluster ? tile / a.Hkv * p.n_split : tile / a.Hkv;
+  const int split = (int)(p.cluster ? blockIdx.x % p.n_split : rest % p.n_split);
   const int64_t unit = longest_first(bt, rest / p.n_split, units, p.tq);
   UnitTokens ut;
   if (unit < 0 || !unit_tokens(bt, unit, p.tq, p.err, ut)) return;
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
     chunks = (n_union + pps - 1) / pps * spp;
   } else {
     chunks = (keys + N - 1) / N;
-    if (split >= unit_splits(keys, a.split_len)) return;
+    if (split >= unit_splits(keys, a.split_len) && !p.cluster) return;
   }
   const int c0 = split * (a.split_len / N);  // chunks [c0, c0 + nch)
   const int nch = max(0, (split == p.n_split - 1 ? chunks : min(chunks, c0 + a.split_len / N)) - c0);
@@ -176,16 +178,66 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   auto part_at = [&](int r) {
     return ((int64_t)(ut.t0 + r / G) * a.Hq + kvh * G + r % G) * p.n_split + split;
   };
-  if (nch == 0 || (sQ & 1023u)) {  // block-uniform
-    if (threadIdx.x == 0 && (sQ & 1023u)) record_error(p.err, SA_DEV_ERR_INDEX);
+  if (sQ & 1023u) {  // (the same in every CTA of the launch)
+    if (threadIdx.x == 0) record_error(p.err, SA_DEV_ERR_INDEX);
+    return;
+  }
+  // A cluster's CTAs leave their results here: rows of D + 4 floats (so that the
+  // writes of neighbouring rows take different banks), maximum and sum behind.
+  constexpr int OS = D + 4;
+  static_assert(kChM * OS * 4 + kChM * 8 <= Cfg::kSmemBytes, "results do not fit");
+  float* s_o = reinterpret_cast<float*>(smem_raw);
+  float2* s_ml = reinterpret_cast<float2*>(smem_raw + kChM * OS * 4);
+  auto join = [&]() {
+    cluster_arrive();
+    cluster_wait();
+    const int n = p.n_split;
+    for (int idx = split * kChThreads + threadIdx.x; idx < rows * (D / 4); idx += n * kChThreads) {
+      const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+      float2 ml[8];
+      float4 o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.f);
+        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < n) {
+          ml[i] = ld_cluster2(cluster_map(smem_u32(s_ml + r), i));
+          o[i] = ld_cluster4(cluster_map(smem_u32(s_o + r * OS + d), i));
+        }
+      }
+      float mx = -INFINITY, lsum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, ml[i].x);
+      const float mu = mx == -INFINITY ? 0.f : mx;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;  // saw no key: wrote no row
+        const float c = ex2(ml[i].x - mu);
+        lsum += ml[i].y * c;
+        acc.x += o[i].x * c;
+        acc.y += o[i].y * c;
+        acc.z += o[i].z * c;
+        acc.w += o[i].w * c;
+      }
+      const float inv = lsum > 0.f ? 1.0f / lsum : (lsum == 0.f ? 0.f : lsum);
+      *reinterpret_cast<uint2*>(out_row(r) + d) =
+          make_uint2(Half<T>::pack(acc.x * inv, acc.y * inv), Half<T>::pack(acc.z * inv, acc.w * inv));
+    }
+    cluster_arrive();  // nobody leaves while its shared memory is read
+    cluster_wait();
+  };
+  if (nch == 0) {  // block-uniform
     for (int r = threadIdx.x; r < rows; r += kChThreads) {
       if (p.n_split == 1) {
         for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(out_row(r) + d) = make_uint4(0, 0, 0, 0);
+      } else if (p.cluster) {
+        s_ml[r] = make_float2(-INFINITY, 0.f);
       } else {
-        p.part_ml[part_at(r) * 2] = -INFINITY;
-        p.part_ml[part_at(r) * 2 + 1] = 0.f;
+        *reinterpret_cast<float2*>(p.part_ml + part_at(r) * 2) = make_float2(-INFINITY, 0.f);
       }
     }
+    if (p.cluster) join();
     return;
   }
 
@@ -512,7 +564,19 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
       tmem_wait_ld();
 #pragma unroll
       for (int cc = 0; cc < D / 32; ++cc) reg_fence32(o32[cc]);
-      if (p.n_split > 1) {
+      if (p.cluster) {
+        // (every copy into the rings and every product has retired: V's last slot says so)
+        if (row_ok) {
+          float4* dst = reinterpret_cast<float4*>(s_o + row * OS);
+#pragma unroll
+          for (int cc = 0; cc < D / 32; ++cc)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              dst[cc * 8 + i] = make_float4(__uint_as_float(o32[cc][4 * i]), __uint_as_float(o32[cc][4 * i + 1]),
+                                            __uint_as_float(o32[cc][4 * i + 2]), __uint_as_float(o32[cc][4 * i + 3]));
+          s_ml[row] = make_float2(m_ref, l);
+        }
+      } else if (p.n_split > 1) {
         if (row_ok) {
           const int64_t at = part_at(row);
           float4* dst = reinterpret_cast<float4*>(p.part_o + at * D);
@@ -579,6 +643,7 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, Cfg::kTmemCols);
+  if (p.cluster) join();
 }
 
 template <typename T, int D, bool SPARSE>
@@ -596,8 +661,18 @@ static int launch_chunk(const PagedAttnParams& prm, int64_t units, cudaStream_t 
         prm, units);
     SA_CHECK_CUDA(cudaGetLastError());
   }
-  kern<<<(unsigned)blocks, kChThreads, ChunkCfg<D>::kSmemBytes, stream>>>(prm, units);
-  SA_CHECK_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kChThreads);
+  cfg.dynamicSmemBytes = ChunkCfg<D>::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = prm.cluster ? (unsigned)prm.n_split : 1u;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = prm.cluster ? 1 : 0;
+  SA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, prm, units));
   return SA_OK;
 }
 
