@@ -192,8 +192,17 @@ __device__ __forceinline__ int unit_splits(int keys, int split_len) { return max
 
 }  // namespace sa
 
+// Strides of dimensions with one element may hold anything: n strides over sizes, set to the ones
+// they would have in a contiguous tensor whose last dimension has D elements.
+inline void sa_fix_strides(int64_t* strides, const int64_t* sizes, int n, int64_t D) {
+  int64_t inner = D;
+  for (int i = n - 1; i >= 0; --i) {
+    if (sizes[i] == 1) strides[i] = inner;
+    inner *= sizes[i];
+  }
+}
 // Host checks of a packed batch (sa_paged_append.cu).
-int sa_check_paged_batch(const sa_paged_batch* b, const char* what);
+int sa_check_paged_batch(sa_paged_batch* b, const char* what);
 // Pages of 16-bit elements: 16-byte aligned base, strides (page, head, slot) that are multiples of 8
 // elements, below 2^36 elements, and at least D.
 int sa_check_pages(const void* base, const int64_t strides[3], int D, const char* name);

@@ -4,12 +4,16 @@
 //
 //   y = x * rsqrt(mean(x^2) + eps) * w,  o[d] = y[d] cos[d] -+ y[d +- D/2] sin[d]
 //
-// Every value is read once and written once, so the memory rate bounds it. Two
-// kinds of warps share the grid: q warps take up to kQHeads heads of one token
-// (its cos/sin row stays in registers); page warps take the new tokens of one
-// page of one kv head, in order, so that the page's bounds are the running
-// minimum and maximum of one warp: no atomics, and the same bounds however the
-// tokens were cut into calls.
+// Every value is read once and written once, so the memory rate bounds it. Half
+// a warp holds a row, each lane the same part of both halves of the head, so that
+// a value and its rotation partner share a lane and two rows share each step of
+// the norm's sum. Two kinds of warps share the grid: page warps, which go first
+// (they run longest), take the new tokens of one page of one kv head, so that
+// the page's bounds are the minimum and maximum of one warp: no atomics, and the
+// same bounds however the tokens were cut into calls; q warps take up to kQHeads
+// heads at once of one token, whose cos/sin row stays in registers.
+// 10,819 tokens, 32/8 heads of 128: 52 us, 5.2 TB/s; six CTAs a SM with two pairs of
+// tokens in flight (eight: 59 us, and spills; five: 55; four with four pairs: 57).
 #include "sa_paged.cuh"
 
 namespace sa {
@@ -17,99 +21,163 @@ namespace sa {
 constexpr int kQHeads = 8;
 constexpr int kAppendWarps = 4;
 
-template <typename T, int E>
-__device__ __forceinline__ void load_row(const T* p, float (&x)[E]) {
-  if constexpr (E == 4) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    const float2 a = Half<T>::unpack(u.x), b = Half<T>::unpack(u.y);
-    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
-  } else {
-    const float2 a = Half<T>::unpack(*reinterpret_cast<const uint32_t*>(p));
-    x[0] = a.x; x[1] = a.y;
+// A lane's part of a head as it lies in memory: values [H l, H l + H) of the
+// first half and of the second, l = lane % 16, H = 2 or 4.
+template <int H>
+struct Raw {
+  uint32_t w[H];
+  template <typename T>
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (H == 4) {
+      const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + 16 * H);
+      w[0] = a.x; w[1] = a.y; w[2] = b.x; w[3] = b.y;
+    } else {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+      w[1] = *reinterpret_cast<const uint32_t*>(p + 16 * H);
+    }
   }
-}
-// Stores the rounded row and gives back the values as stored.
-template <typename T, int E>
-__device__ __forceinline__ void store_row(T* p, float (&x)[E]) {
-  uint32_t w[E / 2];
+  template <typename T>
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (H == 4) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(p + 16 * H) = make_uint2(w[2], w[3]);
+    } else {
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+      *reinterpret_cast<uint32_t*>(p + 16 * H) = w[1];
+    }
+  }
+};
+// The same in 32 bits, in pairs for the packed arithmetic.
+template <int H>
+struct Part {
+  uint64_t lo[H / 2], hi[H / 2];
+  template <typename T>
+  __device__ __forceinline__ void from(const Raw<H>& r) {
 #pragma unroll
-  for (int i = 0; i < E / 2; ++i) {
-    w[i] = Half<T>::pack(x[2 * i], x[2 * i + 1]);
-    const float2 r = Half<T>::unpack(w[i]);
-    x[2 * i] = r.x;
-    x[2 * i + 1] = r.y;
+    for (int i = 0; i < H / 2; ++i) {
+      const float2 a = Half<T>::unpack(r.w[i]), b = Half<T>::unpack(r.w[H / 2 + i]);
+      lo[i] = f2pack(a.x, a.y);
+      hi[i] = f2pack(b.x, b.y);
+    }
   }
-  if constexpr (E == 4)
-    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-  else
-    *reinterpret_cast<uint32_t*>(p) = w[0];
-}
+  template <typename T>
+  __device__ __forceinline__ void to(Raw<H>& r) const {
+#pragma unroll
+    for (int i = 0; i < H / 2; ++i) {
+      float x, y;
+      f2unpack(lo[i], x, y);
+      r.w[i] = Half<T>::pack(x, y);
+      f2unpack(hi[i], x, y);
+      r.w[H / 2 + i] = Half<T>::pack(x, y);
+    }
+  }
+};
+constexpr uint64_t kSigns = 0x8000000080000000ull;
 
-// RMSNorm (when w is given) and rotation of one row held by a warp, E values a
-// lane: element d's partner d +- D/2 sits in lane ^ 16 at the same slot.
-template <int E>
-__device__ __forceinline__ void norm_rope(float (&x)[E], bool norm, const float (&w)[E], const float (&c)[E],
-                                          const float (&s)[E], float eps, int lane) {
+// What a row is turned by: the weight's and the table's products (weight 1 without a norm).
+template <int H>
+struct Turn {
+  uint64_t lc[H / 2], hs[H / 2], hc[H / 2], ls[H / 2];  // o_lo = r (lo lc + hi hs), o_hi = r (hi hc + lo ls)
+  template <typename T>
+  __device__ __forceinline__ void from(const Raw<H>& cos, const Raw<H>& sin, const Part<H>& w) {
+    Part<H> c, s;
+    c.template from<T>(cos);
+    s.template from<T>(sin);
+#pragma unroll
+    for (int i = 0; i < H / 2; ++i) {
+      lc[i] = mul2(c.lo[i], w.lo[i]);
+      hs[i] = mul2(s.lo[i], w.hi[i]) ^ kSigns;
+      hc[i] = mul2(c.hi[i], w.hi[i]);
+      ls[i] = mul2(s.hi[i], w.lo[i]);
+    }
+  }
+};
+
+// RMSNorm (when asked) and rotation of the row that half a warp holds.
+template <typename T, int H>
+__device__ __forceinline__ void norm_rope(Raw<H>& row, bool norm, const Turn<H>& t, float eps) {
+  Part<H> x, o;
+  x.template from<T>(row);
+  float r = 1.f;
   if (norm) {
-    float ss = 0.f;
+    uint64_t s2 = 0ull;
 #pragma unroll
-    for (int e = 0; e < E; ++e) ss += x[e] * x[e];
+    for (int i = 0; i < H / 2; ++i) s2 = fma2(x.hi[i], x.hi[i], fma2(x.lo[i], x.lo[i], s2));
+    float a, b;
+    f2unpack(s2, a, b);
+    float ss = a + b;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = rsqrtf(ss / (32 * E) + eps);
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = x[e] * r * w[e];
+    for (int k = 8; k > 0; k >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, k);
+    r = rsqrtf(ss / (32 * H) + eps);
   }
+  const uint64_t r2 = f2pack(r, r);
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const float partner = __shfl_xor_sync(0xffffffffu, x[e], 16);
-    x[e] = x[e] * c[e] + (lane < 16 ? -partner : partner) * s[e];
+  for (int i = 0; i < H / 2; ++i) {
+    o.lo[i] = mul2(r2, fma2(x.hi[i], t.hs[i], mul2(x.lo[i], t.lc[i])));
+    o.hi[i] = mul2(r2, fma2(x.lo[i], t.ls[i], mul2(x.hi[i], t.hc[i])));
   }
+  o.template to<T>(row);
 }
 
-template <typename T, int E>
-__global__ void __launch_bounds__(32 * kAppendWarps)
-    paged_append_kernel(const __grid_constant__ sa_paged_append_args a, int64_t q_units, int64_t page_units,
-                        int32_t* err) {
-  constexpr int D = 32 * E;
-  const int lane = threadIdx.x & 31;
+template <typename T, int H>
+__global__ void __launch_bounds__(32 * kAppendWarps, 6)
+    paged_append_kernel(const __grid_constant__ sa_paged_append_args a, uint32_t page_units, uint32_t q_units,
+                        uint32_t q_heads, int32_t* err) {
+  constexpr int D = 32 * H;
+  const int lane = threadIdx.x & 31, half = lane >> 4;
   const sa_paged_batch& bt = a.batch;
-  int64_t u = (int64_t)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
-  const int at = E * lane;
+  uint32_t u = blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
+  const int at = H * (lane & 15);
   const T* cos_t = reinterpret_cast<const T*>(a.cos) + at;
   const T* sin_t = reinterpret_cast<const T*>(a.sin) + at;
   const T* qkv = reinterpret_cast<const T*>(a.qkv) + at;
+  Part<H> w;
+#pragma unroll
+  for (int i = 0; i < H / 2; ++i) w.lo[i] = w.hi[i] = f2pack(1.f, 1.f);
+  auto load_weight = [&](const void* p) {
+    if (!p) return;
+    Raw<H> x;
+    x.load(reinterpret_cast<const T*>(p) + at);
+    w.template from<T>(x);
+  };
 
-  if (u < q_units) {
-    const int groups = (a.Hq + kQHeads - 1) / kQHeads;
-    const int h0 = (int)(u % groups) * kQHeads;
+  if (u >= page_units) {
+    // ---------------------------------------------------------------- q
+    u -= page_units;
+    if (u >= q_units) return;
+    const uint32_t groups = (a.Hq + q_heads - 1) / q_heads, token = u / groups;
+    const int h_first = (int)((u - token * groups) * q_heads), h_end = min(h_first + (int)q_heads, a.Hq);
     UnitTokens ut;
-    if (!unit_tokens(bt, u / groups, 1, err, ut)) return;
+    if (!unit_tokens(bt, token, 1, err, ut)) return;
     if (ut.pos0 >= a.positions) {
       if (lane == 0) record_error(err, SA_DEV_ERR_INDEX);
       return;
     }
-    float w[E], c[E], s[E], x[kQHeads][E];
-    const T* src = qkv + (int64_t)ut.t0 * a.qkv_st + (int64_t)h0 * D;
-#pragma unroll
-    for (int h = 0; h < kQHeads; ++h)
-      if (h0 + h < a.Hq) load_row<T, E>(src + h * D, x[h]);
-    load_row<T, E>(cos_t + (int64_t)ut.pos0 * D, c);
-    load_row<T, E>(sin_t + (int64_t)ut.pos0 * D, s);
-    if (a.q_weight) load_row<T, E>(reinterpret_cast<const T*>(a.q_weight) + at, w);
+    const T* src = qkv + (int64_t)ut.t0 * a.qkv_st;
     T* dst = reinterpret_cast<T*>(a.q_out) + (int64_t)ut.t0 * a.q_strides[0] + at;
+    Turn<H> turn;
+    {
+      Raw<H> c, s;
+      c.load(cos_t + (int64_t)ut.pos0 * D);
+      s.load(sin_t + (int64_t)ut.pos0 * D);
+      load_weight(a.q_weight);
+      turn.template from<T>(c, s, w);
+    }
+    for (int h0 = h_first + half; h0 - half < h_end; h0 += kQHeads) {
+      Raw<H> x[kQHeads / 2];
 #pragma unroll
-    for (int h = 0; h < kQHeads; ++h)
-      if (h0 + h < a.Hq) {
-        norm_rope<E>(x[h], a.q_weight != nullptr, w, c, s, a.eps, lane);
-        store_row<T, E>(dst + (int64_t)(h0 + h) * a.q_strides[1], x[h]);
+      for (int i = 0; i < kQHeads / 2; ++i) x[i].load(src + min(h0 + 2 * i, h_end - 1) * D);
+#pragma unroll
+      for (int i = 0; i < kQHeads / 2; ++i) {
+        norm_rope<T, H>(x[i], a.q_weight != nullptr, turn, a.eps);
+        if (h0 + 2 * i < h_end) x[i].store(dst + (int64_t)(h0 + 2 * i) * a.q_strides[1]);
       }
+    }
     return;
   }
-  u -= q_units;
-  if (u >= page_units) return;
-  const int kvh = (int)(u % a.Hkv);
-  const int64_t run = u / a.Hkv;
+  // ------------------------------------------------------------------ k, v
+  const uint32_t run = u / (uint32_t)a.Hkv;
+  const int kvh = (int)(u - run * (uint32_t)a.Hkv);
   // Runs of one page: sequence b takes the numbers from cu_q[b] / page_size + 2 b
   // on, which leaves room for the pages that n tokens can touch, at most
   // floor(n / page_size) + 2.
@@ -122,7 +190,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps)
     return;
   }
   const int64_t start = len - (c1 - c0);
-  const int64_t page_at = start / ps + (run - (c0 / ps + 2 * (int64_t)b));
+  const int64_t page_at = start / ps + ((int64_t)run - (c0 / ps + 2 * (int64_t)b));
   const int p0 = (int)max(start, page_at * ps), p1 = (int)min((int64_t)len, (page_at + 1) * ps);
   if (p0 >= p1) return;
   const int page = page_at < bt.max_pages ? __ldg(bt.table + b * bt.table_stride + page_at) : -1;
@@ -137,57 +205,83 @@ __global__ void __launch_bounds__(32 * kAppendWarps)
                          (int64_t)kvh * a.b_strides[1] + at
                    : nullptr;
   const T* ks = qkv + ((int64_t)c0 - start) * a.qkv_st + (int64_t)(a.Hq + kvh) * D;  // + position * qkv_st
-  float w[E], low[E], high[E];
-  if (a.k_weight) load_row<T, E>(reinterpret_cast<const T*>(a.k_weight) + at, w);
+  load_weight(a.k_weight);
+  float low[2 * H], high[2 * H];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
+  for (int e = 0; e < 2 * H; ++e) {
     low[e] = INFINITY;
     high[e] = -INFINITY;
   }
+  auto widen = [&](const Raw<H>& lo, const Raw<H>& hi) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const float2 l = Half<T>::unpack(lo.w[i]), h = Half<T>::unpack(hi.w[i]);
+      low[2 * i] = min_nan(low[2 * i], l.x);
+      low[2 * i + 1] = min_nan(low[2 * i + 1], l.y);
+      high[2 * i] = max_nan(high[2 * i], h.x);
+      high[2 * i + 1] = max_nan(high[2 * i + 1], h.y);
+    }
+  };
   if (bd && p0 % ps) {
-    load_row<T, E>(bd, low);
-    load_row<T, E>(bd + a.b_strides[2], high);
+    Raw<H> l, h;
+    l.load(bd);
+    h.load(bd + a.b_strides[2]);
+    widen(l, h);
   }
-  constexpr int U = 4;  // tokens in flight
-  for (int p = p0; p < end; p += U) {
-    float k[U][E], v[U][E], c[U][E], s[U][E];
+  constexpr int U = 2;  // pairs of tokens in flight, a token per half warp
+  for (int p = p0 + half; p - half < end; p += 2 * U) {
+    Raw<H> k[U], v[U], c[U], s[U];
 #pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (p + i < end) {
-        const T* src = ks + (int64_t)(p + i) * a.qkv_st;
-        load_row<T, E>(src, k[i]);
-        load_row<T, E>(src + (int64_t)a.Hkv * D, v[i]);
-        load_row<T, E>(cos_t + (int64_t)(p + i) * D, c[i]);
-        load_row<T, E>(sin_t + (int64_t)(p + i) * D, s[i]);
+    for (int i = 0; i < U; ++i) {
+      const int q = min(p + 2 * i, end - 1);
+      const T* src = ks + (int64_t)q * a.qkv_st;
+      k[i].load(src);
+      v[i].load(src + (int64_t)a.Hkv * D);
+      c[i].load(cos_t + (int64_t)q * D);
+      s[i].load(sin_t + (int64_t)q * D);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int q = p + 2 * i, slot = q & (ps - 1);
+      Turn<H> turn;
+      turn.template from<T>(c[i], s[i], w);
+      norm_rope<T, H>(k[i], a.k_weight != nullptr, turn, a.eps);
+      if (q < end) {
+        k[i].store(kd + (int64_t)slot * a.k_strides[2]);
+        v[i].store(vd + (int64_t)slot * a.v_strides[2]);
+        widen(k[i], k[i]);
       }
-#pragma unroll
-    for (int i = 0; i < U; ++i)
-      if (p + i < end) {
-        const int slot = (p + i) % ps;
-        norm_rope<E>(k[i], a.k_weight != nullptr, w, c[i], s[i], a.eps, lane);
-        store_row<T, E>(kd + (int64_t)slot * a.k_strides[2], k[i]);
-        store_row<T, E>(vd + (int64_t)slot * a.v_strides[2], v[i]);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          low[e] = min_nan(low[e], k[i][e]);
-          high[e] = max_nan(high[e], k[i][e]);
-        }
-      }
+    }
   }
   if (bd) {
-    store_row<T, E>(bd, low);
-    store_row<T, E>(bd + a.b_strides[2], high);
+    Raw<H> out;  // the half warps' bounds together; one stores the low ones, the other the high ones
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      float l[2], h[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[e] = min_nan(low[2 * i + e], __shfl_xor_sync(0xffffffffu, low[2 * i + e], 16));
+        h[e] = max_nan(high[2 * i + e], __shfl_xor_sync(0xffffffffu, high[2 * i + e], 16));
+      }
+      out.w[i] = half == 0 ? Half<T>::pack(l[0], l[1]) : Half<T>::pack(h[0], h[1]);
+    }
+    out.store(bd + (half == 0 ? 0 : a.b_strides[2]));
   }
 }
 
 template <typename T, int E>
 static int launch_append(const sa_paged_append_args& a, cudaStream_t stream) {
-  const int64_t q_units = (int64_t)a.batch.N * ((a.Hq + kQHeads - 1) / kQHeads);
+  // Heads per q warp: 8, and more of them in large batches, where a warp's start
+  // counts more than the number of warps.
+  const int64_t eights = (a.Hq + kQHeads - 1) / kQHeads;
+  int64_t per = a.batch.N * eights / 8192;
+  per = per < 1 ? 1 : per > eights ? eights : per;
+  const int64_t q_units = (int64_t)a.batch.N * ((a.Hq + per * kQHeads - 1) / (per * kQHeads));
   const int64_t page_units = (a.batch.N / a.batch.page_size + 2 * (int64_t)a.batch.B) * a.Hkv;
-  const int64_t blocks = (q_units + page_units + kAppendWarps - 1) / kAppendWarps;
-  if (blocks > 0x7fffffff) return sa_fail(SA_ERR_INVALID, "paged append: too many tokens");
-  paged_append_kernel<T, E>
-      <<<(unsigned)blocks, 32 * kAppendWarps, 0, stream>>>(a, q_units, page_units, sa_device_error_ptr());
+  if (q_units + page_units > 0x7fffff00) return sa_fail(SA_ERR_INVALID, "paged append: too many tokens");
+  paged_append_kernel<T, E><<<(unsigned)((q_units + page_units + kAppendWarps - 1) / kAppendWarps), 32 * kAppendWarps,
+                              0, stream>>>(a, (uint32_t)page_units, (uint32_t)q_units, (uint32_t)(per * kQHeads),
+                                           sa_device_error_ptr());
   SA_CHECK_CUDA(cudaGetLastError());
   return SA_OK;
 }
@@ -196,7 +290,7 @@ static int launch_append(const sa_paged_append_args& a, cudaStream_t stream) {
 
 using namespace sa;
 
-int sa_check_paged_batch(const sa_paged_batch* b, const char* what) {
+int sa_check_paged_batch(sa_paged_batch* b, const char* what) {
   if (!b->table || !b->cu_q || !b->seq_lens) return sa_fail(SA_ERR_INVALID, "%s: NULL batch pointer", what);
   if (b->B <= 0 || b->N <= 0 || b->max_pages <= 0 || b->num_pages <= 0)
     return sa_fail(SA_ERR_INVALID, "%s: non-positive size (B=%d N=%d max_pages=%d num_pages=%d)", what, b->B, b->N,
@@ -205,7 +299,8 @@ int sa_check_paged_batch(const sa_paged_batch* b, const char* what) {
     return sa_fail(SA_ERR_UNSUPPORTED, "%s: page_size %d unsupported (16, 32, 64 or 128)", what, b->page_size);
   if ((int64_t)b->max_pages * b->page_size > 0x7fffffff)
     return sa_fail(SA_ERR_INVALID, "%s: max_pages * page_size must stay below 2^31", what);
-  if (b->table_stride < 0 || (b->B > 1 && b->table_stride < b->max_pages))
+  if (b->B == 1) b->table_stride = b->max_pages;
+  if (b->table_stride < b->max_pages)
     return sa_fail(SA_ERR_INVALID, "%s: table_stride %lld below max_pages %d", what, (long long)b->table_stride,
                    b->max_pages);
   return SA_OK;
@@ -230,8 +325,9 @@ int sa_check_pages(const void* base, const int64_t strides[3], int D, const char
   return SA_OK;
 }
 
-extern "C" int sa_paged_append(const sa_paged_append_args* a, sa_stream_t stream_) {
-  if (!a) return sa_fail(SA_ERR_INVALID, "args is NULL");
+extern "C" int sa_paged_append(const sa_paged_append_args* args, sa_stream_t stream_) {
+  if (!args) return sa_fail(SA_ERR_INVALID, "args is NULL");
+  sa_paged_append_args own = *args, *a = &own;
   int rc = sa_check_paged_batch(&a->batch, "paged append");
   if (rc) return rc;
   if (!a->qkv || !a->cos || !a->sin || !a->q_out) return sa_fail(SA_ERR_INVALID, "NULL tensor pointer");
@@ -240,6 +336,13 @@ extern "C" int sa_paged_append(const sa_paged_append_args* a, sa_stream_t stream
   if (a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv)
     return sa_fail(SA_ERR_INVALID, "Hq=%d not a multiple of Hkv=%d", a->Hq, a->Hkv);
   if (a->positions <= 0) return sa_fail(SA_ERR_INVALID, "positions must be positive");
+  const int64_t rows[2] = {a->batch.N, a->Hq}, pool[3] = {a->batch.num_pages, a->Hkv, a->batch.page_size},
+                bnd[3] = {a->batch.num_pages, a->Hkv, 2};
+  if (a->batch.N == 1) a->qkv_st = (int64_t)(a->Hq + 2 * a->Hkv) * a->D;
+  sa_fix_strides(a->q_strides, rows, 2, a->D);
+  sa_fix_strides(a->k_strides, pool, 3, a->D);
+  sa_fix_strides(a->v_strides, pool, 3, a->D);
+  sa_fix_strides(a->b_strides, bnd, 3, a->D);
   if ((rc = sa_check_pages(a->k_pages, a->k_strides, a->D, "k_pages"))) return rc;
   if ((rc = sa_check_pages(a->v_pages, a->v_strides, a->D, "v_pages"))) return rc;
   if (a->bounds && (rc = sa_check_pages(a->bounds, a->b_strides, a->D, "bounds"))) return rc;

@@ -663,8 +663,8 @@ static int sa_page_map(CUtensorMap* m, const sa_paged_attn_args& a, const void* 
   return sa_make_map_nd(m, base, 5, dims, st, b, name);
 }
 
-static int check_paged_attn(const sa_paged_attn_args* a) {
-  if (!a) return sa_fail(SA_ERR_INVALID, "args is NULL");
+// Checks the arguments, and fills in the strides of dimensions with one element.
+static int check_paged_attn(sa_paged_attn_args* a) {
   int rc = sa_check_paged_batch(&a->batch, "paged attention");
   if (rc) return rc;
   if (!a->q || !a->out) return sa_fail(SA_ERR_INVALID, "NULL tensor pointer");
@@ -675,6 +675,13 @@ static int check_paged_attn(const sa_paged_attn_args* a) {
   if (a->max_q < 1 || a->max_len < 1) return sa_fail(SA_ERR_INVALID, "max_q and max_len must be at least 1");
   if (!(a->scale > 0.f) || a->scale > 3.0e38f) return sa_fail(SA_ERR_INVALID, "scale must be positive and finite");
   if (a->split_len < 0 || a->num_sms < 0) return sa_fail(SA_ERR_INVALID, "negative split_len or num_sms");
+  const int64_t rows[2] = {a->batch.N, a->Hq}, pool[3] = {a->batch.num_pages, a->Hkv, a->batch.page_size},
+                lists[2] = {a->batch.N, a->Hkv};
+  sa_fix_strides(a->q_strides, rows, 2, a->D);
+  sa_fix_strides(a->o_strides, rows, 2, a->D);
+  sa_fix_strides(a->k_strides, pool, 3, a->D);
+  sa_fix_strides(a->v_strides, pool, 3, a->D);
+  sa_fix_strides(a->blocks_strides, lists, 2, a->n_blocks);
   if ((rc = sa_check_pages(a->k_pages, a->k_strides, a->D, "k_pages"))) return rc;
   if ((rc = sa_check_pages(a->v_pages, a->v_strides, a->D, "v_pages"))) return rc;
   const int64_t* st[2] = {a->q_strides, a->o_strides};
@@ -695,7 +702,9 @@ static int check_paged_attn(const sa_paged_attn_args* a) {
 
 using namespace sa;
 
-extern "C" int sa_paged_attn_workspace(const sa_paged_attn_args* a, int64_t* floats) {
+extern "C" int sa_paged_attn_workspace(const sa_paged_attn_args* args, int64_t* floats) {
+  if (!args) return sa_fail(SA_ERR_INVALID, "args is NULL");
+  sa_paged_attn_args own = *args, *a = &own;
   int rc = check_paged_attn(a);
   if (rc) return rc;
   if (!floats) return sa_fail(SA_ERR_INVALID, "floats is NULL");
@@ -706,7 +715,9 @@ extern "C" int sa_paged_attn_workspace(const sa_paged_attn_args* a, int64_t* flo
   return SA_OK;
 }
 
-extern "C" int sa_paged_attn(const sa_paged_attn_args* a, sa_stream_t stream_) {
+extern "C" int sa_paged_attn(const sa_paged_attn_args* args, sa_stream_t stream_) {
+  if (!args) return sa_fail(SA_ERR_INVALID, "args is NULL");
+  sa_paged_attn_args own = *args, *a = &own;
   int rc = check_paged_attn(a);
   if (rc) return rc;
   const int sms = a->num_sms > 0 ? a->num_sms : sa_num_sms();

@@ -457,8 +457,9 @@ static int launch_select(const sa_paged_select_args& a, cudaStream_t stream) {
 
 using namespace sa;
 
-extern "C" int sa_paged_select(const sa_paged_select_args* a, sa_stream_t stream_) {
-  if (!a) return sa_fail(SA_ERR_INVALID, "args is NULL");
+extern "C" int sa_paged_select(const sa_paged_select_args* args, sa_stream_t stream_) {
+  if (!args) return sa_fail(SA_ERR_INVALID, "args is NULL");
+  sa_paged_select_args own = *args, *a = &own;
   int rc = sa_check_paged_batch(&a->batch, "paged select");
   if (rc) return rc;
   if (!a->q || !a->out) return sa_fail(SA_ERR_INVALID, "NULL tensor pointer");
@@ -473,6 +474,11 @@ extern "C" int sa_paged_select(const sa_paged_select_args* a, sa_stream_t stream
                    kSelMaxKeep, a->first, a->recent, a->keep);
   if (a->batch.max_pages > kSelMaxPages)
     return sa_fail(SA_ERR_UNSUPPORTED, "max_pages %d above %d", a->batch.max_pages, kSelMaxPages);
+  const int64_t rows[2] = {a->batch.N, a->Hq}, lists[2] = {a->batch.N, a->Hkv},
+                bnd[3] = {a->batch.num_pages, a->Hkv, 2};
+  sa_fix_strides(a->q_strides, rows, 2, a->D);
+  sa_fix_strides(a->out_strides, lists, 2, a->keep);
+  sa_fix_strides(a->b_strides, bnd, 3, a->D);
   if ((rc = sa_check_pages(a->bounds, a->b_strides, a->D, "bounds"))) return rc;
   if (a->q_strides[0] < 0 || a->q_strides[1] < 0 || a->out_strides[0] < a->keep || a->out_strides[1] < a->keep)
     return sa_fail(SA_ERR_INVALID, "bad strides of q or out");

@@ -449,19 +449,25 @@ def topk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: int
 # ---------------------------------------------------------------------------
 # Paged cache, packed ragged batches (sa_paged_*.cu)
 # ---------------------------------------------------------------------------
+_NO3, _NO4 = (0, 0, 0), (0, 0, 0, 0)
 _HALF = {torch.bfloat16: _capi.SA_BF16, torch.float16: _capi.SA_FP16}
 
 
 def _paged_check(name: str, dtype: torch.dtype, dev: int, halves, ints) -> None:
     """Type, device and layout of a paged op's tensors: 16-bit ones of ``dtype``,
     int32 ones, all on device ``dev`` with a contiguous last dimension."""
-    for want, ts in ((dtype, halves), (torch.int32, ints)):
-        for t in ts:
-            if t.dtype is not want or t.get_device() != dev:
-                raise TypeError(f"{name}: {want} on cuda:{dev} expected, got {t.dtype} on {t.device}")
-            if t.stride(-1) != 1 and t.shape[-1] > 1:
-                raise ValueError(f"{name}: the last dimension of every tensor must be contiguous, got strides "
-                                 f"{t.stride()} of {tuple(t.shape)}")
+    for t in halves:
+        if t.dtype is not dtype or t.get_device() != dev:
+            raise TypeError(f"{name}: {dtype} on cuda:{dev} expected, got {t.dtype} on {t.device}")
+        if t.stride(-1) != 1:
+            raise ValueError(f"{name}: the last dimension must be contiguous, got strides {t.stride()} of "
+                             f"{tuple(t.shape)}")
+    for t in ints:
+        if t.dtype is not torch.int32 or t.get_device() != dev:
+            raise TypeError(f"{name}: int32 on cuda:{dev} expected, got {t.dtype} on {t.device}")
+        if t.stride(-1) != 1 and t.shape[-1] > 1:
+            raise ValueError(f"{name}: the last dimension must be contiguous, got strides {t.stride()} of "
+                             f"{tuple(t.shape)}")
 
 
 def _paged_dtype(name: str, t: torch.Tensor) -> int:
@@ -473,29 +479,22 @@ def _paged_dtype(name: str, t: torch.Tensor) -> int:
     return code
 
 
-def _outer(t: torch.Tensor, n: int) -> tuple[int, ...]:
-    """Element strides of the first n dimensions; one of a single element gets the
-    stride of a contiguous tensor (torch leaves any value there)."""
-    s, shape = t.stride(), t.shape
-    if 1 not in shape[:n]:
-        return s[:n]
-    return tuple(math.prod(shape[i + 1:]) if shape[i] == 1 else s[i] for i in range(n))
-
-
 def _paged_batch(name: str, N: int, page_table, cu_q, seq_lens, num_pages: int, page_size: int) -> tuple:
     B = seq_lens.numel()
-    if page_table.dim() != 2 or seq_lens.dim() != 1 or cu_q.shape != (B + 1,) or page_table.shape[0] != B:
+    if page_table.dim() != 2 or seq_lens.dim() != 1 or cu_q.dim() != 1 or cu_q.numel() != B + 1 or \
+            page_table.shape[0] != B:
         raise ValueError(f"{name}: page_table [B, pages], cu_q [B + 1] and seq_lens [B] expected, got "
                          f"{tuple(page_table.shape)}, {tuple(cu_q.shape)} and {tuple(seq_lens.shape)}")
-    width = page_table.shape[1]
-    return (page_table.data_ptr(), cu_q.data_ptr(), seq_lens.data_ptr(), page_table.stride(0) if B > 1 else width, B,
-            N, width, num_pages, page_size)
+    return (page_table.data_ptr(), cu_q.data_ptr(), seq_lens.data_ptr(), page_table.stride(0), B, N,
+            page_table.shape[1], num_pages, page_size)
 
 
-def _check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, Hkv: int, D: int) -> None:
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or k_pages.shape[1] != Hkv or k_pages.shape[3] != D:
+def _check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, Hkv: int, D: int):
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or shape[1] != Hkv or shape[3] != D:
         raise ValueError(f"{name}: k_pages / v_pages must be [pages, {Hkv}, page_size, {D}], got "
-                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
+                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
+    return shape[0], shape[2]
 
 
 def _paged_call(fn, args: bytes, dev: int) -> None:
@@ -540,25 +539,25 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor | None, 
     _paged_check(name, qkv.dtype, dev,
                  [t for t in (qkv, cos, sin, k_pages, v_pages, q_out, q_weight, k_weight, k_bounds) if t is not None],
                  (page_table, cu_q, seq_lens))
-    _check_pages(name, k_pages, v_pages, Hkv, D)
+    pages, page_size = _check_pages(name, k_pages, v_pages, Hkv, D)
     if qkv.stride(1) != D or q_out.shape != (N, Hq, D):
         raise ValueError(f"{name}: qkv heads must be contiguous and q_out [N, Hq, D]")
     if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != D or not cos.is_contiguous() or \
             not sin.is_contiguous():
         raise ValueError(f"{name}: cos / sin must be contiguous [positions, {D}]")
-    if (q_weight is not None and q_weight.shape != (D,)) or (k_weight is not None and k_weight.shape != (D,)):
+    if (q_weight is not None and q_weight.numel() != D) or (k_weight is not None and k_weight.numel() != D):
         raise ValueError(f"{name}: weights must be [{D}]")
-    if k_bounds is not None and k_bounds.shape != (k_pages.shape[0], Hkv, 2, D):
+    if k_bounds is not None and k_bounds.shape != (pages, Hkv, 2, D):
         raise ValueError(f"{name}: k_bounds must be [pages, {Hkv}, 2, {D}], got {tuple(k_bounds.shape)}")
-    batch = _paged_batch(name, N, page_table, cu_q, seq_lens, k_pages.shape[0], k_pages.shape[2])
+    batch = _paged_batch(name, N, page_table, cu_q, seq_lens, pages, page_size)
     if N == 0 or batch[4] == 0:
         return q_out
     args = _capi.PAGED_APPEND.pack(
-        *batch, qkv.data_ptr(), qkv.stride(0) if N > 1 else heads * D,
-        q_weight.data_ptr() if q_weight is not None else 0, k_weight.data_ptr() if k_weight is not None else 0,
-        cos.data_ptr(), sin.data_ptr(), q_out.data_ptr(), *_outer(q_out, 2), k_pages.data_ptr(), *_outer(k_pages, 3),
-        v_pages.data_ptr(), *_outer(v_pages, 3), k_bounds.data_ptr() if k_bounds is not None else 0,
-        *(_outer(k_bounds, 3) if k_bounds is not None else (0, 0, 0)), Hq, Hkv, D, cos.shape[0], code, eps)
+        *batch, qkv.data_ptr(), qkv.stride(0), q_weight.data_ptr() if q_weight is not None else 0,
+        k_weight.data_ptr() if k_weight is not None else 0, cos.data_ptr(), sin.data_ptr(), q_out.data_ptr(),
+        *q_out.stride()[:2], k_pages.data_ptr(), *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3],
+        k_bounds.data_ptr() if k_bounds is not None else 0, *(k_bounds.stride()[:3] if k_bounds is not None else _NO3),
+        Hq, Hkv, D, cos.shape[0], code, eps)
     _paged_call(_capi.load().sa_paged_append, args, dev)
     return q_out
 
@@ -592,8 +591,8 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, page_table: torc
     batch = _paged_batch(name, N, page_table, cu_q, seq_lens, pages, page_size)
     if N == 0 or batch[4] == 0:
         return out
-    args = _capi.PAGED_SELECT.pack(*batch, q.data_ptr(), *_outer(q, 2), k_bounds.data_ptr(), *_outer(k_bounds, 3),
-                                   out.data_ptr(), *_outer(out, 2), Hq, Hkv, D, code, keep, first, recent,
+    args = _capi.PAGED_SELECT.pack(*batch, q.data_ptr(), *q.stride()[:2], k_bounds.data_ptr(),
+                                   *k_bounds.stride()[:3], out.data_ptr(), *out.stride()[:2], Hq, Hkv, D, code, keep, first, recent,
                                    N if max_q is None else max_q)
     _paged_call(_capi.load().sa_paged_select, args, dev)
     return out
@@ -601,33 +600,38 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, page_table: torc
 
 def _paged_attn_args(name, q, k_pages, v_pages, page_table, cu_q, seq_lens, out, max_q, max_len, blocks, scale,
                      split_len):
-    """Packed arguments of sa_paged_attn (workspace last), or None for an empty batch."""
+    """Arguments of sa_paged_attn but for the workspace, or None for an empty batch."""
     code = _paged_dtype(name, q)
     if q.dim() != 3 or k_pages.dim() != 4 or out.shape != q.shape:
         raise ValueError(f"{name}: q and out [N, Hq, D] and pages of 4 dimensions expected, got {tuple(q.shape)}, "
                          f"{tuple(out.shape)} and {tuple(k_pages.shape)}")
     N, Hq, D = q.shape
-    pages, Hkv, page_size = k_pages.shape[:3]
+    Hkv = k_pages.shape[1]
     dev = q.get_device()
     _paged_check(name, q.dtype, dev, (q, k_pages, v_pages, out),
                  (page_table, cu_q, seq_lens) if blocks is None else (page_table, cu_q, seq_lens, blocks))
-    _check_pages(name, k_pages, v_pages, Hkv, D)
-    if blocks is not None and (blocks.dim() != 3 or blocks.shape[:2] != (N, Hkv)):
+    pages, page_size = _check_pages(name, k_pages, v_pages, Hkv, D)
+    if blocks is None:
+        kept = _NO4
+    elif blocks.dim() != 3 or blocks.shape[0] != N or blocks.shape[1] != Hkv:
         raise ValueError(f"{name}: blocks must be [{N}, {Hkv}, n], got {tuple(blocks.shape)}")
+    else:
+        kept = (blocks.data_ptr(), *blocks.stride()[:2], blocks.shape[2])
     batch = _paged_batch(name, N, page_table, cu_q, seq_lens, pages, page_size)
     if N == 0 or batch[4] == 0:
         return None
-    return (*batch, q.data_ptr(), out.data_ptr(), *_outer(q, 2), *_outer(out, 2), k_pages.data_ptr(),
-            *_outer(k_pages, 3), v_pages.data_ptr(), *_outer(v_pages, 3),
-            *((0, 0, 0, 0) if blocks is None else (blocks.data_ptr(), *_outer(blocks, 2), blocks.shape[2])),
-            Hq, Hkv, D, code, 1.0 / math.sqrt(D) if scale is None else scale, N if max_q is None else max_q,
-            page_table.shape[1] * page_size if max_len is None else max_len, 0 if split_len is None else split_len,
-            _num_sms(q.device))
+    return (*batch, q.data_ptr(), out.data_ptr(), *q.stride()[:2], *out.stride()[:2], k_pages.data_ptr(),
+            *k_pages.stride()[:3], v_pages.data_ptr(), *v_pages.stride()[:3], *kept, Hq, Hkv, D, code,
+            1.0 / math.sqrt(D) if scale is None else scale, N if max_q is None else max_q,
+            batch[6] * page_size if max_len is None else max_len, 0 if split_len is None else split_len,
+            _NUM_SMS.get(dev) or _num_sms(q.device))
 
 
-def _paged_workspace(args, dev: int) -> int:
+def _paged_workspace(packed: bytes) -> int:
     n = ctypes.c_int64(0)
-    _capi.check(_capi.load().sa_paged_attn_workspace(_capi.PAGED_ATTN.pack(*args, 0), ctypes.byref(n)))
+    rc = _capi.load().sa_paged_attn_workspace(packed, ctypes.byref(n))
+    if rc:
+        _capi.check(rc)
     return n.value
 
 
@@ -638,7 +642,7 @@ def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, v_pages: t
     """float32 elements of workspace that paged_attention with these arguments needs."""
     args = _paged_attn_args("paged_attention_workspace", q, k_pages, v_pages, page_table, cu_q, seq_lens, q, max_q,
                             max_len, blocks, None, split_len)
-    return 0 if args is None else _paged_workspace(args, q.get_device())
+    return 0 if args is None else _paged_workspace(_capi.PAGED_ATTN.pack(*args, 0))
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -660,22 +664,22 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     call keeps to itself (allocated per call when None)."""
     name = "paged_attention"
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = torch.empty_like(q)
     args = _paged_attn_args(name, q, k_pages, v_pages, page_table, cu_q, seq_lens, out, max_q, max_len, blocks, scale,
                             split_len)
     if args is None:
         return out
     dev = q.get_device()
-    need = _paged_workspace(args, dev)
-    ptr = 0
+    packed = _capi.PAGED_ATTN.pack(*args, 0)
+    need = _paged_workspace(packed)
     if need:
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.float32, device=q.device)
         elif workspace.dtype != torch.float32 or workspace.get_device() != dev or not workspace.is_contiguous() or \
                 workspace.numel() < need:
             raise ValueError(f"{name}: workspace must be {need} contiguous float32 on cuda:{dev}")
-        ptr = workspace.data_ptr()
-    _paged_call(_capi.load().sa_paged_attn, _capi.PAGED_ATTN.pack(*args, ptr), dev)
+        packed = _capi.PAGED_ATTN.pack(*args, workspace.data_ptr())
+    _paged_call(_capi.load().sa_paged_attn, packed, dev)
     return out
 
 
