@@ -164,6 +164,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// 64-key chunks of one of n parts of a tile.
+__host__ __device__ __forceinline__ int tile_part(int chunks, int n) { return (chunks + n - 1) / n; }
+
 // One launch of the attention kernels.
 struct PagedAttnParams {
   CUtensorMap tm_q;  // the chunk kernel's
@@ -174,6 +177,7 @@ struct PagedAttnParams {
   int32_t gh;       // heads per unit
   int32_t nhg;      // units per kv head and token tile: ceil(group / gh)
   int32_t n_split;  // grid splits: ceil(max_len / split_len)
+  int32_t chunk;    // the chunk kernel's launch
   int32_t cluster;  // the splits of a tile are one thread-block cluster and join in it (chunk kernel)
   float scale_log2;
   float* part_o;    // [N, Hq, n_split, D]

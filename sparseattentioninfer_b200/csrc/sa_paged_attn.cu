@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
   UnitTokens ut;
   if (!unit_tokens(a.batch, t, 1, nullptr, ut)) return;
   int n = p.n_split;
-  if (!sparse) {
+  if (!sparse && !p.chunk) {
     // The splits that the token's unit ran: as far as its last token sees.
     const int c0 = __ldg(a.batch.cu_q + ut.b), c1 = __ldg(a.batch.cu_q + ut.b + 1);
     const int in = (ut.t0 - c0) % p.tq;
@@ -552,18 +552,19 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   const int64_t lines = (r.tq == 1 ? r.units : full > some ? full : some) * a.Hkv * r.nhg;
   if (a.split_len <= 0) {
     if (r.chunk) {
-      // Tiles are split only to fill the slots: a split costs its tile's start, end
-      // and partial results again. Up to 8 splits join in a cluster, 256 keys each
-      // at least; more of them, of 1,024 keys, only where 8 would leave over 1,280
-      // (one sequence of 16k keys, 32 rows: 38 us with 8, 29 with 16).
-      int64_t splits = pow2_below(resident / (lines < 1 ? 1 : lines), 8);
-      int least = 256;
-      if (splits == 8 && longest > 8 * 1280) {
-        splits = slots / lines;
-        least = 1024;
+      // Tiles in n equal parts: as many waves as that takes, of a part's keys and
+      // what a tile costs apart from its keys (start, end, partial results: about
+      // 640 keys' time, and 1,000 more where the parts join through the workspace).
+      int64_t best = 0;
+      len = longest;
+      for (int64_t n = 1; n <= 64 && (n == 1 || longest / n >= 256); n *= 2) {
+        const int64_t waves = (lines * n + slots - 1) / slots;
+        const int64_t cost = waves * (longest / n + 640) + (n > 8 ? 1000 : 0);
+        if (n == 1 || cost < best) {
+          best = cost;
+          len = (longest + n - 1) / n;
+        }
       }
-      len = (longest + splits - 1) / splits;
-      if (len < least) len = least;
     } else {
       // Half a wave of lines or more: only the longest are cut, so that a ragged
       // batch ends together. Fewer: as many splits as a cluster joins with an SM
@@ -585,10 +586,12 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   if ((longest + len - 1) / len > 512) len = ((longest + 511) / 512 + kRowKeys - 1) / kRowKeys * kRowKeys;
   r.split_len = (int)len;
   r.n_split = (int)((longest + len - 1) / len);
-  // A cluster's CTAs wait for one another: only where the whole grid is resident at once.
+  // A cluster's CTAs wait for one another. The rows kernel's splits are of equal
+  // length, and short units leave some of them without keys: clusters only where
+  // the whole grid is resident at once. Tiles are cut into equal parts: always.
   const int64_t grid = r.units * r.n_split * a.Hkv * r.nhg;
   r.wide = !r.chunk && r.n_split <= 8 && grid <= (r.n_split > 1 ? resident / 2 : sms);
-  r.cluster = r.chunk && r.n_split > 1 && r.n_split <= 8 && grid <= resident;
+  r.cluster = r.chunk && r.n_split > 1 && r.n_split <= 8;
   r.part = r.n_split > 1 && !r.wide && !r.cluster ? (int64_t)a.batch.N * a.Hq * r.n_split * (a.D + 2) : 0;
   return r;
 }
@@ -734,6 +737,7 @@ extern "C" int sa_paged_attn(const sa_paged_attn_args* args, sa_stream_t stream_
   prm.gh = r.gh;
   prm.nhg = r.nhg;
   prm.n_split = r.n_split;
+  prm.chunk = r.chunk;
   prm.cluster = r.cluster;
   prm.scale_log2 = a->scale * 1.4426950408889634f;
   prm.part_o = a->workspace;

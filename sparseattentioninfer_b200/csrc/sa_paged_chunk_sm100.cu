@@ -164,10 +164,9 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
     chunks = (n_union + pps - 1) / pps * spp;
   } else {
     chunks = (keys + N - 1) / N;
-    if (split >= unit_splits(keys, a.split_len) && !p.cluster) return;
   }
-  const int c0 = split * (a.split_len / N);  // chunks [c0, c0 + nch)
-  const int nch = max(0, (split == p.n_split - 1 ? chunks : min(chunks, c0 + a.split_len / N)) - c0);
+  // Every tile is cut into n_split parts of its own length: chunks [c0, c0 + nch).
+  const int per = tile_part(chunks, p.n_split), c0 = min(split * per, chunks), nch = min(chunks - c0, per);
   const int rows = ut.n * G;
   const uint32_t sQ = smem_u32(smem_raw), sK = sQ + Cfg::kQBytes, sV = sK + NSK * Cfg::kKVBytes;
 
@@ -233,7 +232,7 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(out_row(r) + d) = make_uint4(0, 0, 0, 0);
       } else if (p.cluster) {
         s_ml[r] = make_float2(-INFINITY, 0.f);
-      } else {
+      } else {  // (the join kernel reads it)
         *reinterpret_cast<float2*>(p.part_ml + part_at(r) * 2) = make_float2(-INFINITY, 0.f);
       }
     }
