@@ -10,8 +10,8 @@
 // the norm's sum. Two kinds of warps share the grid: page warps, which go first
 // (they run longest), take the new tokens of one page of one kv head, so that
 // the page's bounds are the minimum and maximum of one warp: no atomics, and the
-// same bounds however the tokens were cut into calls; q warps take up to kQHeads
-// heads at once of one token, whose cos/sin row stays in registers.
+// same bounds however the tokens were cut into calls (where sequences bring many
+// tokens the CTA's warps share a page); q warps take up to kQHeads heads at once of one token, whose cos/sin row stays in registers.
 // 10,819 tokens, 32/8 heads of 128: 52 us, 5.2 TB/s; six CTAs a SM with two pairs of
 // tokens in flight (eight: 59 us, and spills; five: 55; four with four pairs: 57).
 #include "sa_paged.cuh"
@@ -121,12 +121,14 @@ __device__ __forceinline__ void norm_rope(Raw<H>& row, bool norm, const Turn<H>&
 
 template <typename T, int H>
 __global__ void __launch_bounds__(32 * kAppendWarps, 6)
-    paged_append_kernel(const __grid_constant__ sa_paged_append_args a, uint32_t page_units, uint32_t q_units,
-                        uint32_t q_heads, int32_t* err) {
+    paged_append_kernel(const __grid_constant__ sa_paged_append_args a, uint32_t page_blocks, bool shared,
+                        uint32_t q_units, uint32_t q_heads, int32_t* err) {
   constexpr int D = 32 * H;
   const int lane = threadIdx.x & 31, half = lane >> 4;
   const sa_paged_batch& bt = a.batch;
-  uint32_t u = blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
+  __shared__ float s_low[kAppendWarps][D], s_high[kAppendWarps][D];
+  const int warp = threadIdx.x >> 5;
+  uint32_t u;
   const int at = H * (lane & 15);
   const T* cos_t = reinterpret_cast<const T*>(a.cos) + at;
   const T* sin_t = reinterpret_cast<const T*>(a.sin) + at;
@@ -141,9 +143,9 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 6)
     w.template from<T>(x);
   };
 
-  if (u >= page_units) {
+  if (blockIdx.x >= page_blocks) {
     // ---------------------------------------------------------------- q
-    u -= page_units;
+    u = (blockIdx.x - page_blocks) * kAppendWarps + warp;
     if (u >= q_units) return;
     const uint32_t groups = (a.Hq + q_heads - 1) / q_heads, token = u / groups;
     const int h_first = (int)((u - token * groups) * q_heads), h_end = min(h_first + (int)q_heads, a.Hq);
@@ -176,6 +178,8 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 6)
     return;
   }
   // ------------------------------------------------------------------ k, v
+  // A warp a page, or the CTA's warps together (then all of them leave or stay).
+  u = shared ? blockIdx.x : blockIdx.x * kAppendWarps + warp;
   const uint32_t run = u / (uint32_t)a.Hkv;
   const int kvh = (int)(u - run * (uint32_t)a.Hkv);
   // Runs of one page: sequence b takes the numbers from cu_q[b] / page_size + 2 b
@@ -229,7 +233,8 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 6)
     widen(l, h);
   }
   constexpr int U = 2;  // pairs of tokens in flight, a token per half warp
-  for (int p = p0 + half; p - half < end; p += 2 * U) {
+  const int first = p0 + (shared ? warp * 2 * U : 0), step = 2 * U * (shared ? kAppendWarps : 1);
+  for (int p = first + half; p - half < end; p += step) {
     Raw<H> k[U], v[U], c[U], s[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -253,20 +258,37 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 6)
       }
     }
   }
-  if (bd) {
-    Raw<H> out;  // the half warps' bounds together; one stores the low ones, the other the high ones
+  if (!bd) return;
+  // The half warps' bounds together, and the warps' where they share the page; one
+  // half warp stores the low ones, the other the high ones.
 #pragma unroll
-    for (int i = 0; i < H; ++i) {
-      float l[2], h[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        l[e] = min_nan(low[2 * i + e], __shfl_xor_sync(0xffffffffu, low[2 * i + e], 16));
-        h[e] = max_nan(high[2 * i + e], __shfl_xor_sync(0xffffffffu, high[2 * i + e], 16));
-      }
-      out.w[i] = half == 0 ? Half<T>::pack(l[0], l[1]) : Half<T>::pack(h[0], h[1]);
-    }
-    out.store(bd + (half == 0 ? 0 : a.b_strides[2]));
+  for (int e = 0; e < 2 * H; ++e) {
+    low[e] = min_nan(low[e], __shfl_xor_sync(0xffffffffu, low[e], 16));
+    high[e] = max_nan(high[e], __shfl_xor_sync(0xffffffffu, high[e], 16));
   }
+  if (shared) {
+    if (half == 0) {
+#pragma unroll
+      for (int e = 0; e < 2 * H; ++e) {
+        s_low[warp][e * 16 + lane] = low[e];
+        s_high[warp][e * 16 + lane] = high[e];
+      }
+    }
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int w = 1; w < kAppendWarps; ++w)
+#pragma unroll
+      for (int e = 0; e < 2 * H; ++e) {
+        low[e] = min_nan(low[e], s_low[w][e * 16 + (lane & 15)]);
+        high[e] = max_nan(high[e], s_high[w][e * 16 + (lane & 15)]);
+      }
+  }
+  Raw<H> out;
+#pragma unroll
+  for (int i = 0; i < H; ++i)
+    out.w[i] = half == 0 ? Half<T>::pack(low[2 * i], low[2 * i + 1]) : Half<T>::pack(high[2 * i], high[2 * i + 1]);
+  out.store(bd + (half == 0 ? 0 : a.b_strides[2]));
 }
 
 template <typename T, int E>
@@ -278,10 +300,14 @@ static int launch_append(const sa_paged_append_args& a, cudaStream_t stream) {
   per = per < 1 ? 1 : per > eights ? eights : per;
   const int64_t q_units = (int64_t)a.batch.N * ((a.Hq + per * kQHeads - 1) / (per * kQHeads));
   const int64_t page_units = (a.batch.N / a.batch.page_size + 2 * (int64_t)a.batch.B) * a.Hkv;
-  if (q_units + page_units > 0x7fffff00) return sa_fail(SA_ERR_INVALID, "paged append: too many tokens");
-  paged_append_kernel<T, E><<<(unsigned)((q_units + page_units + kAppendWarps - 1) / kAppendWarps), 32 * kAppendWarps,
-                              0, stream>>>(a, (uint32_t)page_units, (uint32_t)q_units, (uint32_t)(per * kQHeads),
-                                           sa_device_error_ptr());
+  // 16 tokens a sequence and more: four warps a page (680 tokens of 6 sequences,
+  // pages of 128: 16 us with one).
+  const bool shared = a.batch.N / a.batch.B >= 16;
+  const int64_t page_blocks = shared ? page_units : (page_units + kAppendWarps - 1) / kAppendWarps;
+  const int64_t blocks = page_blocks + (q_units + kAppendWarps - 1) / kAppendWarps;
+  if (q_units > 0x7fffffff || blocks > 0x7fffffff) return sa_fail(SA_ERR_INVALID, "paged append: too many tokens");
+  paged_append_kernel<T, E><<<(unsigned)blocks, 32 * kAppendWarps, 0, stream>>>(
+      a, (uint32_t)page_blocks, shared, (uint32_t)q_units, (uint32_t)(per * kQHeads), sa_device_error_ptr());
   SA_CHECK_CUDA(cudaGetLastError());
   return SA_OK;
 }

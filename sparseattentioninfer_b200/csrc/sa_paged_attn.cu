@@ -19,6 +19,7 @@
 // splits of a unit are a thread-block cluster and join through its shared memory
 // (2,048 keys of 8 kv heads: 11.8 -> 7.6 us); others go through the workspace and
 // a second kernel.
+#include <cmath>
 #include <cstring>
 
 #include "sa_paged.cuh"
@@ -513,12 +514,18 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   // of 2k keys 11 against 13 and 14 against 14.
   r.chunk = group <= 128 && (int64_t)a.max_q * group > 48;
   r.page_cap = 0;
-  if (a.blocks && r.chunk) {
-    // A tile reads the union of its tokens' pages once, the rows kernel every
-    // token's pages. Lists that may well cover the table make the union pay.
-    const int64_t tokens = a.max_q < 128 / group ? a.max_q : 128 / group;
-    const int64_t seen = (longest + a.batch.page_size - 1) / a.batch.page_size;
-    r.chunk = tokens * a.n_blocks >= seen && a.batch.max_pages <= kChunkMaxPages;
+  if (a.blocks) {
+    // The rows kernel reads every token's pages, a tile the union of its tokens'.
+    // Both in 64-key steps: 3.2 ns each in all against 6.3 (whole GPU) and no less
+    // than about 0.9 us a step of one tile, 7 us more for the union and the tile's
+    // start. The union is taken as of lists drawn at random; real neighbours share more.
+    const double ps = a.batch.page_size, tokens = a.max_q < 128 / group ? a.max_q : 128 / group;
+    const double seen = ceil((double)longest / ps), kept = a.n_blocks < seen ? a.n_blocks : seen;
+    const double pages = seen * (1. - pow(1. - kept / seen, tokens)), steps = pages * ps / kRowKeys;
+    const double lines = (a.batch.N / (128. / group) + 1.) * a.Hkv;
+    const double rows_us = 0.0032 * a.batch.N * a.Hkv * ceil(kept * ps / kRowKeys);
+    const double tile_us = 7. + fmax(0.0063 * lines * steps, 0.9 * steps / fmax(1., fmin(8., 2 * sms / lines)));
+    r.chunk = r.chunk && a.batch.max_pages <= kChunkMaxPages && tile_us < rows_us;
     if (r.chunk) {
       r.page_cap = (int64_t)(128 / group) * a.n_blocks;
       if (r.page_cap > a.batch.max_pages) r.page_cap = a.batch.max_pages;
