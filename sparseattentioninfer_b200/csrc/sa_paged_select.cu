@@ -95,7 +95,7 @@ struct MidList {
 // ONE: a token a CTA, whose warps share its selection.
 template <typename T, int D, bool ONE>
 __global__ void __launch_bounds__(kSelThreads, 3)
-    paged_select_kernel(const __grid_constant__ sa_paged_select_args a, int tq, int32_t* err) {
+    paged_select_kernel(const __grid_constant__ sa_paged_select_args a, int tq, int parts, int32_t* err) {
   using Cfg = SelectCfg<T, D>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int s_amax[kSelTokens];
@@ -108,7 +108,9 @@ __global__ void __launch_bounds__(kSelThreads, 3)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kvh = blockIdx.y, G = a.Hq / a.Hkv, ps = bt.page_size, W = bt.max_pages;
   UnitTokens ut;
-  if (!unit_tokens(bt, blockIdx.x, tq, err, ut)) return;
+  // In small batches `parts` CTAs, a cluster, score a unit's pages; the first selects.
+  const int part = blockIdx.x % parts;
+  if (!unit_tokens(bt, blockIdx.x / parts, tq, err, ut)) return;
   const int nall = min((ut.pos0 + ut.n - 1) / ps, W - 1) + 1;  // pages that the last token sees
   const int32_t* trow = bt.table + (int64_t)ut.b * bt.table_stride;
   const T* bounds = reinterpret_cast<const T*>(a.bounds) + (int64_t)kvh * a.b_strides[1];
@@ -165,22 +167,32 @@ __global__ void __launch_bounds__(kSelThreads, 3)
         at[Cfg::kPart] = Half<T>::from(fabsf(v) + 0.001953125f);
       }
     }
-    __syncthreads();
+    uint32_t keys_at = smem_u32(keys), amax_at = smem_u32(s_amax), wild_at = smem_u32(s_wild);
+    if (parts > 1) {
+      cluster_arrive();  // the first CTA's maxima are set, and it is there to be written to
+      cluster_wait();
+      keys_at = cluster_map(keys_at, 0);
+      amax_at = cluster_map(amax_at, 0);
+      wild_at = cluster_map(wild_at, 0);
+    } else {
+      __syncthreads();
+    }
+    const int first16 = (part * kSelWarps + warp) * 16, step16 = parts * kSelWarps * 16;
     // Scores. Lane (r, j) = (lane / 4, lane % 4) loads 16 bytes of pages r and r + 8
     // per 32 channels; the channels of a k-step are permuted alike in both operands.
     const int j = lane & 3;
     int page[2];  // read a round ahead
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int p = warp * 16 + (lane >> 2) + 8 * i;
+      const int p = first16 + (lane >> 2) + 8 * i;
       page[i] = p < nall ? __ldg(trow + p) : -1;
     }
-    for (int p0 = warp * 16; p0 < nall; p0 += kSelWarps * 16) {
+    for (int p0 = first16; p0 < nall; p0 += step16) {
       const T* src[2];
       bool have[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int p = p0 + (lane >> 2) + 8 * i, next = p + kSelWarps * 16;
+        const int p = p0 + (lane >> 2) + 8 * i, next = p + step16;
         have[i] = page[i] >= 0 && page[i] < bt.num_pages;
         if (p < nall && !have[i]) record_error(err, SA_DEV_ERR_INDEX);
         src[i] = bounds + (int64_t)(have[i] ? page[i] : 0) * a.b_strides[0] + j * 8;
@@ -228,14 +240,33 @@ __global__ void __launch_bounds__(kSelThreads, 3)
             k = order_key(hi[2 * i + e] + lo[2 * i + e]);
             top = max_nan(top, have[i] ? ab[2 * i + e] : INFINITY);  // a bad page: the row is summed again whole
           }
-          keys[(int64_t)t * W + p] = (uint64_t)k << 32;
+          if (parts == 1)
+            keys[(int64_t)t * W + p] = (uint64_t)k << 32;
+          else
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(keys_at + (uint32_t)(t * W + p) * 8),
+                         "l"((uint64_t)k << 32)
+                         : "memory");
         }
-        if (!(top < 3e38f)) s_wild[t] = 1;
-        else atomicMax(&s_amax[t], __float_as_int(top));
+        if (parts == 1) {
+          if (!(top < 3e38f)) s_wild[t] = 1;
+          else atomicMax(&s_amax[t], __float_as_int(top));
+        } else if (!(top < 3e38f)) {
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(wild_at + t * 4), "r"(1) : "memory");
+        } else {
+          asm volatile("red.relaxed.cluster.shared::cluster.max.s32 [%0], %1;" ::"r"(amax_at + t * 4),
+                       "r"(__float_as_int(top))
+                       : "memory");
+        }
       }
     }
-    __syncthreads();
+    if (parts > 1) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
   }
+  if (part > 0) return;  // (nobody reads from these CTAs)
   // Selection: a warp a token, or the CTA's warps together for a single one.
   constexpr int GW = ONE ? kSelWarps : 1;  // warps per row
   for (int t = ONE ? 0 : warp; t < ut.n; t += kSelWarps) {
@@ -442,14 +473,29 @@ static int launch_select(const sa_paged_select_args& a, cudaStream_t stream) {
   if ((int64_t)tq * a.batch.max_pages * 8 > 65536) tq = 65536 / (a.batch.max_pages * 8);
   if (tq < 1) tq = 1;
   const int64_t units = unit_count(a.batch.N, a.batch.B, tq);
-  if (units > 0x7fffffff) return sa_fail(SA_ERR_INVALID, "paged select: batch too large");
   const int bytes = Cfg::kKeys + tq * a.batch.max_pages * 8;
   static bool done[2][64];
   auto kern = tq == 1 ? paged_select_kernel<T, D, true> : paged_select_kernel<T, D, false>;
   int rc = sa_smem_once(reinterpret_cast<const void*>(kern), Cfg::kKeys + kSelMaxPages * 8, done[tq == 1]);
   if (rc) return rc;
-  kern<<<dim3((unsigned)units, a.Hkv), kSelThreads, bytes, stream>>>(a, tq, sa_device_error_ptr());
-  SA_CHECK_CUDA(cudaGetLastError());
+  // Few units: up to 8 CTAs each, of 128 pages at least, while all are resident at
+  // two a SM (2 tokens, 8 kv heads, 1,270 pages of 16: 22 -> 15 us).
+  const int sms = sa_num_sms();
+  int parts = 1;
+  while (parts < 8 && units * a.Hkv * parts * 2 <= sms * 7 / 4 && a.batch.max_pages / (parts * 2) >= 128) parts *= 2;
+  if (units * parts > 0x7fffffff) return sa_fail(SA_ERR_INVALID, "paged select: batch too large");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * parts), a.Hkv);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = parts;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
+  SA_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, a, tq, parts, sa_device_error_ptr()));
   return SA_OK;
 }
 
