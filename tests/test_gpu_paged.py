@@ -26,7 +26,7 @@ def rope_tables(n, D, dtype, theta=1e6):
     ([0, 7, 100, 3], [37, 0, 65, 1], 6, 2, 128, 32, torch.float16, "slots", 0),            # ragged, one without tokens
     ([63, 64, 1], [130, 129, 300], 20, 4, 64, 64, torch.bfloat16, "wide", 5),
     ([200] * 40, [2] * 40, 9, 3, 128, 128, torch.float16, "heads", 1),
-    ([10], [1000], 16, 16, 64, 128, torch.bfloat16, "slots", 0),
+    ([10], [1000], 16, 8, 64, 128, torch.bfloat16, "slots", 0),
 ])
 @pytest.mark.parametrize("normed", [True, False])
 def test_append(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, normed):
@@ -252,3 +252,191 @@ def test_prefill_then_decode_with_kept_pages():
         assert torch.equal(kept.cpu(), P.select(bt, q, bounds, 5, 1, 2))
         out = ops.paged_attention(q, k, v, *bt.batch, blocks=kept)
         _assert_attention(bt, out, q.cpu(), k, v, 1 / math.sqrt(D), kept)
+
+
+@pytest.mark.parametrize("keep", [None, 4])
+def test_captured_steps_replay_as_the_cache_grows(keep):
+    """One captured decode step (append, select, attend) replayed for a growing,
+    ragged batch equals the same steps run eagerly; the lengths, offsets and page
+    table are read on the device."""
+    Hq, Hkv, D, page, B, steps = 8, 2, 128, 16, 3, 6
+    g = torch.Generator().manual_seed(1)
+    start = [14, 0, 95]
+    w = torch.ones(D, dtype=torch.bfloat16, device=DEV)
+    cos, sin = (t.to(DEV) for t in rope_tables(128, D, torch.bfloat16))
+    table = torch.randperm(40, generator=g)[:B * 8].view(B, 8).int().to(DEV)
+    pool = [torch.randn(40, Hkv, page, D, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2)]
+    inputs = torch.randn(steps, B, Hq + 2 * Hkv, D, generator=g).to(torch.bfloat16).to(DEV)
+    cu = torch.arange(B + 1, dtype=torch.int32, device=DEV)
+    bt = P.Batch(start, [0] * B, Hq=Hq, Hkv=Hkv, D=D, page=page, width=8)
+    bt.table, bt.pages = table.cpu(), 40
+
+    def run(graph):
+        k, v = (t.clone() for t in pool)
+        bounds = P.bounds_of(bt, k).to(DEV)
+        lens = torch.tensor(start, dtype=torch.int32, device=DEV)
+        x = inputs[0].clone()
+
+        def step():
+            lens.add_(1)
+            q = ops.paged_qk_norm_rope_append(x, w, w, cos, sin, k, v, table, cu, lens, Hq=Hq, Hkv=Hkv,
+                                              k_bounds=bounds)
+            blocks = None if keep is None else ops.paged_block_select(q, bounds, table, cu, lens, page_size=page,
+                                                                      keep=keep, max_q=1)
+            return ops.paged_attention(q, k, v, table, cu, lens, max_q=1, blocks=blocks, split_len=64)
+
+        outs = []
+        if graph:
+            cg = torch.cuda.CUDAGraph()
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                step()
+            torch.cuda.current_stream().wait_stream(s)
+            with torch.cuda.graph(cg):
+                out = step()
+            for t, u in zip((k, v), pool):
+                t.copy_(u)
+            bounds.copy_(P.bounds_of(bt, k))
+            lens.copy_(torch.tensor(start, dtype=torch.int32))
+        for i in range(steps):
+            x.copy_(inputs[i])
+            if graph:
+                cg.replay()
+                outs.append(out.clone())
+            else:
+                outs.append(step())
+        return torch.stack(outs), k, v, bounds
+
+    for a, b in zip(run(False), run(True)):
+        assert torch.equal(a, b)
+    assert _capi.device_error() == 0
+
+
+def test_side_stream_and_caller_workspace():
+    bt = P.Batch([700, 30], [1, 1], Hq=4, Hkv=2, D=64, page=32, device=DEV)
+    q, k, v = _qkv(bt)
+    q = q.to(DEV)
+    args = (q, k, v, *bt.batch)
+    kw = dict(max_q=1, max_len=2000, split_len=64)  # more splits than a cluster joins
+    n = ops.paged_attention_workspace(*args, **kw)
+    assert n > 0
+    want = ops.paged_attention(*args, **kw)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    ws = torch.full((n,), float("nan"), device=DEV)
+    with torch.cuda.stream(s):
+        got = ops.paged_attention(*args, workspace=ws, **kw)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    with pytest.raises(ValueError, match="workspace"):
+        ops.paged_attention(*args, workspace=ws[:-1], **kw)
+    _assert_attention(bt, got, q.cpu(), k, v, 1 / math.sqrt(64))
+
+
+def test_pages_past_two_to_the_31_elements():
+    """The pages in use lie behind the first 2^31 elements of the pools."""
+    Hq, Hkv, D, page = 16, 8, 128, 128
+    pages = 2 ** 31 // (Hkv * page * D) + 20
+    bt = P.Batch([300, 5], [4, 150], Hq=Hq, Hkv=Hkv, D=D, page=page, device=DEV)
+    small = [bt.pool(), bt.pool()]
+    big = [torch.empty(pages, Hkv, page, D, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    at = pages - bt.pages
+    for b, s in zip(big, small):
+        b[at:] = s
+    far = (bt.table + at).to(DEV)
+    x = torch.randn(bt.N, Hq + 2 * Hkv, D, generator=bt.g).to(torch.bfloat16).to(DEV)
+    cos, sin = (t.to(DEV) for t in rope_tables(400, D, torch.bfloat16))
+    res = []
+    for (k, v), table in ((small, bt.table.to(DEV)), (big, far)):
+        bounds = torch.zeros(k.shape[0], Hkv, 2, D, dtype=torch.bfloat16, device=DEV)
+        cu, ln = bt.batch[1:]
+        q = ops.paged_qk_norm_rope_append(x, None, None, cos, sin, k, v, table, cu, ln, Hq=Hq, Hkv=Hkv,
+                                          k_bounds=bounds)
+        kept = ops.paged_block_select(q, bounds, table, cu, ln, page_size=page, keep=2)
+        res.append([q, kept] + [ops.paged_attention(q, k, v, table, cu, ln, **kw) for kw in
+                                (dict(max_q=1), dict(max_q=150), dict(blocks=kept, max_q=1), dict(blocks=kept))])
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
+    assert torch.equal(big[0][at:].view(torch.int16), small[0].view(torch.int16))
+    assert _capi.device_error() == 0
+
+
+def test_many_heads_a_group_and_many_sequences():
+    for ctx, new, Hq, Hkv in (([70, 0], [1, 3], 136, 1), ([33] * 70, [1, 2] * 35, 4, 2)):
+        bt = P.Batch(ctx, new, Hq=Hq, Hkv=Hkv, D=64, page=16, device=DEV)
+        q, k, v = _qkv(bt)
+        for kw in ({}, dict(max_q=1)):
+            _assert_attention(bt, ops.paged_attention(q.to(DEV), k, v, *bt.batch, **kw), q, k, v, 0.125)
+
+
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_bad_batches_are_reported_and_left_out(max_q):
+    """What the device finds wrong sets the error word; the sound sequences come out right."""
+    def batch():
+        bt = P.Batch([50, 20, 40], [3, 30, 2], Hq=8, Hkv=2, D=64, page=16, device=DEV, seed=5)
+        return bt, *_qkv(bt)
+
+    def attend(bt, q, k, v, table, cu, lens):
+        out = torch.full(q.shape, 7.0, dtype=q.dtype, device=DEV)
+        ops.paged_attention(q.to(DEV), k, v, table, cu, lens, max_q=max_q, out=out)
+        assert _capi.device_error() == 2
+        assert _capi.device_error() == 0  # read and cleared
+        ref, mag = P.attention(bt, q, k, v, 0.125)
+        ok = ((out.cpu().double() - ref).abs() <= P.attention_tolerance(ref, mag, q.dtype)).all(-1).all(-1)
+        return out, [bool(ok[s:s + n].all()) for s, n in zip(bt.starts, bt.new)]
+
+    bt, q, k, v = batch()
+    table, cu, lens = bt.batch
+    for bad in (-1, bt.pages, 2 ** 30):  # a page that is not there: its keys are left out
+        t = table.clone()
+        t[1, 0] = bad
+        _, good = attend(bt, q, k, v, t, cu, lens)
+        assert good == [True, False, True]
+    n = lens.clone()
+    n[1] = 29  # fewer keys than new tokens
+    out, good = attend(bt, q, k, v, table, cu, n)
+    assert good == [True, False, True] and (out[3:33] == 7).all()
+    n[1] = 16 * bt.width + 1  # more keys than the table holds
+    _, good = attend(bt, q, k, v, table, cu, n)
+    assert good[0] and good[2]
+    c = cu.clone()
+    c[3] = bt.N + 9  # rows that are not there
+    out, good = attend(bt, q, k, v, table, c, lens)
+    assert good == [True, True, False]
+    blocks = _random_blocks(bt, 4)
+    blocks[4, 1] = torch.tensor([2, 2, -1, -1])  # not ascending
+    blocks[5, 0] = torch.tensor([0, 3, 10 ** 6, -1])  # behind the token
+    got = torch.zeros_like(q, device=DEV)
+    ops.paged_attention(q.to(DEV), k, v, table, cu, lens, max_q=max_q, out=got, blocks=blocks.to(DEV))
+    assert _capi.device_error() == 2
+    ref, mag = P.attention(bt, q, k, v, 0.125, blocks.where(blocks < 99, -1))
+    ok = ((got.cpu().double() - ref).abs() <= P.attention_tolerance(ref, mag, q.dtype)).flatten(1).all(1)
+    assert ok[[i for i in range(bt.N) if i not in (4, 5)]].all()
+    # select and append
+    bounds = P.bounds_of(bt, k).to(DEV)
+    t = table.clone()
+    t[1, 1] = bt.pages
+    got = ops.paged_block_select(q.to(DEV), bounds, t, cu, lens, page_size=16, keep=2, first=0, recent=1).cpu()
+    assert _capi.device_error() == 2
+    want = P.select(bt, q, bounds, 2, 0, 1)
+    assert torch.equal(got[:3], want[:3]) and torch.equal(got[33:], want[33:])
+    cos, sin = (x.to(DEV) for x in rope_tables(52, 64, torch.bfloat16))  # position 52 has no angle
+    x = torch.randn(bt.N, 12, 64, generator=bt.g).to(torch.bfloat16).to(DEV)
+    kb = k.clone()
+    ops.paged_qk_norm_rope_append(x, None, None, cos, sin, kb, v.clone(), t, cu, lens, Hq=8, Hkv=2, k_bounds=bounds)
+    assert _capi.device_error() == 2
+    changed = (kb.view(torch.int16) != k.view(torch.int16)).flatten(2).any(-1).any(-1).nonzero().flatten().tolist()
+    allowed = {int(table[0, 3]), int(table[1, 2]), int(table[1, 3]), int(table[2, 2])}
+    assert set(changed) <= allowed and _capi.device_error() == 0
+
+
+def test_a_sequence_with_nan_does_not_reach_the_others():
+    bt = P.Batch([40, 50, 20], [20, 1, 20], Hq=4, Hkv=2, D=64, page=16, device=DEV)
+    q, k, v = _qkv(bt)
+    want = [ops.paged_attention(q.to(DEV), k, v, *bt.batch, max_q=m) for m in (1, 20)]
+    for t in (k, v):
+        t[bt.table[1, 1].item()] = float("nan")
+    for w, m in zip(want, (1, 20)):
+        got = ops.paged_attention(q.to(DEV), k, v, *bt.batch, max_q=m)
+        assert torch.equal(got[:20], w[:20]) and torch.equal(got[21:], w[21:]) and got[20].isnan().all()
