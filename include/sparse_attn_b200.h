@@ -33,7 +33,8 @@ enum {
   SA_ERR_UNSUPPORTED = -2, /* valid but unsupported (dtype, head_dim, device)    */
   SA_ERR_CUDA = -3,        /* a CUDA runtime/driver call failed                   */
   SA_ERR_TIMEOUT = -4,     /* a device-side bounded wait expired (see below)      */
-  SA_ERR_CSR = -5          /* CSR schedule failed host-side validation           */
+  SA_ERR_CSR = -5,         /* CSR schedule failed host-side validation           */
+  SA_ERR_WORKSPACE = -6    /* this call needs a workspace and was given none      */
 };
 
 /* BigBird layout of one KV group: (block_size, global, sliding, random), the
@@ -391,7 +392,8 @@ SA_API int sa_paged_append(const sa_paged_append_args* args, sa_stream_t stream)
  * choice of kernel and the split of long sequences: any value >= 1 is correct
  * for max_q; max_len must not be exceeded (SA_DEV_ERR_INDEX, keys cut).
  * workspace: sa_paged_attn_workspace(args) floats of device memory, used by this
- * call alone while it runs; 0 floats = may be NULL. */
+ * call alone while it runs; 0 floats = may be NULL. Without one where it is
+ * needed sa_paged_attn launches nothing and returns SA_ERR_WORKSPACE. */
 typedef struct sa_paged_attn_args {
   sa_paged_batch batch;
   const void* q;

@@ -54,6 +54,7 @@ SA_ERR_UNSUPPORTED = -2
 SA_ERR_CUDA = -3
 SA_ERR_TIMEOUT = -4
 SA_ERR_CSR = -5
+SA_ERR_WORKSPACE = -6
 SA_BIGBIRD = 0
 SA_BIGBIRD2 = 1
 SA_BF16 = 0

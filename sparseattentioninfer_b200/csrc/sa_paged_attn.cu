@@ -733,7 +733,8 @@ extern "C" int sa_paged_attn(const sa_paged_attn_args* args, sa_stream_t stream_
   const int sms = a->num_sms > 0 ? a->num_sms : sa_num_sms();
   if (sms <= 0) return sa_fail(SA_ERR_CUDA, "cannot query SM count");
   const AttnPlan r = attn_plan(*a, sms);
-  if (r.workspace(*a) > 0 && !a->workspace) return sa_fail(SA_ERR_INVALID, "paged attention: workspace is NULL");
+  if (r.workspace(*a) > 0 && !a->workspace)
+    return sa_fail(SA_ERR_WORKSPACE, "paged attention: this call needs a workspace");
   PagedAttnParams prm;
   memset(&prm, 0, sizeof(prm));
   if ((rc = sa_page_map(&prm.tm_k, *a, a->k_pages, a->k_strides, !r.chunk, "k_pages"))) return rc;

@@ -88,7 +88,7 @@ def test_attention_workspace_is_wanted_only_for_long_splits():
     assert need(split_len=4096, **long) == 5 * 8 * splits * (128 + 2)
     assert need(split_len=64000, **long) == 0
     a = _attn(split_len=4096, **long)
-    assert lib.sa_paged_attn(ctypes.addressof(a), None) == _capi.SA_ERR_INVALID
+    assert lib.sa_paged_attn(ctypes.addressof(a), None) == _capi.SA_ERR_WORKSPACE
     assert b"workspace" in lib.sa_last_error()
     assert lib.sa_paged_attn(None, None) == lib.sa_paged_attn_workspace(None, ctypes.byref(n)) == _capi.SA_ERR_INVALID
 
