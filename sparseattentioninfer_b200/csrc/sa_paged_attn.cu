@@ -39,8 +39,9 @@ struct PagedRowCfg {
   static constexpr int kGroups = WIDE ? 2 : 1;
   static constexpr int kConsumers = 4 * kGroups;  // warps
   static constexpr int kThreads = 32 * (kConsumers + 1);
-  // Otherwise two CTAs on an SM, four where the registers and 64-wide heads allow it.
-  static constexpr int kStages = WIDE ? 196608 / kStageBytes : (D == 64 && ROWS == 16) ? 6 : 3;
+  // Otherwise three stages: two CTAs on an SM, four with heads of 64 (16 sequences of
+  // 16k keys, 32 rows: 56 us, against 66 with two CTAs of six stages).
+  static constexpr int kStages = WIDE ? 196608 / kStageBytes : 3;
   static constexpr int kSmemBytes = kStages * kStageBytes;
   static_assert(kConsumers * ROWS * D * 4 <= kSmemBytes, "ring too small for the partial outputs");
 };
@@ -517,14 +518,15 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   if (a.blocks) {
     // The rows kernel reads every token's pages, a tile the union of its tokens'.
     // Both in 64-key steps: 3.2 ns each in all against 6.3 (whole GPU) and no less
-    // than about 0.9 us a step of one tile, 7 us more for the union and the tile's
-    // start. The union is taken as of lists drawn at random; real neighbours share more.
+    // than about 0.9 us a step of one tile (of a split tile's part), 13 us more for
+    // the union and the tile's start and end. The union is taken as of lists drawn at random; real neighbours share more.
     const double ps = a.batch.page_size, tokens = a.max_q < 128 / group ? a.max_q : 128 / group;
     const double seen = ceil((double)longest / ps), kept = a.n_blocks < seen ? a.n_blocks : seen;
     const double pages = seen * (1. - pow(1. - kept / seen, tokens)), steps = pages * ps / kRowKeys;
     const double lines = (a.batch.N / (128. / group) + 1.) * a.Hkv;
     const double rows_us = 0.0032 * a.batch.N * a.Hkv * ceil(kept * ps / kRowKeys);
-    const double tile_us = 7. + fmax(0.0063 * lines * steps, 0.9 * steps / fmax(1., fmin(8., 2 * sms / lines)));
+    const double parts = fmax(1., fmin(fmin(8., 2 * sms / lines), steps / 4));
+    const double tile_us = 13. + fmax(0.0063 * lines * steps, 0.9 * steps / parts);
     r.chunk = r.chunk && a.batch.max_pages <= kChunkMaxPages && tile_us < rows_us;
     if (r.chunk) {
       r.page_cap = (int64_t)(128 / group) * a.n_blocks;
@@ -549,11 +551,11 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   }
   longest = (longest + kRowKeys - 1) / kRowKeys * kRowKeys;
   int64_t len = ((int64_t)a.split_len + kRowKeys - 1) / kRowKeys * kRowKeys;
-  const int64_t slots = 2ll * sms;  // resident CTAs of either kernel
-  // Those of a grid of clusters: up to 8 CTAs have to fit in one GPC, which leaves
-  // some of its SMs over (18 clusters of 8 CTAs that take an SM each, 144 in all,
+  const int64_t slots = (r.chunk || a.D == 128 ? 2ll : 4ll) * sms;  // resident CTAs
+  // Those of a grid of clusters with an SM for each CTA: up to 8 CTAs have to fit in
+  // one GPC, which leaves some of its SMs over (18 clusters of 8, 144 CTAs in all,
   // ran in two waves on 148 SMs, 16 in one).
-  const int64_t resident = slots * 7 / 8;
+  const int64_t resident = sms * 7 / 8;
   // Tiles that the batch has at least: full ones, and one a sequence.
   const int64_t full = a.batch.N / r.tq + 1, some = a.batch.B < a.batch.N ? a.batch.B : a.batch.N;
   const int64_t lines = (r.tq == 1 ? r.units : full > some ? full : some) * a.Hkv * r.nhg;
@@ -579,7 +581,7 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
       // one wave. 256 keys each at least.
       len = 4096;
       if (2 * lines < slots) {
-        const int64_t fit = pow2_below(resident / 2 / lines, 8);
+        const int64_t fit = pow2_below(resident / lines, 8);
         const int64_t splits = fit >= 2 && longest <= fit * 2048 ? fit : (slots + lines - 1) / lines;
         len = (longest + splits - 1) / splits;
         if (len < 256) len = 256;
@@ -597,7 +599,7 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   // length, and short units leave some of them without keys: clusters only where
   // the whole grid is resident at once. Tiles are cut into equal parts: always.
   const int64_t grid = r.units * r.n_split * a.Hkv * r.nhg;
-  r.wide = !r.chunk && r.n_split <= 8 && grid <= (r.n_split > 1 ? resident / 2 : sms);
+  r.wide = !r.chunk && r.n_split <= 8 && grid <= (r.n_split > 1 ? resident : sms);
   r.cluster = r.chunk && r.n_split > 1 && r.n_split <= 8;
   r.part = r.n_split > 1 && !r.wide && !r.cluster ? (int64_t)a.batch.N * a.Hq * r.n_split * (a.D + 2) : 0;
   return r;

@@ -241,6 +241,9 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   }
 
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&p.tm_q);
+    tma_prefetch_desc(&p.tm_k);
+    tma_prefetch_desc(&p.tm_v);
     mbar_init(smem_u32(&bar_q), 1);
     mbar_init(smem_u32(&bar_drain), 1);
     for (int i = 0; i < NSK; ++i) {
