@@ -561,14 +561,24 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   const int64_t lines = (r.tq == 1 ? r.units : full > some ? full : some) * a.Hkv * r.nhg;
   if (a.split_len <= 0) {
     if (r.chunk) {
-      // Tiles in n equal parts: as many waves as that takes, of a part's keys and
-      // what a tile costs apart from its keys (start, end, partial results: about
-      // 640 keys' time, and 1,000 more where the parts join through the workspace).
-      int64_t best = 0;
+      // Tiles in n equal parts, by estimated time in keys of a full SM. A part costs
+      // 640 keys apart from its own (start, end, results), 150 more in a cluster,
+      // 1,000 more where the parts join through the workspace. With kept pages all
+      // tiles are alike: whole waves of them. Without, they go longest first and
+      // are 0.55 of the longest on average: the longest part alone (an SM runs one
+      // CTA in 0.6 of the time of two), or all of them over the slots.
+      double best = 0.;
       len = longest;
-      for (int64_t n = 1; n <= 64 && (n == 1 || longest / n >= 256); n *= 2) {
-        const int64_t waves = (lines * n + slots - 1) / slots;
-        const int64_t cost = waves * (longest / n + 640) + (n > 8 ? 1000 : 0);
+      for (int64_t n = 1; n <= 64 && (n == 1 || longest / n >= (a.blocks ? 256 : 128)); n *= 2) {
+        const double part = (double)longest / n, load = (double)(lines * n) / slots;
+        double cost = n > 8 ? 1000. : 0.;
+        if (a.blocks) {
+          cost += ceil(load) * (part + 640.);
+        } else {
+          cost += fmax(0.6 * part + 640., load * (0.55 * part + 640.));
+          if (n > 1) cost += 150.;
+          if (load > 0.875) cost += 320.;
+        }
         if (n == 1 || cost < best) {
           best = cost;
           len = (longest + n - 1) / n;
@@ -585,6 +595,8 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
         const int64_t splits = fit >= 2 && longest <= fit * 2048 ? fit : (slots + lines - 1) / lines;
         len = (longest + splits - 1) / splits;
         if (len < 256) len = 256;
+        // (the second kernel costs about 4 us, as long as 400 keys take a CTA)
+        if (lines * splits > resident && longest - len < 400) len = longest;
         if (len > 4096) len = 4096;
       }
     }
