@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kSelThreads, 3)
   __shared__ int s_amax[kSelTokens];
   __shared__ int s_wild[kSelTokens];  // the row has a score that is not finite
   __shared__ MidList s_mid[ONE ? 1 : kSelWarps];
-  __shared__ uint32_t s_part[3][kSelWarps];
+  __shared__ uint2 s_part[3][kSelWarps];
   double* qd = reinterpret_cast<double*>(smem + Cfg::kQd);
   uint64_t* keys = reinterpret_cast<uint64_t*>(smem + Cfg::kKeys);
   const sa_paged_batch& bt = a.batch;
@@ -301,21 +301,26 @@ __global__ void __launch_bounds__(kSelThreads, 3)
       for (int p = b0 + kSelRegs * 32 + lane; p < b1; p += 32) f(key(p));
     };
     int turn = 0;
-    auto join = [&](uint32_t v, auto op) {  // over the group's warps; s_part has three turns
+    auto join2 = [&](uint2 v, auto op) {  // over the group's warps; s_part has three turns
       if constexpr (ONE) {
-        uint32_t* part = s_part[turn];
+        uint2* part = s_part[turn];
         turn = turn == 2 ? 0 : turn + 1;
         if (lane == 0) part[warp] = v;
         __syncthreads();
         v = part[0];
 #pragma unroll
-        for (int w = 1; w < kSelWarps; ++w) v = op(v, part[w]);
+        for (int w = 1; w < kSelWarps; ++w) {
+          v.x = op(v.x, part[w].x);
+          v.y = op(v.y, part[w].y);
+        }
       }
       return v;
     };
-    auto sum = [&](int c) {
-      return (int)join(__reduce_add_sync(kAll, (unsigned)c), [](uint32_t x, uint32_t y) { return x + y; });
+    auto sum2 = [&](uint32_t x, uint32_t y) {
+      return join2(make_uint2(__reduce_add_sync(kAll, x), __reduce_add_sync(kAll, y)),
+                   [](uint32_t x, uint32_t y) { return x + y; });
     };
+    auto sum = [&](int c) { return (int)sum2((uint32_t)c, 0u).x; };
     auto group_sync = [&]() {
       if constexpr (ONE)
         __syncthreads();
@@ -335,32 +340,53 @@ __global__ void __launch_bounds__(kSelThreads, 3)
           kmax = max(kmax, k);
           kmin = min(kmin, k - 1);  // (the zeros go to the top)
         });
-        kmax = join(__reduce_max_sync(kAll, kmax), [](uint32_t x, uint32_t y) { return max(x, y); });
-        kmin = join(__reduce_min_sync(kAll, kmin), [](uint32_t x, uint32_t y) { return min(x, y); }) + 1;
-        // The largest bound that `need` keys reach, from the first bit that differs on.
-        const int bits = 32 - __clz(kmax ^ kmin);
+        // (as the maxima of k and of ~k)
+        const uint2 ends = join2(make_uint2(__reduce_max_sync(kAll, kmax), __reduce_max_sync(kAll, ~kmin)),
+                                 [](uint32_t x, uint32_t y) { return max(x, y); });
+        kmax = ends.x;
+        kmin = ~ends.y + 1;
+        // The largest bound that `need` keys reach, two bits a step from the first bit
+        // that differs on down to where a bit is a sixteenth of eps or less: what is
+        // open then is summed again anyhow.
+        const float eps2 = __int_as_float(s_amax[t]) * (2.f / 16384.f);
+        const float size = fmaxf(fabsf(key_value(kmax)), fabsf(key_value(kmin)));
+        int bits = 32 - __clz(kmax ^ kmin), fine = 0;
+        if (eps2 > 0.f && size > 0.f) fine = max(0, min(bits, ilogbf(eps2) - ilogbf(size) + 23 - 4));
         uint32_t v = bits == 32 ? 0u : (kmax >> bits) << bits;
-        for (int b = bits - 1; b >= 0; --b) {
-          const uint32_t cand = v | (1u << b);
-          int c = 0;
-          each([&](uint32_t k) { c += k >= cand ? 1 : 0; });
-          c = sum(c);
-          if (c >= need) v = cand;
-          if (c == need) break;
+        bool whole = false;
+        while (bits > fine && !whole) {
+          bits = max(bits - 2, 0);
+          // (with one bit left the upper two bounds lie behind it: too few keys reach them)
+          const uint32_t x1 = v + (1u << bits), x2 = v + (2u << bits), x3 = v + (3u << bits);
+          uint32_t c12 = 0, c3 = 0;  // counts, 16 bits each: at most 16,384 pages
+          each([&](uint32_t k) {
+            c12 += k >= x1 ? 1u : 0u;
+            c12 += k >= x2 ? 0x10000u : 0u;
+            c3 += k >= x3 ? 1u : 0u;
+          });
+          const uint2 c = sum2(c12, c3);
+          const int n1 = c.x & 0xffff, n2 = c.x >> 16, n3 = c.y;
+          const int n = n3 >= need ? n3 : n2 >= need ? n2 : n1;
+          if (n >= need) v = n3 >= need ? x3 : n2 >= need ? x2 : x1;
+          whole = n == need;
         }
-        uint32_t kth = kAll;  // the smallest key that reaches it (v > 0: no key is 0)
-        each([&](uint32_t k) { kth = k >= max(v, 1u) ? min(kth, k) : kth; });
-        kth = join(__reduce_min_sync(kAll, kth), [](uint32_t x, uint32_t y) { return min(x, y); });
-        const float th = key_value(kth), eps2 = __int_as_float(s_amax[t]) * (2.f / 16384.f);
-        from = order_key(th - eps2);
-        above = order_key(th + eps2);
+        uint32_t k0 = v, k1 = v + ((1u << bits) - 1);  // the need-th key lies here
+        if (whole) {  // it is the smallest that reaches v (v > 0: no key is 0)
+          uint32_t kth = 0;
+          each([&](uint32_t k) { kth = k >= v ? max(kth, ~k) : kth; });
+          k0 = k1 =
+              ~join2(make_uint2(__reduce_max_sync(kAll, kth), 0u), [](uint32_t x, uint32_t y) { return max(x, y); }).x;
+        }
+        from = order_key(key_value(k0) - eps2);
+        above = order_key(key_value(k1) + eps2);
         n_from = 0;
         each([&](uint32_t k) {
           n_from += k >= from ? 1 : 0;
           n_above += k > above ? 1 : 0;
         });
-        n_from = sum(n_from);
-        n_above = sum(n_above);
+        const uint2 c = sum2(n_from, n_above);
+        n_from = c.x;
+        n_above = c.y;
       }
       if (n_from == need) {
         bar = (uint64_t)from << 32;
@@ -438,14 +464,12 @@ __global__ void __launch_bounds__(kSelThreads, 3)
       c = __reduce_add_sync(kAll, c);
       e = __reduce_add_sync(kAll, e);
       __syncthreads();  // the last join's part may still be read
-      if (lane == 0) {
-        s_part[0][warp] = c;
-        s_part[1][warp] = e;
-      }
+      if (lane == 0) s_part[0][warp] = make_uint2(c, e);
       __syncthreads();
       for (int w = 0; w < warp; ++w) {
-        base += s_part[0][w] + min((int)s_part[1][w], max(0, ties - eq_before));
-        eq_before += s_part[1][w];
+        const int n = s_part[0][w].x, eq = s_part[0][w].y;
+        base += n + min(eq, max(0, ties - eq_before));
+        eq_before += eq;
       }
     }
     for (int i = gl; i < a.first + a.recent; i += 32 * GW)
