@@ -1,15 +1,19 @@
-"""Build the in-tree C-ABI library ``_lib/libsa_b200.so`` with nvcc for sm_100a.
+"""Build the in-tree C-ABI library ``_lib/libsa_b200.so`` with nvcc for sm_100a, and
+``_lib/_sa_paged.so``, the compiled Python binding of the paged-cache operators.
 
 The library is plain CUDA C++ (no torch headers), so it builds without a GPU and
-loads in any process through ctypes. Run ``python sparseattentioninfer_b200/_build.py`` (as a file: importing the
+loads in any process through ctypes; the binding is host C++ against the headers
+of the installed torch. Run ``python sparseattentioninfer_b200/_build.py`` (as a file: importing the
 package itself requires the built library).
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -17,6 +21,8 @@ CSRC = PKG / "csrc"
 LIB_DIR = PKG / "_lib"
 LIB_PATH = LIB_DIR / "libsa_b200.so"
 INCLUDE = PKG.parent / "include"
+BINDING_SRC = CSRC / "paged_binding.cpp"
+BINDING_PATH = LIB_DIR / "_sa_paged.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 BASE_FLAGS = [
@@ -39,11 +45,36 @@ def _deps() -> list[Path]:
     return sources() + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
 
 
+def _stale(target: Path, deps: list[Path]) -> bool:
+    return not target.exists() or any(p.stat().st_mtime > target.stat().st_mtime for p in deps)
+
+
 def needs_build() -> bool:
-    if not LIB_PATH.exists():
-        return True
-    t = LIB_PATH.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in _deps())
+    return _stale(LIB_PATH, _deps()) or _stale(BINDING_PATH, _binding_deps())
+
+
+def _binding_deps() -> list[Path]:
+    return [BINDING_SRC, *sorted(INCLUDE.glob("*.h"))]
+
+
+def build_binding(verbose: bool = False) -> Path:
+    """Compile ``csrc/paged_binding.cpp`` against the installed torch (not imported)."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        raise RuntimeError("torch not found; the paged-cache binding cannot be built")
+    torch = Path(spec.origin).parent
+    cuda = Path(nvcc_path()).resolve().parent.parent
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", sysconfig.get_paths()["include"], "-isystem", str(torch / "include"),
+           "-isystem", str(torch / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
+           str(BINDING_SRC), "-o", str(tmp), "-L", str(torch / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
 
 
 def nvcc_path() -> str:
@@ -54,10 +85,13 @@ def nvcc_path() -> str:
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
-    """Compile every ``csrc/*.cu`` into ``_lib/libsa_b200.so`` (skipped when up to date)."""
-    if not force and not needs_build():
-        return LIB_PATH
+    """Compile every ``csrc/*.cu`` into ``_lib/libsa_b200.so``, and the binding
+    (each skipped when up to date)."""
     LIB_DIR.mkdir(exist_ok=True)
+    if force or _stale(BINDING_PATH, _binding_deps()):
+        build_binding(verbose)
+    if not force and not _stale(LIB_PATH, _deps()):
+        return LIB_PATH
     nvcc = nvcc_path()
     objs = []
     build_dir = LIB_DIR / "obj"

@@ -6,12 +6,13 @@ fallback: if the library is missing or fails to load, every entry point raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
-import struct
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "_lib" / "libsa_b200.so"
+BINDING_PATH = _PKG / "_lib" / "_sa_paged.so"
 
 # Every symbol include/sparse_attn_b200.h declares (checked by the CPU tests).
 EXPORTED = (
@@ -134,14 +135,6 @@ class PagedSelectArgs(ctypes.Structure):
                 ("recent", _c_i32), ("max_q", _c_i32)]
 
 
-# The same structures packed in one call (native alignment): filling a ctypes
-# structure field by field costs several microseconds, as much as a small launch.
-_PB = "PPPqiiiii4x"
-PAGED_APPEND = struct.Struct("@" + _PB + "PqPPPPP2qP3qP3qP3qiiiiif0q")
-PAGED_ATTN = struct.Struct("@" + _PB + "PP2q2qP3qP3qP2qiiiiifiiiiP0q")
-PAGED_SELECT = struct.Struct("@" + _PB + "P2qP3qP2qiiiiiiii0q")
-
-
 class ArPeers(ctypes.Structure):
     _fields_ = [("rank", _c_i32), ("world", _c_i32), ("data", _c_p * 8), ("flags", _c_p * 8), ("epoch", _c_p),
                 ("max_ctas", _c_i32)]
@@ -185,11 +178,10 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     lib.sa_silu_mul.argtypes = [_c_p, _c_p, _c_i64, _c_i32, _c_i64, _c_i64, _c_p]
     lib.sa_linear_m8.argtypes = [_c_p, _c_i32, _c_i32, _c_i64, _c_p, _c_i32, _c_i64, _c_p, _c_i64, _c_i32, _c_p]
     lib.sa_topk_softmax_pv.argtypes = [ctypes.POINTER(TopkArgs), _c_p]
-    # (argument structures as PAGED_*.pack() bytes or a pointer to the ctypes structure)
-    lib.sa_paged_append.argtypes = [_c_p, _c_p]
-    lib.sa_paged_attn_workspace.argtypes = [_c_p, ctypes.POINTER(_c_i64)]
-    lib.sa_paged_attn.argtypes = [_c_p, _c_p]
-    lib.sa_paged_select.argtypes = [_c_p, _c_p]
+    lib.sa_paged_append.argtypes = [ctypes.POINTER(PagedAppendArgs), _c_p]
+    lib.sa_paged_attn_workspace.argtypes = [ctypes.POINTER(PagedAttnArgs), ctypes.POINTER(_c_i64)]
+    lib.sa_paged_attn.argtypes = [ctypes.POINTER(PagedAttnArgs), _c_p]
+    lib.sa_paged_select.argtypes = [ctypes.POINTER(PagedSelectArgs), _c_p]
     lib.sa_ar_alloc.argtypes = [ctypes.c_size_t, ctypes.POINTER(_c_p)]
     lib.sa_ar_free.argtypes = [_c_p]
     lib.sa_ar_ipc_handle.argtypes = [_c_p, _c_p]
@@ -203,6 +195,28 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
             getattr(lib, name).restype = ctypes.c_int
     _lib = lib
     return lib
+
+
+_binding = None
+
+
+def paged_binding():
+    """The compiled Python calls of the paged-cache operators (csrc/paged_binding.cpp),
+    loaded once and bound to the loaded library. torch must be imported."""
+    global _binding
+    if _binding is None:
+        if not BINDING_PATH.exists():
+            raise ImportError(
+                f"sparseattentioninfer_b200 binding not found at {BINDING_PATH}; build it with "
+                "`python sparseattentioninfer_b200/_build.py`")
+        spec = importlib.util.spec_from_file_location("_sa_paged", BINDING_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        lib = load()
+        module.init(*(ctypes.cast(getattr(lib, f"sa_paged_{n}"), _c_p).value
+                      for n in ("append", "attn", "attn_workspace", "select")))
+        _binding = module
+    return _binding
 
 
 def check(rc: int) -> None:

@@ -149,26 +149,32 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 6)
     if (u >= q_units) return;
     const uint32_t groups = (a.Hq + q_heads - 1) / q_heads, token = u / groups;
     const int h_first = (int)((u - token * groups) * q_heads), h_end = min(h_first + (int)q_heads, a.Hq);
+    if (token >= (uint32_t)bt.N) return;
+    // The first heads are loaded while the token's position is looked up.
+    const T* src = qkv + (int64_t)token * a.qkv_st;
+    Raw<H> x[kQHeads / 2];
+    auto load_heads = [&](int h0) {
+#pragma unroll
+      for (int i = 0; i < kQHeads / 2; ++i) x[i].load(src + min(h0 + 2 * i, h_end - 1) * D);
+    };
+    load_heads(h_first + half);
+    load_weight(a.q_weight);
     UnitTokens ut;
     if (!unit_tokens(bt, token, 1, err, ut)) return;
     if (ut.pos0 >= a.positions) {
       if (lane == 0) record_error(err, SA_DEV_ERR_INDEX);
       return;
     }
-    const T* src = qkv + (int64_t)ut.t0 * a.qkv_st;
     T* dst = reinterpret_cast<T*>(a.q_out) + (int64_t)ut.t0 * a.q_strides[0] + at;
     Turn<H> turn;
     {
       Raw<H> c, s;
       c.load(cos_t + (int64_t)ut.pos0 * D);
       s.load(sin_t + (int64_t)ut.pos0 * D);
-      load_weight(a.q_weight);
       turn.template from<T>(c, s, w);
     }
     for (int h0 = h_first + half; h0 - half < h_end; h0 += kQHeads) {
-      Raw<H> x[kQHeads / 2];
-#pragma unroll
-      for (int i = 0; i < kQHeads / 2; ++i) x[i].load(src + min(h0 + 2 * i, h_end - 1) * D);
+      if (h0 - half > h_first) load_heads(h0);
 #pragma unroll
       for (int i = 0; i < kQHeads / 2; ++i) {
         norm_rope<T, H>(x[i], a.q_weight != nullptr, turn, a.eps);

@@ -449,58 +449,16 @@ def topk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: int
 # ---------------------------------------------------------------------------
 # Paged cache, packed ragged batches (sa_paged_*.cu)
 # ---------------------------------------------------------------------------
-# (These calls are as short as a small launch: attributes are read once each, a
-# tensor's strides for both the check and the arguments.)
-_NO3, _NO4 = (0, 0, 0), (0, 0, 0, 0)
-_HALF = {torch.bfloat16: _capi.SA_BF16, torch.float16: _capi.SA_FP16}
+# (The checks of these calls are compiled, csrc/paged_binding.cpp: a decode step's
+# kernels are shorter than the same checks in Python.)
+_PAGED = _capi.paged_binding()
 
 
-def _paged_dtype(name: str, t: torch.Tensor) -> int:
-    if not t.is_cuda:
-        raise RuntimeError("cuda_sparse_attention ops need CUDA tensors (there is no CPU path)")
-    code = _HALF.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{name}: bf16 or fp16 tensors expected, got {t.dtype}")
-    return code
-
-
-def _paged_strides(name: str, t: torch.Tensor, dtype: torch.dtype, dev: int, ndim: int) -> tuple:
-    """Strides of all but the last dimension of a tensor of ``dtype`` and ``ndim``
-    dimensions on device ``dev``, the last one contiguous."""
-    s = t.stride()
-    if t.dtype is not dtype or t.get_device() != dev or len(s) != ndim:
-        raise TypeError(f"{name}: {dtype} of {ndim} dimensions on cuda:{dev} expected, got {t.dtype} "
-                        f"{tuple(t.shape)} on {t.device}")
-    if s[-1] != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous, got strides {s} of {tuple(t.shape)}")
-    return s[:-1]
-
-
-def _paged_batch(name: str, N: int, dev: int, page_table, cu_q, seq_lens, num_pages: int, page_size: int) -> tuple:
-    _paged_strides(name, cu_q, torch.int32, dev, 1)
-    _paged_strides(name, seq_lens, torch.int32, dev, 1)
-    B, width = page_table.shape
-    if seq_lens.numel() != B or cu_q.numel() != B + 1:
-        raise ValueError(f"{name}: page_table [B, pages], cu_q [B + 1] and seq_lens [B] expected, got "
-                         f"{tuple(page_table.shape)}, {tuple(cu_q.shape)} and {tuple(seq_lens.shape)}")
-    return (page_table.data_ptr(), cu_q.data_ptr(), seq_lens.data_ptr(),
-            *_paged_strides(name, page_table, torch.int32, dev, 2), B, N, width, num_pages, page_size)
-
-
-def _check_pages(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor, Hkv: int, D: int):
-    shape = k_pages.shape
-    if len(shape) != 4 or v_pages.shape != shape or shape[1] != Hkv or shape[3] != D:
-        raise ValueError(f"{name}: k_pages / v_pages must be [pages, {Hkv}, page_size, {D}], got "
-                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
-    return shape[0], shape[2]
-
-
-def _paged_call(fn, args: bytes, dev: int) -> int:
-    """fn(args, current stream of device dev) with that device current: its status."""
-    if torch._C._cuda_getDevice() == dev:
-        return fn(args, torch._C._cuda_getCurrentRawStream(dev))
-    with torch.cuda.device(dev):
-        return fn(args, torch._C._cuda_getCurrentRawStream(dev))
+def _paged_result(r):
+    """The tensor that a compiled call returned; it returns the C call's status where that is not 0."""
+    if type(r) is int:
+        _capi.check(r)
+    return r
 
 
 def paged_qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
@@ -523,48 +481,8 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor | None, 
     paged_block_select scores). The batch tensors are read on the device, so
     the call can be captured; what they must satisfy is stated in
     sparse_attn_b200.h, and a violation sets the device error word."""
-    name = "paged_qk_norm_rope_append"
-    code = _paged_dtype(name, qkv)
-    if qkv.dim() != 3 or qkv.shape[1] != Hq + 2 * Hkv:
-        raise ValueError(f"{name}: qkv must be [N, {Hq}+2*{Hkv}, D], got {tuple(qkv.shape)}")
-    N, _, D = qkv.shape
-    dev, dt = qkv.get_device(), qkv.dtype
-    if q_out is None:
-        q_out = torch.empty(N, Hq, D, dtype=dt, device=qkv.device)
-    elif q_out.shape != (N, Hq, D):
-        raise ValueError(f"{name}: q_out must be [{N}, {Hq}, {D}], got {tuple(q_out.shape)}")
-    pages, page_size = _check_pages(name, k_pages, v_pages, Hkv, D)
-    positions = cos.shape[0]
-    if cos.shape != sin.shape or cos.shape != (positions, D) or not cos.is_contiguous() or not sin.is_contiguous():
-        raise ValueError(f"{name}: cos / sin must be contiguous [positions, {D}]")
-    _paged_strides(name, cos, dt, dev, 2)
-    _paged_strides(name, sin, dt, dev, 2)
-    weights = [0, 0]
-    for i, w in enumerate((q_weight, k_weight)):
-        if w is not None:
-            _paged_strides(name, w, dt, dev, 1)
-            if w.numel() != D:
-                raise ValueError(f"{name}: weights must be [{D}], got {tuple(w.shape)}")
-            weights[i] = w.data_ptr()
-    st, sh = _paged_strides(name, qkv, dt, dev, 3)
-    if sh != D:
-        raise ValueError(f"{name}: the heads of qkv must be contiguous, got strides {qkv.stride()}")
-    bounds, b_strides = 0, _NO3
-    if k_bounds is not None:
-        if k_bounds.shape != (pages, Hkv, 2, D):
-            raise ValueError(f"{name}: k_bounds must be [{pages}, {Hkv}, 2, {D}], got {tuple(k_bounds.shape)}")
-        bounds, b_strides = k_bounds.data_ptr(), _paged_strides(name, k_bounds, dt, dev, 4)
-    batch = _paged_batch(name, N, dev, page_table, cu_q, seq_lens, pages, page_size)
-    if N == 0 or batch[4] == 0:
-        return q_out
-    rc = _paged_call(_capi.load().sa_paged_append, _capi.PAGED_APPEND.pack(
-        *batch, qkv.data_ptr(), st, *weights, cos.data_ptr(), sin.data_ptr(), q_out.data_ptr(),
-        *_paged_strides(name, q_out, dt, dev, 3), k_pages.data_ptr(), *_paged_strides(name, k_pages, dt, dev, 4),
-        v_pages.data_ptr(), *_paged_strides(name, v_pages, dt, dev, 4), bounds, *b_strides, Hq, Hkv, D, positions,
-        code, eps), dev)
-    if rc:
-        _capi.check(rc)
-    return q_out
+    return _paged_result(_PAGED.append(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_table, cu_q, seq_lens,
+                                       Hq, Hkv, eps, k_bounds, q_out))
 
 
 def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, page_table: torch.Tensor, cu_q: torch.Tensor,
@@ -580,68 +498,8 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, page_table: torc
     the lower index; scores are compared in 64 bits. q [N, Hq, D] and the batch
     tensors as in paged_qk_norm_rope_append; ``max_q`` (most new tokens of one
     sequence) only steers the launch."""
-    name = "paged_block_select"
-    code = _paged_dtype(name, q)
-    if q.dim() != 3 or k_bounds.dim() != 4 or k_bounds.shape[2] != 2 or k_bounds.shape[3] != q.shape[2]:
-        raise ValueError(f"{name}: q [N, Hq, D] and k_bounds [pages, Hkv, 2, D], got {tuple(q.shape)} and "
-                         f"{tuple(k_bounds.shape)}")
-    N, Hq, D = q.shape
-    pages, Hkv = k_bounds.shape[:2]
-    dev, dt = q.get_device(), q.dtype
-    if out is None:
-        out = torch.empty(N, Hkv, keep, dtype=torch.int32, device=q.device)
-    elif out.shape != (N, Hkv, keep):
-        raise ValueError(f"{name}: out must be [{N}, {Hkv}, {keep}], got {tuple(out.shape)}")
-    batch = _paged_batch(name, N, dev, page_table, cu_q, seq_lens, pages, page_size)
-    if N == 0 or batch[4] == 0:
-        return out
-    rc = _paged_call(_capi.load().sa_paged_select, _capi.PAGED_SELECT.pack(
-        *batch, q.data_ptr(), *_paged_strides(name, q, dt, dev, 3), k_bounds.data_ptr(),
-        *_paged_strides(name, k_bounds, dt, dev, 4), out.data_ptr(),
-        *_paged_strides(name, out, torch.int32, dev, 3), Hq, Hkv, D, code, keep, first, recent,
-        N if max_q is None else max_q), dev)
-    if rc:
-        _capi.check(rc)
-    return out
-
-
-def _paged_attn_args(name, q, k_pages, v_pages, page_table, cu_q, seq_lens, out, max_q, max_len, blocks, scale,
-                     split_len):
-    """Arguments of sa_paged_attn but for the workspace, or None for an empty batch.
-    ``out`` None: a new tensor; returned first."""
-    code = _paged_dtype(name, q)
-    if q.dim() != 3 or k_pages.dim() != 4:
-        raise ValueError(f"{name}: q [N, Hq, D] and pages of 4 dimensions expected, got {tuple(q.shape)} and "
-                         f"{tuple(k_pages.shape)}")
-    N, Hq, D = q.shape
-    Hkv = k_pages.shape[1]
-    dev, dt = q.get_device(), q.dtype
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != q.shape:
-        raise ValueError(f"{name}: out must be {tuple(q.shape)}, got {tuple(out.shape)}")
-    pages, page_size = _check_pages(name, k_pages, v_pages, Hkv, D)
-    kept = _NO4
-    if blocks is not None:
-        if blocks.dim() != 3 or blocks.shape[0] != N or blocks.shape[1] != Hkv:
-            raise ValueError(f"{name}: blocks must be [{N}, {Hkv}, n], got {tuple(blocks.shape)}")
-        kept = (blocks.data_ptr(), *_paged_strides(name, blocks, torch.int32, dev, 3), blocks.shape[2])
-    batch = _paged_batch(name, N, dev, page_table, cu_q, seq_lens, pages, page_size)
-    if N == 0 or batch[4] == 0:
-        return out, None
-    return out, (*batch, q.data_ptr(), out.data_ptr(), *_paged_strides(name, q, dt, dev, 3),
-                 *_paged_strides(name, out, dt, dev, 3), k_pages.data_ptr(),
-                 *_paged_strides(name, k_pages, dt, dev, 4), v_pages.data_ptr(),
-                 *_paged_strides(name, v_pages, dt, dev, 4), *kept, Hq, Hkv, D, code,
-                 1.0 / math.sqrt(D) if scale is None else scale, N if max_q is None else max_q,
-                 batch[6] * page_size if max_len is None else max_len, 0 if split_len is None else split_len,
-                 _NUM_SMS.get(dev) or _num_sms(q.device))
-
-
-def _paged_workspace(packed: bytes) -> int:
-    n = ctypes.c_int64(0)
-    _capi.check(_capi.load().sa_paged_attn_workspace(packed, ctypes.byref(n)))
-    return n.value
+    return _paged_result(_PAGED.select(q, k_bounds, page_table, cu_q, seq_lens, page_size, keep, first, recent, max_q,
+                                       out))
 
 
 def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -649,9 +507,10 @@ def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, v_pages: t
                               max_q: int | None = None, max_len: int | None = None,
                               blocks: torch.Tensor | None = None, split_len: int | None = None) -> int:
     """float32 elements of workspace that paged_attention with these arguments needs."""
-    _, args = _paged_attn_args("paged_attention_workspace", q, k_pages, v_pages, page_table, cu_q, seq_lens, q, max_q,
-                               max_len, blocks, None, split_len)
-    return 0 if args is None else _paged_workspace(_capi.PAGED_ATTN.pack(*args, 0))
+    n = _PAGED.workspace(q, k_pages, v_pages, page_table, cu_q, seq_lens, max_q, max_len, blocks, None, split_len, None)
+    if n < 0:
+        _capi.check(n)
+    return n
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -671,27 +530,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     their defaults are N and the page table's width. ``workspace``: float32
     buffer of at least paged_attention_workspace(...) elements that a captured
     call keeps to itself (allocated per call when None)."""
-    name = "paged_attention"
-    out, args = _paged_attn_args(name, q, k_pages, v_pages, page_table, cu_q, seq_lens, out, max_q, max_len, blocks,
-                                 scale, split_len)
-    if args is None:
-        return out
-    dev, fn = q.get_device(), _capi.load().sa_paged_attn
-    if workspace is None:
-        rc = _paged_call(fn, _capi.PAGED_ATTN.pack(*args, 0), dev)
-        if rc == _capi.SA_ERR_WORKSPACE:
-            need = _paged_workspace(_capi.PAGED_ATTN.pack(*args, 0))
-            workspace = torch.empty(need, dtype=torch.float32, device=q.device)
-            rc = _paged_call(fn, _capi.PAGED_ATTN.pack(*args, workspace.data_ptr()), dev)
-    else:
-        need = _paged_workspace(_capi.PAGED_ATTN.pack(*args, 0))
-        if workspace.dtype != torch.float32 or workspace.get_device() != dev or not workspace.is_contiguous() or \
-                workspace.numel() < need:
-            raise ValueError(f"{name}: workspace must be {need} contiguous float32 on cuda:{dev}")
-        rc = _paged_call(fn, _capi.PAGED_ATTN.pack(*args, workspace.data_ptr()), dev)
-    if rc:
-        _capi.check(rc)
-    return out
+    return _paged_result(_PAGED.attention(q, k_pages, v_pages, page_table, cu_q, seq_lens, max_q, max_len, blocks, scale,
+                                          split_len, out, workspace))
 
 
 def sparse_attn(q, k, v, block_pairs, block_pair_offsets, block_size: int, *, scale: float | None = None):
