@@ -34,7 +34,6 @@ namespace sa {
 
 constexpr int kChM = 128;      // query rows
 constexpr int kChN = 64;       // keys per chunk
-constexpr int kChMeta = 16;    // ring of page masks; see kMetaRing of the block-sparse kernel
 constexpr int kChThreads = 192;
 
 template <typename T>
@@ -57,7 +56,9 @@ struct ChunkCfg {
   static constexpr int kVStages = kBufs - kKStages > 4 ? 4 : kBufs - kKStages;
   static constexpr int kSmemBytes = kQBytes + (kKStages + kVStages) * kKVBytes;
   static_assert(kKStages >= 2 && kVStages >= 2, "not enough shared memory");
-  static_assert(kKStages + 3 < kChMeta, "mask ring too short");
+  // Two batches of pages are described at a time: a batch holds at least 8 chunks, and
+  // the producer is at most kVStages ahead of the softmax.
+  static_assert(kVStages < 8, "producer may run a batch ahead");
 };
 
 // The ascending union of the lists of one tile's tokens. Entries behind the first
@@ -133,9 +134,9 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   constexpr uint32_t SB = D;  // first S/P column
   __shared__ __align__(8) uint64_t bar_q, bar_drain;
   __shared__ __align__(8) uint64_t bar_k_full[NSK], bar_k_empty[NSK], bar_v_full[NSV], bar_v_empty[NSV];
-  __shared__ __align__(8) uint64_t bar_p_full[2], bar_meta[kChMeta];
-  __shared__ uint32_t meta_mask[kChMeta];  // 16-key groups of the chunk that hold keys
-  __shared__ int meta_blk[SPARSE ? kChMeta : 1][4];  // logical pages of the chunk, -1: none
+  __shared__ __align__(8) uint64_t bar_p_full[2], bar_meta[2];
+  __shared__ uint32_t meta_have[2];               // which of a batch's 32 pages are there
+  __shared__ int meta_blk[SPARSE ? 2 : 1][32];  // logical pages of the batch, -1: none
   __shared__ uint32_t tmem_base_sh;
   __shared__ int abort_flag;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -156,6 +157,7 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   const int keys = unit_keys(ut, a.max_len);
   if (keys < min(ut.pos0 + ut.n, ut.len) && lane == 0) record_error(p.err, SA_DEV_ERR_INDEX);
   const int pps = ps < N ? N / ps : 1, spp = ps > N ? ps / N : 1, box = min(ps, N);  // pages per chunk, chunks per page
+  const int lpps = 31 - __clz(pps), lspp = 31 - __clz(spp), lbox = 31 - __clz(box);  // (all powers of two)
   const int32_t* union_at = nullptr;
   int n_union = 0, chunks;
   if constexpr (SPARSE) {
@@ -167,6 +169,7 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   }
   // Every tile is cut into n_split parts of its own length: chunks [c0, c0 + nch).
   const int per = tile_part(chunks, p.n_split), c0 = min(split * per, chunks), nch = min(chunks - c0, per);
+  const int e0 = (c0 >> lspp) << lpps;  // the part's first page
   const int rows = ut.n * G;
   const uint32_t sQ = smem_u32(smem_raw), sK = sQ + Cfg::kQBytes, sV = sK + NSK * Cfg::kKVBytes;
 
@@ -254,8 +257,10 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
       mbar_init(smem_u32(&bar_v_full[i]), 1);
       mbar_init(smem_u32(&bar_v_empty[i]), 1);
     }
-    for (int i = 0; i < kChMeta; ++i) mbar_init(smem_u32(&bar_meta[i]), 1);
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&bar_p_full[i]), 128);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bar_meta[i]), 1);
+      mbar_init(smem_u32(&bar_p_full[i]), 128);
+    }
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -271,7 +276,11 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
 
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
-    // Lane j < pps loads page j of a chunk; page numbers are read 32 ahead.
+    // Lane j < pps loads page j of a chunk. Page numbers come in batches of 32, read a
+    // batch ahead, and what the softmax has to know of them is handed over by the batch:
+    // this warp's own steps can set the pace of a tile (with divisions and a mask for each
+    // chunk they took 1,000 cycles of a chunk's 1,800: 283 -> 257 us on 432 tiles over 3k
+    // to 11k keys in pages of 16, 574 -> 560 on two prompts of 6k in pages of 128).
     if (lane == 0) {
       mbar_arrive_expect_tx(smem_u32(&bar_q), (uint32_t)p.tq * G * D * 2);
 #pragma unroll
@@ -279,49 +288,39 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         tma_load_4d(sQ + r * kChM * 128, &p.tm_q, smem_u32(&bar_q), r * 64, kvh * G, ut.t0, 0);
     }
     const int32_t* trow = bt.table + (int64_t)ut.b * bt.table_stride;
-    const int e0 = c0 / spp * pps;
-    int page = bt.num_pages, entry = -1, base = -32, kn = 0, vn = 0;  // chunks of K and V issued
+    int page = bt.num_pages, base = -32, kn = 0, vn = 0;  // chunks of K and V issued
+    int next_page = 0, next_blk = -1;  // the batch ahead: table entry, logical page (-1: none)
     bool ok = true, bad = false;
+    auto fetch = [&](int from) {
+      int64_t blk = (int64_t)e0 + from + lane;
+      if constexpr (SPARSE) blk = blk < n_union ? __ldg(union_at + blk) : -1;
+      next_blk = blk >= 0 && blk * ps < keys ? (int)blk : -1;
+      if (next_blk >= 0) next_page = __ldg(trow + next_blk);
+    };
+    fetch(0);
     for (int g = 0; g < nch; ++g) {
-      const int first = (c0 + g) / spp * pps - e0;
+      const int first = (((c0 + g) >> lspp) << lpps) - e0;
       if (first >= base + 32) {
         base = first;
-        int64_t blk = (int64_t)e0 + base + lane;
-        page = bt.num_pages;  // behind the last page: reads as zeros
-        if constexpr (SPARSE) {
-          blk = blk < n_union ? __ldg(union_at + blk) : -1;
-          entry = (int)blk;
-        }
-        if (blk >= 0 && blk * ps < keys) {
-          const int pg = __ldg(trow + blk);
-          if (pg < 0 || pg >= bt.num_pages)
-            bad = true;
-          else
-            page = pg;
-        }
+        const int slot = (base >> 5) & 1;
+        const bool there = next_blk >= 0 && next_page >= 0 && next_page < bt.num_pages;
+        bad |= next_blk >= 0 && !there;
+        page = there ? next_page : bt.num_pages;  // behind the last page: reads as zeros
+        const unsigned have = __ballot_sync(0xffffffffu, there);
+        if constexpr (SPARSE) meta_blk[slot][lane] = next_blk;
+        if (lane == 0) meta_have[slot] = have;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_meta[slot]));
+        fetch(base + 32);
       }
-      const int src = (first - base + (lane < pps ? lane : 0)) & 31;
-      const int pg = __shfl_sync(0xffffffffu, page, src);
-      const int blk_of = SPARSE ? __shfl_sync(0xffffffffu, entry, src) : 0;
-      const int off = spp > 1 ? ((c0 + g) % spp) * N : 0;
-      const unsigned have = __ballot_sync(0xffffffffu, lane < pps && pg < bt.num_pages);
-      const int ks = g % NSK, vs = g % NSV, ms = g % kChMeta;
+      const int pg = __shfl_sync(0xffffffffu, page, (first - base + (lane < pps ? lane : 0)) & 31);
+      const int off = ((c0 + g) & (spp - 1)) * N;
+      const int ks = g % NSK, vs = g % NSV;
       if (g >= NSK) {
         ok = mbar_wait(smem_u32(&bar_k_empty[ks]), ((g / NSK) - 1) & 1, abort_v, p.err);
         if (!__all_sync(0xffffffffu, ok)) break;
       }
-      if constexpr (SPARSE) {
-        if (lane < pps) meta_blk[ms][lane] = blk_of;
-        __syncwarp();
-      }
-      if (lane == 0) {
-        uint32_t mask = 0;
-        for (int j = 0; j < pps; ++j)
-          if ((have >> j) & 1u) mask |= ((1u << (box / 16)) - 1) << (j * (box / 16));
-        meta_mask[ms] = mask;
-        mbar_arrive(smem_u32(&bar_meta[ms]));
-        mbar_arrive_expect_tx(smem_u32(&bar_k_full[ks]), Cfg::kKVBytes);
-      }
+      if (lane == 0) mbar_arrive_expect_tx(smem_u32(&bar_k_full[ks]), Cfg::kKVBytes);
       __syncwarp();
       if (lane < pps) {
 #pragma unroll
@@ -380,9 +379,9 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
       for (int g = 0; ok && g < nch; ++g) {
         // S of the next chunk goes in before this chunk's PV.
         if (g + 1 < nch && !(ok = next_s(g + 1))) break;
-        if (!(ok = mbar_wait(smem_u32(&bar_p_full[g & 1]), (g >> 1) & 1, abort_v, p.err))) break;
         const int vs = g % NSV;
         if (!(ok = mbar_wait(smem_u32(&bar_v_full[vs]), (g / NSV) & 1, abort_v, p.err))) break;
+        if (!(ok = mbar_wait(smem_u32(&bar_p_full[g & 1]), (g >> 1) & 1, abort_v, p.err))) break;
         tc_fence_after();
         const uint32_t pbuf = tmem + SB + (g & 1) * N;
         const uint64_t vst = v_desc + (uint64_t)((vs * Cfg::kKVBytes) >> 4);
@@ -418,7 +417,7 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
     if constexpr (SPARSE) {
       if (row_ok) {
         list = a.blocks + (int64_t)(ut.t0 + row / G) * a.blocks_strides[0] + (int64_t)kvh * a.blocks_strides[1];
-        const int from = __ldg(union_at + c0 / spp * pps);  // first page of this split
+        const int from = __ldg(union_at + e0);  // first page of this split
         int hi = c0 > 0 ? a.n_blocks : 0;
         while (ptr < hi) {
           const int mid = (ptr + hi) >> 1;
@@ -431,29 +430,35 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         ahead = want == kNone ? kNone : entry_at(ptr + 1);
       }
     }
+    int batch = -1;
+    uint32_t have_all = 0;
     for (int g = 0; g < nch; ++g) {
-      const int ms = g % kChMeta;
-      ok = mbar_wait(smem_u32(&bar_meta[ms]), (g / kChMeta) & 1, abort_v, p.err);
-      if (!__all_sync(FULL, ok)) { ok = false; break; }
-      const uint32_t mask = meta_mask[ms];
+      const int first = (((c0 + g) >> lspp) << lpps) - e0;
+      if (first >> 5 != batch) {
+        batch = first >> 5;
+        ok = mbar_wait(smem_u32(&bar_meta[batch & 1]), (batch >> 1) & 1, abort_v, p.err);
+        if (!__all_sync(FULL, ok)) { ok = false; break; }
+        have_all = meta_have[batch & 1];
+      }
+      const uint32_t have = have_all >> (first & 31);  // page j of the chunk: bit j
       ok = mbar_wait(smem_u32(&bar_k_empty[g % NSK]), (g / NSK) & 1, abort_v, p.err);  // S is in TMEM
       if (!__all_sync(FULL, ok)) { ok = false; break; }
       tc_fence_after();
       const uint32_t sbuf = tmem + lane_base + SB + (g & 1) * N;
-      const int off = SPARSE ? (c0 + g) % spp * N : (c0 + g) * N;  // first key, in its page or of all
+      const int off = SPARSE ? ((c0 + g) & (spp - 1)) * N : (c0 + g) * N;  // first key, in its page or of all
       int lim[4];  // column i of the chunk is seen when i % 16 <= lim[i / 16]
       bool plain = true, skip = false, tail = false;
       if constexpr (SPARSE) {
         bool any = false;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int jp = q * 16 / box, blk = meta_blk[ms][jp];
+          const int jp = q * 16 >> lbox, blk = meta_blk[batch & 1][(first & 31) + jp];
           const int key0 = blk * ps + off + q * 16 - jp * box;
-          lim[q] = blk == want && ((mask >> q) & 1u) ? min(pos - key0, 15) : -1;
+          lim[q] = blk == want && ((have >> jp) & 1u) ? min(pos - key0, 15) : -1;
           plain &= lim[q] == 15;
           any |= lim[q] >= 0;
           tail |= blk >= 0 && key0 + 16 > keys;
-          if ((q + 1) * 16 % box == 0 && blk == want && (c0 + g) % spp == spp - 1) {
+          if (((q + 1) * 16 & (box - 1)) == 0 && blk == want && ((c0 + g) & (spp - 1)) == spp - 1) {
             ++ptr;
             want = ahead;
             ahead = want == kNone ? kNone : entry_at(ptr + 1);
@@ -461,10 +466,11 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         }
         skip = !__any_sync(FULL, any);  // no row of the warp sees the chunk
       } else {
-        plain = pos - off >= N - 1 && mask == 0xfu;
+        const uint32_t all = (1u << pps) - 1u;
+        plain = pos - off >= N - 1 && (have & all) == all;
         tail = off + N > keys;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) lim[q] = ((mask >> q) & 1u) ? min(pos - off - q * 16, 15) : -1;
+        for (int q = 0; q < 4; ++q) lim[q] = ((have >> (q * 16 >> lbox)) & 1u) ? min(pos - off - q * 16, 15) : -1;
       }
       uint32_t pk[N / 2];
       if (skip) {
@@ -541,10 +547,10 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         const uint32_t v0 = sV + (g % NSV) * Cfg::kKVBytes;
         for (int i = row; i < N * 8 * R; i += 128) {
           // 16-byte piece i: page, region, row
-          const int jp = i / (box * 8 * R), r = jp * box + ((i >> 3) & (box - 1));
+          const int jp = i / (8 * R) >> lbox, r = jp * box + ((i >> 3) & (box - 1));
           int key = off + r;
           if constexpr (SPARSE) {
-            const int blk = meta_blk[ms][jp];
+            const int blk = meta_blk[batch & 1][(first & 31) + jp];
             key = blk < 0 ? 0 : blk * ps + off + r - jp * box;  // (none: read as zeros)
           }
           if (key >= keys)
