@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const sa_paged_attn_args& a = p.a;
   const sa_paged_batch& bt = a.batch;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int G = p.gh, ps = bt.page_size;
   // The tiles that see the most keys come first (448 tiles of 3.2k to 11.2k keys:
   // 299 -> 282 us), all heads of a token tile side by side.
@@ -351,51 +351,70 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
     mbar_wait(smem_u32(&bar_q), 0, never, nullptr);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = chunk_idesc<T>(N, false);
-      constexpr uint32_t idesc_pv = chunk_idesc<T>(D, true);
-      const uint64_t q_desc = smem_desc_sw128(sQ, 16, 1024);
-      const uint64_t k_desc = smem_desc_sw128(sK, 16, 1024);
-      // V lies page by page, a page's 64-column regions one behind the other.
-      const uint64_t v_desc = smem_desc_sw128(sV, box * 128, 1024);
-      const int lks = 31 - __clz(box) - 4;  // log2 of the 16-key steps per page
-      // S = Q K^T of chunk g; its commit frees the K slot and tells the softmax.
-      auto next_s = [&](int g) -> bool {
-        const int ks = g % NSK;
-        if (!mbar_wait(smem_u32(&bar_k_full[ks]), (g / NSK) & 1, abort_v, p.err)) return false;
-        tc_fence_after();
-        const uint32_t d = tmem + SB + (g & 1) * N;
-        const uint64_t kst = k_desc + (uint64_t)((ks * Cfg::kKVBytes) >> 4);
+    // The whole warp goes through the loop with values that are the same in all lanes,
+    // and one elected lane issues: the operands then need no moves out of a thread's own
+    // registers, which had taken 50 cycles a product (12 products a chunk).
+    constexpr uint32_t idesc_s = chunk_idesc<T>(N, false);
+    constexpr uint32_t idesc_pv = chunk_idesc<T>(D, true);
+    const unsigned FULL = 0xffffffffu;
+    const uint32_t tm = __shfl_sync(FULL, tmem, 0);
+    const int n = __shfl_sync(FULL, nch, 0);
+    // Descriptors: the upper halves are constant, the lower ones hold the address.
+    const uint64_t desc_up = smem_desc_sw128(0, 0, 1024);
+    const uint32_t q_lo = __shfl_sync(FULL, (uint32_t)smem_desc_sw128(sQ, 16, 0), 0);
+    const uint32_t k_lo = __shfl_sync(FULL, (uint32_t)smem_desc_sw128(sK, 16, 0), 0);
+    // V lies page by page, a page's 64-column regions one behind the other.
+    const uint32_t v_lo = __shfl_sync(FULL, (uint32_t)smem_desc_sw128(sV, box * 128, 0), 0);
+    uint32_t v_at[N / 16];
+#pragma unroll
+    for (int k = 0; k < N / 16; ++k) {
+      const int lks = lbox - 4;  // log2 of the 16-key steps per page
+      v_at[k] = __shfl_sync(FULL, v_lo + (((k >> lks) * box * (D * 2) + (k & ((1 << lks) - 1)) * 2048) >> 4), 0);
+    }
+    const bool lead = elect_one();
+    auto wait = [&](uint64_t* bar, int phase) -> bool {
+      return __all_sync(FULL, mbar_wait(smem_u32(bar), phase & 1, abort_v, p.err));
+    };
+    // S = Q K^T of chunk g; its commit frees the K slot and tells the softmax.
+    auto next_s = [&](int g) -> bool {
+      const int ks = g % NSK;
+      if (!wait(&bar_k_full[ks], g / NSK)) return false;
+      tc_fence_after();
+      const uint32_t d = tm + SB + (g & 1) * N;
+      const uint32_t k_at = k_lo + ((ks * Cfg::kKVBytes) >> 4);
+      if (lead) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const int r = k >> 2, kk = k & 3;
-          mma_ss(d, q_desc + ((r * kChM * 128 + kk * 32) >> 4), kst + ((r * N * 128 + kk * 32) >> 4), idesc_s,
-                 k > 0 ? 1u : 0u);
+          mma_ss(d, desc_up | (q_lo + ((r * kChM * 128 + kk * 32) >> 4)), desc_up | (k_at + ((r * N * 128 + kk * 32) >> 4)),
+                 idesc_s, k > 0 ? 1u : 0u);
         }
         mma_commit(smem_u32(&bar_k_empty[ks]));
-        return true;
-      };
-      bool ok = mbar_wait(smem_u32(&bar_q), 0, abort_v, p.err) && next_s(0);
-      for (int g = 0; ok && g < nch; ++g) {
-        // S of the next chunk goes in before this chunk's PV.
-        if (g + 1 < nch && !(ok = next_s(g + 1))) break;
-        const int vs = g % NSV;
-        if (!(ok = mbar_wait(smem_u32(&bar_v_full[vs]), (g / NSV) & 1, abort_v, p.err))) break;
-        if (!(ok = mbar_wait(smem_u32(&bar_p_full[g & 1]), (g >> 1) & 1, abort_v, p.err))) break;
-        tc_fence_after();
-        const uint32_t pbuf = tmem + SB + (g & 1) * N;
-        const uint64_t vst = v_desc + (uint64_t)((vs * Cfg::kKVBytes) >> 4);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = wait(&bar_q, 0) && next_s(0);
+    for (int g = 0; ok && g < n; ++g) {
+      // S of the next chunk goes in before this chunk's PV.
+      if (g + 1 < n && !(ok = next_s(g + 1))) break;
+      const int vs = g % NSV;
+      if (!(ok = wait(&bar_v_full[vs], g / NSV))) break;
+      if (!(ok = wait(&bar_p_full[g & 1], g >> 1))) break;
+      tc_fence_after();
+      const uint32_t pbuf = tm + SB + (g & 1) * N;
+      const uint32_t v_off = (vs * Cfg::kKVBytes) >> 4;
+      if (lead) {
 #pragma unroll
         for (int k = 0; k < N / 16; ++k)
-          mma_ts(tmem, pbuf + k * 8,
-                 vst + (uint64_t)(((k >> lks) * box * (D * 2) + (k & ((1 << lks) - 1)) * 2048) >> 4), idesc_pv,
-                 (k > 0 || g > 0) ? 1u : 0u);
+          mma_ts(tm, pbuf + k * 8, desc_up | (v_at[k] + v_off), idesc_pv, (k > 0 || g > 0) ? 1u : 0u);
         mma_commit(smem_u32(&bar_v_empty[vs]));  // PV of chunk g retired: V slot free, O holds it
       }
-      mma_commit(smem_u32(&bar_drain));
-      int zero = 0;
-      mbar_wait(smem_u32(&bar_drain), 0, &zero, nullptr);
+      __syncwarp();
     }
+    if (lead) mma_commit(smem_u32(&bar_drain));
+    int zero = 0;
+    mbar_wait(smem_u32(&bar_drain), 0, &zero, nullptr);
   } else {
     // ------------------------------------------------------------------ softmax
     const int wr = warp & 3;  // TMEM lane quadrant this warp may access
