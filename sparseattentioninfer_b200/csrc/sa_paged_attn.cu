@@ -516,17 +516,20 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   r.chunk = group <= 128 && (int64_t)a.max_q * group > 48;
   r.page_cap = 0;
   if (a.blocks) {
-    // The rows kernel reads every token's pages, a tile the union of its tokens'.
-    // Both in 64-key steps: 3.2 ns each in all against 6.3 (whole GPU) and no less
-    // than about 0.9 us a step of one tile (of a split tile's part), 13 us more for
-    // the union and the tile's start and end. The union is taken as of lists drawn at random; real neighbours share more.
-    const double ps = a.batch.page_size, tokens = a.max_q < 128 / group ? a.max_q : 128 / group;
+    // The rows kernel reads every token's pages, a tile the union of its tokens',
+    // taken as of lists drawn at random (real neighbours share more). Times fitted to
+    // 45 drawn calls, where they pick the slower kernel (by more than 5%) twice: rows,
+    // ns a token and kv head: 8 and 2.6 a 64-key step (heads of 64: 6 and 1.5); tiles:
+    // 4 ns a step and tile over the whole GPU (3), ten steps' worth for a tile's start
+    // and end, and no less than 1.2 us a step of one tile's part.
+    const double ps = a.batch.page_size, tokens = a.max_q < 128 / group ? a.max_q : 128 / group, w = a.D / 128.;
     const double seen = ceil((double)longest / ps), kept = a.n_blocks < seen ? a.n_blocks : seen;
     const double pages = seen * (1. - pow(1. - kept / seen, tokens)), steps = pages * ps / kRowKeys;
-    const double lines = (a.batch.N / (128. / group) + 1.) * a.Hkv;
-    const double rows_us = 0.0032 * a.batch.N * a.Hkv * ceil(kept * ps / kRowKeys);
+    const double lines = fmax(a.batch.N / (128. / group) + 1., fmin(a.batch.B, a.batch.N)) * a.Hkv;
+    const double rows_us =
+        6. + 0.001 * a.batch.N * a.Hkv * (4. + 4. * w + (0.4 + 2.2 * w) * ceil(kept * ps / kRowKeys));
     const double parts = fmax(1., fmin(fmin(8., 2 * sms / lines), steps / 4));
-    const double tile_us = 13. + fmax(0.0063 * lines * steps, 0.9 * steps / parts);
+    const double tile_us = 12. + fmax(0.001 * (2. + 2. * w) * lines * (steps + 10.), 1.2 * (steps / parts + 4.));
     r.chunk = r.chunk && a.batch.max_pages <= kChunkMaxPages && tile_us < rows_us;
     if (r.chunk) {
       r.page_cap = (int64_t)(128 / group) * a.n_blocks;
