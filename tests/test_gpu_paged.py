@@ -179,6 +179,37 @@ def test_sparse_attention(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, keep, 
     _assert_attention(bt, out, q, k, v, 1 / math.sqrt(D), blocks, before)
 
 
+# Calls that tiles of 128 rows serve, over kept pages too: groups that divide 128 and
+# that do not, more pages than one, two and three batches of 32, single tokens and
+# sequences without new ones among the chunks.
+TILES = [
+    ([2100, 0], [260, 100], 4, 4, 128, 16, torch.bfloat16, "heads", 3),
+    ([1000, 40, 7], [333, 64, 1], 16, 8, 64, 16, torch.float16, "slots", 0),
+    ([1600, 0, 3], [70, 290, 0], 24, 8, 64, 32, torch.bfloat16, "wide", 2),
+    ([129, 0], [150, 301], 40, 8, 128, 64, torch.bfloat16, "heads", 0),
+    ([4500], [500], 6, 6, 64, 64, torch.float16, "heads", 1),
+    ([600, 0], [190, 400], 20, 10, 128, 128, torch.float16, "heads", 0),
+]
+
+
+@pytest.mark.parametrize("ctx,new,Hq,Hkv,D,page,dtype,layout,pad", TILES)
+@pytest.mark.parametrize("keep", [None, 3, 40])
+@pytest.mark.parametrize("split_len", [None, 192])
+def test_tiles(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, keep, split_len):
+    bt = P.Batch(ctx, new, Hq=Hq, Hkv=Hkv, D=D, page=page, dtype=dtype, device=DEV, seed=D + page, pad=pad,
+                 layout=layout)
+    q, k, v = _qkv(bt)
+    blocks = None if keep is None else _random_blocks(bt, keep, seed=1, empty=True)
+    kw = dict(max_q=max(new), max_len=max(bt.lens), split_len=split_len,
+              blocks=None if blocks is None else blocks.to(DEV))
+    if keep == 40:  # (room for the unions of the lists: tiles it is; three small pages may go by rows)
+        assert ops.paged_attention_workspace(q.to(DEV), k, v, *bt.batch, **kw) > 0
+    out = torch.full((bt.N, Hq, D), 3.0, dtype=dtype, device=DEV)
+    before = out.clone()
+    ops.paged_attention(q.to(DEV), k, v, *bt.batch, out=out, **kw)
+    _assert_attention(bt, out, q, k, v, 1 / math.sqrt(D), blocks, before)
+
+
 def test_attention_scale_and_strided_rows():
     bt = P.Batch([40, 3], [5, 9], Hq=4, Hkv=2, D=64, page=16, device=DEV)
     q, k, v = _qkv(bt)
