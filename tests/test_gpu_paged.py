@@ -471,3 +471,37 @@ def test_a_sequence_with_nan_does_not_reach_the_others():
     for w, m in zip(want, (1, 20)):
         got = ops.paged_attention(q.to(DEV), k, v, *bt.batch, max_q=m)
         assert torch.equal(got[:20], w[:20]) and torch.equal(got[21:], w[21:]) and got[20].isnan().all()
+
+
+def test_bad_lists_and_pages_in_tiles():
+    """Lists that do not ascend, entries behind the token and pages that are not there
+    are reported; rows that do not keep them come out right."""
+    bt = P.Batch([700, 60], [250, 150], Hq=8, Hkv=4, D=128, page=32, device=DEV, seed=9)
+    q, k, v = _qkv(bt)
+    table, cu, lens = bt.batch
+    blocks = _random_blocks(bt, 20)
+    bad_rows = {4: [2, 2], 37: [0, 3, 10 ** 6], 255: [5, 1, 2], 300: [0, 6, 7]}  # (300 sees 3 pages)
+    for r, entries in bad_rows.items():
+        blocks[r, 1] = -1
+        blocks[r, 1, :len(entries)] = torch.tensor(entries)
+    kw = dict(max_q=250, max_len=max(bt.lens))
+    assert ops.paged_attention_workspace(q.to(DEV), k, v, table, cu, lens, blocks=blocks.to(DEV), **kw) > 0  # tiles
+    got = torch.full(q.shape, 3.0, dtype=q.dtype, device=DEV)
+    ops.paged_attention(q.to(DEV), k, v, table, cu, lens, blocks=blocks.to(DEV), out=got, **kw)
+    assert _capi.device_error() == 2
+    sound = blocks.clone()
+    for r in bad_rows:
+        sound[r, 1] = -1
+    ref, mag = P.attention(bt, q, k, v, 128 ** -0.5, sound)
+    ok = ((got.cpu().double() - ref).abs() <= P.attention_tolerance(ref, mag, q.dtype)).all(-1)  # [N, Hq]
+    ok[list(bad_rows), 2:4] = True  # (the two heads of kv head 1)
+    assert ok.all()
+    t = table.clone()
+    t[0, 7] = bt.pages
+    sound = torch.where((blocks == 7) & (torch.arange(bt.N) < 250)[:, None, None], -2, blocks)
+    keeps = (sound == -2).any(-1)  # [N, Hkv]
+    ops.paged_attention(q.to(DEV), k, v, t, cu, lens, blocks=blocks.to(DEV), out=got, **kw)
+    assert _capi.device_error() == 2
+    ok = ((got.cpu().double() - ref).abs() <= P.attention_tolerance(ref, mag, q.dtype)).all(-1)
+    ok[list(bad_rows), 2:4] = True
+    assert (ok | keeps.repeat_interleave(2, 1)).all() and keeps.any() and not keeps.all()
