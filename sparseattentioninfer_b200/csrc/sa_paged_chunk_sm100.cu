@@ -19,6 +19,11 @@
 // Slots behind the last key may hold anything: S there is masked, and V's rows
 // are set to zero in shared memory by the softmax warps before P is handed over.
 // Unsplit tiles write out = O / l; split ones their O, maximum and sum.
+// A step of 128 rows x 64 keys takes an SM some 930 cycles at heads of 128: 640 of
+// the tensor pipe (Q K^T has to read 6 KB of shared memory for 32 cycles of products),
+// 512 of the exponentials' units, and neither is full; 520 ns on tiles of 8k keys,
+// 1,190 TFLOP/s. Two softmax threads a row were 4.5% slower, exponentials on the FMA
+// pipe 1 to 11%.
 //
 // With kept pages a tile walks the union of its tokens' lists (a small kernel
 // before writes it, ascending) and each row follows its own list along: the next
