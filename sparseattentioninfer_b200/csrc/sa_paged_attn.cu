@@ -509,11 +509,19 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   const int group = a.Hq / a.Hkv;
   const int64_t cap = (int64_t)a.batch.max_pages * a.batch.page_size;
   int64_t longest = a.max_len < cap ? a.max_len : cap;  // keys of the longest unit
-  // Up to three 16-row units a sequence the rows kernel, above the chunk kernel:
-  // 16 sequences of 16k keys, 8 kv heads of 128: 32 rows 217 us against 180, 64
-  // rows 367 against 178; of 2k keys 34 against 37 and 61 against 40; one sequence
-  // of 2k keys 11 against 13 and 14 against 14.
-  r.chunk = group <= 128 && (int64_t)a.max_q * group > 48;
+  // Above three 16-row units a sequence the tiles: 16 sequences of 16k keys, 8 kv heads
+  // of 128, 64 rows 366 us by rows and 180 by tiles, of 2k keys 60 and 35; one sequence
+  // of 2k keys 14 and 12. One unit: the rows kernel. Between them by the load: with
+  // enough of it a tile costs as much as 1.7 units (heads of 64: 2.4), with little the
+  // tiles' longer start counts. 24 to 48 rows, heads of 128 (rows, tiles, us): 32 lines
+  // of 500 keys 10 and 11, of 2k 21-24 and 18, of 8k 45-52 and 33; 512 lines of 500
+  // keys 48-68 and 39-41, of 8k 392-569 and 349-355; 8 lines of 8k keys 21 and 22.
+  const int64_t rows = (int64_t)a.max_q * group, some = a.batch.B < a.batch.N ? a.batch.B : a.batch.N;
+  r.chunk = group <= 128 && rows > 48;
+  if (!r.chunk && !a.blocks && group <= 128 && rows > 16) {
+    const double units = ceil((double)a.batch.N * group / (16. * some)), tiles = (double)some * a.Hkv;
+    r.chunk = units >= (a.D == 128 ? 2 : 3) && tiles >= 16 && tiles * (longest - 400.) >= 48000.;
+  }
   r.page_cap = 0;
   if (a.blocks) {
     // The rows kernel reads every token's pages, a tile the union of its tokens',
@@ -560,7 +568,7 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   // ran in two waves on 148 SMs, 16 in one).
   const int64_t resident = sms * 7 / 8;
   // Tiles that the batch has at least: full ones, and one a sequence.
-  const int64_t full = a.batch.N / r.tq + 1, some = a.batch.B < a.batch.N ? a.batch.B : a.batch.N;
+  const int64_t full = a.batch.N / r.tq + 1;
   const int64_t lines = (r.tq == 1 ? r.units : full > some ? full : some) * a.Hkv * r.nhg;
   if (a.split_len <= 0) {
     if (r.chunk) {

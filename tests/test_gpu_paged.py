@@ -210,6 +210,17 @@ def test_tiles(ctx, new, Hq, Hkv, D, page, dtype, layout, pad, keep, split_len):
     _assert_attention(bt, out, q, k, v, 1 / math.sqrt(D), blocks, before)
 
 
+@pytest.mark.parametrize("D,new", [(128, 5), (64, 9), (128, 1)])
+@pytest.mark.parametrize("hint", [None, 1, 3])
+def test_drafts_of_many_sequences(D, new, hint):
+    """A few tokens of each of many sequences: by rows or by tiles, whichever the sizes ask for."""
+    bt = P.Batch([1500 + 7 * i for i in range(40)], [new - i % 2 * (new > 1) for i in range(40)], Hq=8, Hkv=2, D=D,
+                 page=32, device=DEV)
+    q, k, v = _qkv(bt)
+    got = ops.paged_attention(q.to(DEV), k, v, *bt.batch, max_q=hint or new, max_len=max(bt.lens))
+    _assert_attention(bt, got, q, k, v, 1 / math.sqrt(D))
+
+
 def test_attention_scale_and_strided_rows():
     bt = P.Batch([40, 3], [5, 9], Hq=4, Hkv=2, D=64, page=16, device=DEV)
     q, k, v = _qkv(bt)
