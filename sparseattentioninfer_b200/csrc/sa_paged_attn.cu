@@ -497,11 +497,38 @@ struct AttnPlan {
   int64_t workspace(const sa_paged_attn_args& a) const { return part + units * a.Hkv * (page_cap + (page_cap > 0)); }
 };
 
-// The largest power of two that is at most n and at most `most`, 1 at least.
-static int64_t pow2_below(int64_t n, int64_t most) {
-  int64_t r = 1;
-  while (2 * r <= n && 2 * r <= most) r *= 2;
-  return r;
+// How many clusters of n CTAs, an SM for each CTA, the device holds at once. A cluster
+// has to fit in one GPC, whose sizes differ from chip to chip: with 148 SMs 16 of 8 CTAs
+// ran in one wave on one, in two on another (24 rows over 2k keys, 8 kv heads: 15.7 us,
+// in clusters of 7 10.3). Asked once a device and n.
+static int64_t clusters_at_once(int n, int sms) {
+  static int known[64][9];
+  if (n == 1) return sms;
+  using Cfg = PagedRowCfg<128, 16, true>;
+  auto kern = paged_rows_kernel<__nv_bfloat16, 128, false, 16, true>;
+  static bool done[64];
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms * 7 / 8 / n;
+  if (known[dev][n] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(n * sms));
+    cfg.blockDim = dim3(Cfg::kThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)n;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int found = 0;
+    if (sa_smem_once(reinterpret_cast<const void*>(kern), Cfg::kSmemBytes, done) != 0 ||
+        cudaOccupancyMaxActiveClusters(&found, kern, &cfg) != cudaSuccess || found < 1) {
+      cudaGetLastError();
+      return sms * 7 / 8 / n;
+    }
+    known[dev][n] = found;
+  }
+  return known[dev][n] < sms / n ? known[dev][n] : sms / n;
 }
 
 static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
@@ -563,10 +590,12 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   longest = (longest + kRowKeys - 1) / kRowKeys * kRowKeys;
   int64_t len = ((int64_t)a.split_len + kRowKeys - 1) / kRowKeys * kRowKeys;
   const int64_t slots = (r.chunk || a.D == 128 ? 2ll : 4ll) * sms;  // resident CTAs
-  // Those of a grid of clusters with an SM for each CTA: up to 8 CTAs have to fit in
-  // one GPC, which leaves some of its SMs over (18 clusters of 8, 144 CTAs in all,
-  // ran in two waves on 148 SMs, 16 in one).
-  const int64_t resident = sms * 7 / 8;
+  // Units with tokens (others that are launched leave at once): known where every
+  // sequence brings max_q, else as if a sequence's last unit were half full.
+  const int64_t even = (int64_t)a.batch.B * ((a.max_q + r.tq - 1) / r.tq);
+  const double guess = ceil((double)a.batch.N / r.tq + a.batch.B * (r.tq - 1.) / (2. * r.tq));
+  const double likely = r.tq == 1 ? r.units : (int64_t)a.batch.B * a.max_q == a.batch.N ? even : fmax(guess, some);
+  auto fits = [&](int64_t n) { return n <= 8 && likely * a.Hkv * r.nhg <= clusters_at_once((int)n, sms); };
   // Tiles that the batch has at least: full ones, and one a sequence.
   const int64_t full = a.batch.N / r.tq + 1;
   const int64_t lines = (r.tq == 1 ? r.units : full > some ? full : some) * a.Hkv * r.nhg;
@@ -602,12 +631,13 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
       // one wave. 256 keys each at least.
       len = 4096;
       if (2 * lines < slots) {
-        const int64_t fit = pow2_below(resident / lines, 8);
+        int64_t fit = 8;
+        while (fit > 1 && !fits(fit)) --fit;
         const int64_t splits = fit >= 2 && longest <= fit * 2048 ? fit : (slots + lines - 1) / lines;
         len = (longest + splits - 1) / splits;
         if (len < 256) len = 256;
         // (the second kernel costs about 4 us, as long as 400 keys take a CTA)
-        if (lines * splits > resident && longest - len < 400) len = longest;
+        if (!fits(splits) && longest - len < 400) len = longest;
         if (len > 4096) len = 4096;
       }
     }
@@ -621,8 +651,7 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   // A cluster's CTAs wait for one another. The rows kernel's splits are of equal
   // length, and short units leave some of them without keys: clusters only where
   // the whole grid is resident at once. Tiles are cut into equal parts: always.
-  const int64_t grid = r.units * r.n_split * a.Hkv * r.nhg;
-  r.wide = !r.chunk && r.n_split <= 8 && grid <= (r.n_split > 1 ? resident : sms);
+  r.wide = !r.chunk && fits(r.n_split);
   r.cluster = r.chunk && r.n_split > 1 && r.n_split <= 8;
   r.part = r.n_split > 1 && !r.wide && !r.cluster ? (int64_t)a.batch.N * a.Hq * r.n_split * (a.D + 2) : 0;
   return r;
