@@ -335,7 +335,7 @@ SA_API int sa_topk_softmax_pv(const sa_topk_args* args, sa_stream_t stream);
  * What they must keep (0 <= cu_q[b] <= cu_q[b+1] <= N, n_b <= seq_lens[b] <=
  * max_pages * page_size, page numbers in [0, num_pages)) is checked there: a
  * violation sets SA_DEV_ERR_INDEX in the device error word and the sequence, or
- * the page's keys, are left out.
+ * the page's keys, are left out (where offsets decrease, any rows may be).
  * page_size: 16, 32, 64 or 128. D: 64 or 128. dtype: SA_BF16 or SA_FP16, one
  * for every 16-bit tensor of a call.
  * ------------------------------------------------------------------------- */
@@ -386,8 +386,10 @@ SA_API int sa_paged_append(const sa_paged_append_args* args, sa_stream_t stream)
  * kv head h / (Hq / Hkv). With blocks [N, Hkv, n_blocks] (logical page indexes,
  * strictly ascending, -1 behind the last) token t of a kv head sees only the
  * listed pages; an index that does not ascend or lies behind the token sets
- * SA_DEV_ERR_INDEX, and entries of its list may be left out. A row that sees no key is 0. Slots past a
- * sequence's length are never used, whatever they hold.
+ * SA_DEV_ERR_INDEX, and entries of its list may be left out. A row that sees no
+ * key is 0. Slots past a sequence's length are never used, whatever they hold; V
+ * of the keys of a sequence has to be finite for those of its new tokens that do
+ * not see them and share a tile with one that does (0 times infinity is NaN).
  * max_q (most new tokens of one sequence) and max_len (most keys) only steer the
  * choice of kernel and the split of long sequences: any value >= 1 is correct
  * for max_q; max_len must not be exceeded (SA_DEV_ERR_INDEX, keys cut).

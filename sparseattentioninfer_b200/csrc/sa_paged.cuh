@@ -40,15 +40,20 @@ struct UnitTokens {
 // All lanes of a warp call it with the same u.
 // Sequences whose offsets decrease or leave [0, N], or that hold fewer keys than
 // new tokens, are dropped (with SA_DEV_ERR_INDEX); a length beyond the table is cut.
+// The search takes the offsets as ascending: who has unit 0 looks at all of them.
 __device__ __forceinline__ bool unit_tokens(const sa_paged_batch& bt, int64_t u, int tq, int32_t* err,
                                             UnitTokens& r) {
   const int32_t* cu = bt.cu_q;
+  bool mixed = false;
+  if (u == 0 && err)
+    for (int b = threadIdx.x & 31; b < bt.B; b += 32) mixed |= __ldg(cu + b) > __ldg(cu + b + 1);
   if (tq == 1) {
     r.b = last_start(bt.B, u, [&](int b) { return (int64_t)__ldg(cu + b); });
   } else {
     r.b = last_start(bt.B, u, [&](int b) { return (int64_t)__ldg(cu + b) / tq + b; });
   }
   const int c0 = __ldg(cu + r.b), c1 = __ldg(cu + r.b + 1), full = __ldg(bt.seq_lens + r.b);
+  if (mixed) record_error(err, SA_DEV_ERR_INDEX);
   const int64_t first = tq == 1 ? u : c0 + (u - (c0 / tq + r.b)) * (int64_t)tq;
   if (first < c0 || first >= c1) return false;  // an empty unit, or rows behind the last sequence
   const int cap = (int)min((int64_t)bt.max_pages * bt.page_size, (int64_t)0x7fffffff);
@@ -66,8 +71,10 @@ __device__ __forceinline__ bool unit_tokens(const sa_paged_batch& bt, int64_t u,
 // Unit number of the u-th tile when tiles are taken longest sequence first and,
 // of one sequence, last tokens (the most keys) first; -1 behind the last tile.
 // One lane a sequence: for up to 32 of them. Longer batches keep their order,
-// from the end: among many sequences the long ones spread by themselves.
-__device__ __forceinline__ int64_t longest_first(const sa_paged_batch& bt, int64_t u, int64_t units, int tq) {
+// from the end: among many sequences the long ones spread by themselves. What
+// unit_tokens would drop has no tiles here (and is reported).
+__device__ __forceinline__ int64_t longest_first(const sa_paged_batch& bt, int64_t u, int64_t units, int tq,
+                                                 int32_t* err) {
   if (bt.B > 32) return units - 1 - u;
   constexpr unsigned A = 0xffffffffu;
   const int lane = threadIdx.x & 31;
@@ -75,8 +82,12 @@ __device__ __forceinline__ int64_t longest_first(const sa_paged_batch& bt, int64
   int64_t start = 0;
   if (lane < bt.B) {
     const int c0 = __ldg(bt.cu_q + lane), c1 = __ldg(bt.cu_q + lane + 1);
-    tiles = max(0, (c1 - c0 + tq - 1) / tq);
     len = __ldg(bt.seq_lens + lane);
+    const bool sound = c0 >= 0 && c0 <= c1 && c1 <= bt.N && c1 - c0 <= len;
+    if (sound)
+      tiles = (c1 - c0 + tq - 1) / tq;
+    else if (c0 != c1)
+      record_error(err, SA_DEV_ERR_INDEX);
     start = tq == 1 ? c0 : c0 / tq + lane;
   }
   int before = 0;  // tiles of longer sequences

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
   const int kvh = (int)(tile % a.Hkv);
   const int64_t rest = p.cluster ? tile / a.Hkv * p.n_split : tile / a.Hkv;
   const int split = (int)(p.cluster ? blockIdx.x % p.n_split : rest % p.n_split);
-  const int64_t unit = longest_first(bt, rest / p.n_split, units, p.tq);
+  const int64_t unit = longest_first(bt, rest / p.n_split, units, p.tq, p.err);
   UnitTokens ut;
   if (unit < 0 || !unit_tokens(bt, unit, p.tq, p.err, ut)) return;
   const int keys = unit_keys(ut, a.max_len);

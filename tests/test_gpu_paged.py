@@ -484,6 +484,34 @@ def test_a_sequence_with_nan_does_not_reach_the_others():
         assert torch.equal(got[:20], w[:20]) and torch.equal(got[21:], w[21:]) and got[20].isnan().all()
 
 
+@pytest.mark.parametrize("max_q", [1, 64])
+def test_offsets_that_leave_the_batch_or_decrease(max_q):
+    """A last offset far behind the batch drops the last sequence alone, the longest
+    though it is; offsets that decrease are reported by each operator."""
+    bt = P.Batch([20, 0, 300], [3, 30, 5], Hq=8, Hkv=2, D=64, page=16, device=DEV)
+    q, k, v = _qkv(bt)
+    table, cu, lens = bt.batch
+    ref, mag = P.attention(bt, q, k, v, 0.125)
+    far = cu.clone()
+    far[3] = 2 ** 30
+    out = torch.full(q.shape, 7.0, dtype=q.dtype, device=DEV)
+    ops.paged_attention(q.to(DEV), k, v, table, far, lens, max_q=max_q, out=out)
+    assert _capi.device_error() == 2
+    ok = (out.cpu().double() - ref).abs() <= P.attention_tolerance(ref, mag, q.dtype)
+    assert ok[:33].all() and (out[33:] == 7).all()
+    bounds = P.bounds_of(bt, k).to(DEV)
+    cos, sin = (x.to(DEV) for x in rope_tables(400, 64, torch.bfloat16))
+    x = torch.randn(bt.N, 12, 64, generator=bt.g).to(torch.bfloat16).to(DEV)
+    for bad in ([0, 9, 3, 38], [0, 33, 3, 3], [0, 3, 33, 20]):
+        c = torch.tensor(bad, dtype=torch.int32, device=DEV)
+        ops.paged_attention(q.to(DEV), k, v, table, c, lens, max_q=max_q)
+        assert _capi.device_error() == 2, bad
+        ops.paged_block_select(q.to(DEV), bounds, table, c, lens, page_size=16, keep=4, max_q=max_q)
+        assert _capi.device_error() == 2, bad
+        ops.paged_qk_norm_rope_append(x, None, None, cos, sin, k.clone(), v.clone(), table, c, lens, Hq=8, Hkv=2)
+        assert _capi.device_error() == 2, bad
+
+
 def test_bad_lists_and_pages_in_tiles():
     """Lists that do not ascend, entries behind the token and pages that are not there
     are reported; rows that do not keep them come out right."""
