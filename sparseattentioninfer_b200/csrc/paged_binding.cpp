@@ -144,6 +144,14 @@ PyObject* guarded(Py_ssize_t have, Py_ssize_t want, F f) {
     if (have != want) raise(PyExc_TypeError, "%zd arguments expected, got %zd", want, have);
     return f();
   } catch (const Raised&) {
+  } catch (const c10::OutOfMemoryError& e) {
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    if (type) PyErr_SetString(type, e.what_without_backtrace());
+    Py_XDECREF(type);
+    Py_XDECREF(torch);
+  } catch (const c10::Error& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }

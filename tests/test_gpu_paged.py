@@ -512,6 +512,15 @@ def test_offsets_that_leave_the_batch_or_decrease(max_q):
         assert _capi.device_error() == 2, bad
 
 
+def test_out_of_memory_is_torchs_own_error():
+    """A result that does not fit is refused by the allocator before anything is launched."""
+    q = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device=DEV)
+    k = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16, device=DEV)
+    i = torch.zeros(2, dtype=torch.int32, device=DEV)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.paged_block_select(q.expand(2 ** 28, 1, 64), k, i[:1].view(1, 1), i, i[:1], page_size=16, keep=4096)
+
+
 def test_bad_lists_and_pages_in_tiles():
     """Lists that do not ascend, entries behind the token and pages that are not there
     are reported; rows that do not keep them come out right."""
