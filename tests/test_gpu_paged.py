@@ -2,6 +2,9 @@
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -510,6 +513,38 @@ def test_offsets_that_leave_the_batch_or_decrease(max_q):
         assert _capi.device_error() == 2, bad
         ops.paged_qk_norm_rope_append(x, None, None, cos, sin, k.clone(), v.clone(), table, c, lens, Hq=8, Hkv=2)
         assert _capi.device_error() == 2, bad
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    """Nothing that the operators set up once needs a call before the capture."""
+    code = """
+import torch
+from sparseattentioninfer_b200 import _capi, ops
+D, N, dev = 128, 3, "cuda"
+k, v = (torch.randn(64, 2, 16, D, device=dev).bfloat16() for _ in range(2))
+bounds = torch.zeros(64, 2, 2, D, device=dev, dtype=torch.bfloat16)
+table = torch.arange(64, device=dev, dtype=torch.int32).view(1, 64)
+cu = torch.tensor([0, N], device=dev, dtype=torch.int32)
+lens = torch.tensor([900], device=dev, dtype=torch.int32)
+cos, sin = (torch.randn(1024, D, device=dev).bfloat16() for _ in range(2))
+qkv = torch.randn(N, 12, D, device=dev).bfloat16()
+def step():
+    q = ops.paged_qk_norm_rope_append(qkv, None, None, cos, sin, k, v, table, cu, lens, Hq=8, Hkv=2, k_bounds=bounds)
+    kept = ops.paged_block_select(q, bounds, table, cu, lens, page_size=16, keep=8, max_q=N)
+    return [q, kept] + [ops.paged_attention(q, k, v, table, cu, lens, **kw) for kw in
+            (dict(max_q=N), dict(max_q=N, max_len=1024, split_len=64), dict(max_q=64), dict(blocks=kept, max_q=N))]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in got]
+assert all(torch.equal(a, b) for a, b in zip(got, step())) and _capi.device_error() == 0
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=str(Path(__file__).resolve().parents[1]))
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
 
 
 def test_out_of_memory_is_torchs_own_error():
