@@ -471,24 +471,47 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
       const uint32_t sbuf = tmem + lane_base + SB + (g & 1) * N;
       const int off = SPARSE ? ((c0 + g) & (spp - 1)) * N : (c0 + g) * N;  // first key, in its page or of all
       int lim[4];  // column i of the chunk is seen when i % 16 <= lim[i / 16]
-      bool plain = true, skip = false, tail = false;
+      int how = 0;
+      bool plain = true, skip = false, tail = false, drop = false;
       if constexpr (SPARSE) {
-        bool any = false;
+        bool any = false, cut = false;
+        auto advance = [&]() {
+          ++ptr;
+          want = ahead;
+          ahead = want == kNone ? kNone : entry_at(ptr + 1);
+        };
+        if (pps == 1) {
+          const int blk = meta_blk[batch & 1][first & 31];
+          const int to = pos - blk * ps - off;  // last column that the row sees of it
+          const bool mine = blk == want, seen = mine && (have & 1u);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int jp = q * 16 >> lbox, blk = meta_blk[batch & 1][(first & 31) + jp];
-          const int key0 = blk * ps + off + q * 16 - jp * box;
-          lim[q] = blk == want && ((have >> jp) & 1u) ? min(pos - key0, 15) : -1;
-          plain &= lim[q] == 15;
-          any |= lim[q] >= 0;
-          tail |= blk >= 0 && key0 + 16 > keys;
-          if (((q + 1) * 16 & (box - 1)) == 0 && blk == want && ((c0 + g) & (spp - 1)) == spp - 1) {
-            ++ptr;
-            want = ahead;
-            ahead = want == kNone ? kNone : entry_at(ptr + 1);
+          for (int q = 0; q < 4; ++q) lim[q] = seen ? min(to - q * 16, 15) : -1;
+          plain = seen && to >= N - 1;
+          any = seen && to >= 0;
+          cut = any && !plain;
+          tail = blk >= 0 && blk * ps + off > keys - N;
+          if (mine && ((c0 + g) & (spp - 1)) == spp - 1) advance();
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int jp = q * 16 >> lbox, blk = meta_blk[batch & 1][(first & 31) + jp];
+            const int key0 = blk * ps + off + q * 16 - jp * box;
+            lim[q] = blk == want && ((have >> jp) & 1u) ? min(pos - key0, 15) : -1;
+            plain &= lim[q] == 15;
+            any |= lim[q] >= 0;
+            cut |= lim[q] >= 0 && lim[q] < 15;
+            tail |= blk >= 0 && key0 > keys - 16;
+            if (((q + 1) * 16 & (box - 1)) == 0 && blk == want) advance();
           }
         }
         skip = !__any_sync(FULL, any);  // no row of the warp sees the chunk
+        // Where every row of the warp sees the whole chunk or none of it, the scores stay
+        // as they are and P is set to zero; else 16 of them together or one by one.
+        drop = !any;
+        if (__all_sync(FULL, plain || drop))
+          how = 0;
+        else
+          how = __any_sync(FULL, cut) ? 2 : 1;
       } else {
         const uint32_t all = (1u << pps) - 1u;
         plain = pos - off >= N - 1 && (have & all) == all;
@@ -497,6 +520,7 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         for (int q = 0; q < 4; ++q) lim[q] = ((have >> (q * 16 >> lbox)) & 1u) ? min(pos - off - q * 16, 15) : -1;
       }
       uint32_t pk[N / 2];
+      if (SPARSE && how > 0) drop = false;
       if (skip) {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) pk[i] = 0u;
@@ -514,16 +538,20 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
             for (int i = 0; i < 32; ++i) s[cc * 32 + i] = __uint_as_float(r32[cc][i]);
           }
         }
-        if (!plain) {
+        if (SPARSE ? how == 2 : !plain) {
 #pragma unroll
           for (int i = 0; i < N; ++i) s[i] = i % 16 <= lim[i / 16] ? s[i] : -INFINITY;
+        } else if (SPARSE && how == 1) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) s[i] = lim[i / 16] >= 0 ? s[i] : -INFINITY;
         }
         float mx8[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) mx8[i] = s[i];
 #pragma unroll
         for (int i = 8; i < N; i += 2) mx8[(i >> 1) & 7] = max3(mx8[(i >> 1) & 7], s[i], s[i + 1]);
-        const float mraw = max3(fmaxf(max3(mx8[0], mx8[1], mx8[2]), mx8[3]), max3(mx8[4], mx8[5], mx8[6]), mx8[7]);
+        float mraw = max3(fmaxf(max3(mx8[0], mx8[1], mx8[2]), mx8[3]), max3(mx8[4], mx8[5], mx8[6]), mx8[7]);
+        if (SPARSE && drop) mraw = -INFINITY;
         const float m_new = fmaxf(m_ref, mraw * p.scale_log2);
         // (a row that has seen no key yet has nothing in O to rescale)
         const bool need = m_ref > -INFINITY && m_new > m_ref + 8.0f;
@@ -561,7 +589,11 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         float a0, a1, b0, b1;
         f2unpack(add2(rs4[0], rs4[1]), a0, a1);
         f2unpack(add2(rs4[2], rs4[3]), b0, b1);
-        l += (a0 + a1) + (b0 + b1);
+        if (!(SPARSE && drop)) l += (a0 + a1) + (b0 + b1);
+        if constexpr (SPARSE) {
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i) pk[i] = drop ? 0u : pk[i];
+        }
       }
       tmem_st32(sbuf, pk);
       if (tail) {
