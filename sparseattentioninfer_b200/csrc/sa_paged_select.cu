@@ -370,7 +370,10 @@ __global__ void __launch_bounds__(kSelThreads, 3)
           if (n >= need) v = n3 >= need ? x3 : n2 >= need ? x2 : x1;
           whole = n == need;
         }
-        uint32_t k0 = v, k1 = v + ((1u << bits) - 1);  // the need-th key lies here
+        // The need-th key lies in [k0, k1], both of them keys of scores: bits may be all
+        // 32 where scores of both signs cancel far below eps, and not every pattern
+        // between is a number.
+        uint32_t k0 = max(v, kmin), k1 = bits < 32 ? min(v + ((1u << bits) - 1), kmax) : kmax;
         if (whole) {  // it is the smallest that reaches v (v > 0: no key is 0)
           uint32_t kth = 0;
           each([&](uint32_t k) { kth = k >= v ? max(kth, ~k) : kth; });
