@@ -393,8 +393,8 @@ SA_API int sa_paged_append(const sa_paged_append_args* args, sa_stream_t stream)
  * max_q (most new tokens of one sequence) and max_len (most keys) only steer the
  * choice of kernel and the split of long sequences: any value >= 1 is correct
  * for max_q; max_len must not be exceeded (SA_DEV_ERR_INDEX, keys cut).
- * workspace: sa_paged_attn_workspace(args) floats of device memory, used by this
- * call alone while it runs; 0 floats = may be NULL. Without one where it is
+ * workspace: sa_paged_attn_workspace(args) floats of device memory, 16-byte
+ * aligned, used by this call alone while it runs; 0 floats = may be NULL. Without one where it is
  * needed sa_paged_attn launches nothing and returns SA_ERR_WORKSPACE. */
 typedef struct sa_paged_attn_args {
   sa_paged_batch batch;

@@ -303,6 +303,8 @@ PyObject* attention(PyObject*, PyObject* const* o, Py_ssize_t n) {
     if (ws.scalar_type() != at::kFloat || ws.device() != c.dev || !ws.is_contiguous() || ws.numel() < need)
       raise(PyExc_ValueError, "%s: workspace must be %lld contiguous float32 on %s, got %s", c.op, (long long)need,
             c.dev.str().c_str(), text(ws).c_str());
+    if (reinterpret_cast<uintptr_t>(ws.data_ptr()) & 15u)
+      raise(PyExc_ValueError, "%s: workspace must be 16-byte aligned", c.op);
     a.workspace = static_cast<float*>(ws.data_ptr());
     return result(c.run(f_attn, a), out);
   });

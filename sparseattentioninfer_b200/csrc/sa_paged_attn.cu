@@ -789,6 +789,8 @@ extern "C" int sa_paged_attn(const sa_paged_attn_args* args, sa_stream_t stream_
   const AttnPlan r = attn_plan(*a, sms);
   if (r.workspace(*a) > 0 && !a->workspace)
     return sa_fail(SA_ERR_WORKSPACE, "paged attention: this call needs a workspace");
+  if (r.workspace(*a) > 0 && (reinterpret_cast<uintptr_t>(a->workspace) & 15u))
+    return sa_fail(SA_ERR_INVALID, "workspace must be 16-byte aligned");
   PagedAttnParams prm;
   memset(&prm, 0, sizeof(prm));
   if ((rc = sa_page_map(&prm.tm_k, *a, a->k_pages, a->k_strides, !r.chunk, "k_pages"))) return rc;

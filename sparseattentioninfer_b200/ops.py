@@ -527,9 +527,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``blocks`` [N, Hkv, n] int32 (paged_block_select's result): the token sees
     only these pages. ``max_q`` (most new tokens of one sequence) and ``max_len``
     (most keys of one sequence; must not be exceeded) only steer the launch;
-    their defaults are N and the page table's width. ``workspace``: float32
-    buffer of at least paged_attention_workspace(...) elements that a captured
-    call keeps to itself (allocated per call when None)."""
+    their defaults are N and the page table's width. ``workspace``: 16-byte
+    aligned float32 buffer of at least paged_attention_workspace(...) elements
+    that a captured call keeps to itself (allocated per call when None)."""
     return _paged_result(_PAGED.attention(q, k_pages, v_pages, page_table, cu_q, seq_lens, max_q, max_len, blocks, scale,
                                           split_len, out, workspace))
 
