@@ -261,6 +261,8 @@ bool attn_args(Call& c, PyObject* const* o, sa_paged_attn_args& a, Tensor* out) 
     const Tensor& b = c.tensor(o[8], "blocks");
     c.strides(b, "blocks", at::kInt, 2, a.blocks_strides);
     c.shape(b, "blocks", {N, k.size(1), b.size(2)});
+    // (a tensor without elements has no address, and none means no lists)
+    if (b.size(2) < 1) raise(PyExc_ValueError, "%s: blocks must have room for one page at least", c.op);
     a.blocks = static_cast<const int32_t*>(b.data_ptr());
     a.n_blocks = c.size(b.size(2), "blocks");
   }
