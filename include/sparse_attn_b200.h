@@ -356,8 +356,9 @@ typedef struct sa_paged_batch {
  *   q_out[t, h] = RoPE(RMSNorm(q)); k -> k_pages; v -> v_pages.
  * bounds [num_pages, Hkv, 2, D] (strides page, head, low/high; may be NULL):
  * lowest and highest value per channel over the keys that a page holds, as
- * stored; a page's first key starts them anew. fp32 arithmetic, one rounding
- * per stored value. A position >= positions or a bad page sets
+ * stored, written for every page that gets a key: of its slots up to the
+ * sequence's last key, so that a sequence may be cut short (rejected drafts)
+ * and go on. fp32 arithmetic, one rounding per stored value. A position >= positions or a bad page sets
  * SA_DEV_ERR_INDEX and that token (that page's k and v) is left out. */
 typedef struct sa_paged_append_args {
   sa_paged_batch batch;
@@ -394,8 +395,9 @@ SA_API int sa_paged_append(const sa_paged_append_args* args, sa_stream_t stream)
  * choice of kernel and the split of long sequences: any value >= 1 is correct
  * for max_q; max_len must not be exceeded (SA_DEV_ERR_INDEX, keys cut).
  * workspace: sa_paged_attn_workspace(args) floats of device memory, 16-byte
- * aligned, used by this call alone while it runs; 0 floats = may be NULL. Without one where it is
- * needed sa_paged_attn launches nothing and returns SA_ERR_WORKSPACE. */
+ * aligned, used by this call alone while it runs; 0 floats = may be NULL. Without
+ * one where it is needed sa_paged_attn launches nothing and returns
+ * SA_ERR_WORKSPACE. */
 typedef struct sa_paged_attn_args {
   sa_paged_batch batch;
   const void* q;

@@ -11,7 +11,9 @@
 // (they run longest), take the new tokens of one page of one kv head, so that
 // the page's bounds are the minimum and maximum of one warp: no atomics, and the
 // same bounds however the tokens were cut into calls (where sequences bring many
-// tokens the CTA's warps share a page); q warps take up to kQHeads heads at once of one token, whose cos/sin row stays in registers.
+// tokens the CTA's warps share a page). Keys that the page holds already are read
+// again for that: a sequence may have taken some back since the bounds were written;
+// q warps take up to kQHeads heads at once of one token, whose cos/sin row stays in registers.
 // 10,819 tokens, 32/8 heads of 128: 52 us, 5.2 TB/s; six CTAs a SM with two pairs of
 // tokens in flight (eight: 59 us, and spills; five: 55; four with four pairs: 57).
 #include "sa_paged.cuh"
@@ -222,21 +224,26 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 6)
     low[e] = INFINITY;
     high[e] = -INFINITY;
   }
-  auto widen = [&](const Raw<H>& lo, const Raw<H>& hi) {
+  auto widen = [&](const Raw<H>& k) {
 #pragma unroll
     for (int i = 0; i < H; ++i) {
-      const float2 l = Half<T>::unpack(lo.w[i]), h = Half<T>::unpack(hi.w[i]);
-      low[2 * i] = min_nan(low[2 * i], l.x);
-      low[2 * i + 1] = min_nan(low[2 * i + 1], l.y);
-      high[2 * i] = max_nan(high[2 * i], h.x);
-      high[2 * i + 1] = max_nan(high[2 * i + 1], h.y);
+      const float2 x = Half<T>::unpack(k.w[i]);
+      low[2 * i] = min_nan(low[2 * i], x.x);
+      low[2 * i + 1] = min_nan(low[2 * i + 1], x.y);
+      high[2 * i] = max_nan(high[2 * i], x.x);
+      high[2 * i + 1] = max_nan(high[2 * i + 1], x.y);
     }
   };
-  if (bd && p0 % ps) {
-    Raw<H> l, h;
-    l.load(bd);
-    h.load(bd + a.b_strides[2]);
-    widen(l, h);
+  // The keys that stay, before the page's first new one, are read again: the old bounds may
+  // still be of keys that the sequence has taken back (rejected drafts).
+  constexpr int S = 8;  // rows in flight, each half warp its own
+  const int stay = bd ? p0 & (ps - 1) : 0;
+  for (int p = (shared ? warp * 2 * S : 0) + half; p - half < stay; p += 2 * S * (shared ? kAppendWarps : 1)) {
+    Raw<H> k[S];
+#pragma unroll
+    for (int i = 0; i < S; ++i) k[i].load(kd + (int64_t)min(p + 2 * i, stay - 1) * a.k_strides[2]);
+#pragma unroll
+    for (int i = 0; i < S; ++i) widen(k[i]);
   }
   constexpr int U = 2;  // pairs of tokens in flight, a token per half warp
   const int first = p0 + (shared ? warp * 2 * U : 0), step = 2 * U * (shared ? kAppendWarps : 1);
@@ -260,7 +267,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 6)
       if (q < end) {
         k[i].store(kd + (int64_t)slot * a.k_strides[2]);
         v[i].store(vd + (int64_t)slot * a.v_strides[2]);
-        widen(k[i], k[i]);
+        widen(k[i]);
       }
     }
   }
@@ -307,8 +314,12 @@ static int launch_append(const sa_paged_append_args& a, cudaStream_t stream) {
   const int64_t q_units = (int64_t)a.batch.N * ((a.Hq + per * kQHeads - 1) / (per * kQHeads));
   const int64_t page_units = (a.batch.N / a.batch.page_size + 2 * (int64_t)a.batch.B) * a.Hkv;
   // 16 tokens a sequence and more: four warps a page (680 tokens of 6 sequences,
-  // pages of 128: 16 us with one).
-  const bool shared = a.batch.N / a.batch.B >= 16;
+  // pages of 128: 16 us with one). So too where bounds are kept of pages that may hold
+  // many keys already, while all of those CTAs are resident at once: one token of 32
+  // sequences, 8 kv heads, pages of 128 with 126 keys 5.6 us, with one warp 8.1; of 128
+  // sequences 12.7 and 13.4, but 9.2 and 5.5 where the pages are new.
+  const bool shared = a.batch.N / a.batch.B >= 16 ||
+                      (a.bounds && a.batch.page_size >= 64 && page_units <= 6 * (int64_t)sa_num_sms());
   const int64_t page_blocks = shared ? page_units : (page_units + kAppendWarps - 1) / kAppendWarps;
   const int64_t blocks = page_blocks + (q_units + kAppendWarps - 1) / kAppendWarps;
   if (q_units > 0x7fffffff || blocks > 0x7fffffff) return sa_fail(SA_ERR_INVALID, "paged append: too many tokens");

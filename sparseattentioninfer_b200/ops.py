@@ -478,7 +478,8 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor | None, 
     throughout). Returns q = RoPE(RMSNorm(q)) [N, Hq, D] (``q_out`` when given);
     a None weight leaves that norm out. ``k_bounds`` [pages, Hkv, 2, D]: lowest
     and highest stored key per channel of each page, kept up to date (what
-    paged_block_select scores). The batch tensors are read on the device, so
+    paged_block_select scores), also where a sequence was cut short before
+    (rejected drafts). The batch tensors are read on the device, so
     the call can be captured; what they must satisfy is stated in
     sparse_attn_b200.h, and a violation sets the device error word."""
     return _paged_result(_PAGED.append(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_table, cu_q, seq_lens,
