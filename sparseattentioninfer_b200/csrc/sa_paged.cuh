@@ -194,7 +194,8 @@ struct PagedAttnParams {
   float* part_o;    // [N, Hq, n_split, D]
   float* part_ml;   // [N, Hq, n_split, 2]
   int32_t* pages;   // chunk kernel with kept pages: each tile's pages [units, Hkv, page_cap],
-  int32_t* n_pages; // and their numbers [units, Hkv]
+  int32_t* n_pages; // and their numbers [units, Hkv],
+  int32_t* list_lens; // and how many entries of each token's list count [N, Hkv]
   int32_t page_cap;
   int32_t* err;
 };

@@ -88,11 +88,20 @@ __global__ void __launch_bounds__(PagedRowCfg<D, ROWS, WIDE>::kThreads) paged_ro
   if constexpr (SPARSE) {
     list = a.blocks + (int64_t)ut.t0 * a.blocks_strides[0] + (int64_t)kvh * a.blocks_strides[1];
     const int per = max(1, a.split_len / kRowKeys);
-    int cnt = 0;
+    // The list ends at its first entry that does not ascend or that the token does not see.
+    int cnt = 0, before = -1;
     for (int i = lane; i - lane < a.n_blocks; i += 32) {
-      const unsigned m = __ballot_sync(0xffffffffu, i < a.n_blocks && __ldg(list + i) >= 0);
-      cnt += m == 0xffffffffu ? 32 : __ffs(~m) - 1;
-      if (m != 0xffffffffu) break;
+      const int e = i < a.n_blocks ? __ldg(list + i) : -1;
+      int prev = __shfl_up_sync(0xffffffffu, e, 1);
+      if (lane == 0) prev = before;
+      const unsigned m = __ballot_sync(0xffffffffu, e > prev && (int64_t)e * ps < keys);
+      const int n = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+      cnt += n;
+      before = __shfl_sync(0xffffffffu, e, n < 32 ? n : 31);
+      if (n < 32) {
+        if (before >= 0 && tid == 0) record_error(p.err, SA_DEV_ERR_INDEX);
+        break;
+      }
     }
     n_list = cnt;
     const int nst = (cnt + pps - 1) >> lpps << lspp;
@@ -158,12 +167,7 @@ __global__ void __launch_bounds__(PagedRowCfg<D, ROWS, WIDE>::kThreads) paged_ro
       page = -1;
       if (i < ne) {
         if constexpr (SPARSE) {
-          const int e = e0 + i;
-          blk = __ldg(list + e);
-          if (blk <= (e > 0 ? __ldg(list + e - 1) : -1) || (int64_t)blk * ps >= keys) {
-            bad = 1;
-            blk = -1;
-          }
+          blk = __ldg(list + e0 + i);
         } else {
           blk = e0 + i;
           if ((int64_t)blk * ps >= keys) blk = -1;
@@ -494,7 +498,9 @@ struct AttnPlan {
   int64_t units;
   int64_t part;      // floats of the split results
   int64_t page_cap;  // entries of a tile's page list; 0: none
-  int64_t workspace(const sa_paged_attn_args& a) const { return part + units * a.Hkv * (page_cap + (page_cap > 0)); }
+  int64_t workspace(const sa_paged_attn_args& a) const {
+    return part + (page_cap > 0 ? (units * (page_cap + 1) + a.batch.N) * a.Hkv : 0);
+  }
 };
 
 // How many clusters of n CTAs, an SM for each CTA, the device holds at once. A cluster
@@ -808,6 +814,7 @@ extern "C" int sa_paged_attn(const sa_paged_attn_args* args, sa_stream_t stream_
   prm.part_ml = a->workspace ? a->workspace + (int64_t)a->batch.N * a->Hq * r.n_split * a->D : nullptr;
   prm.pages = reinterpret_cast<int32_t*>(a->workspace) + r.part;
   prm.n_pages = prm.pages + r.units * a->Hkv * r.page_cap;
+  prm.list_lens = prm.n_pages + r.units * a->Hkv;
   prm.page_cap = (int32_t)r.page_cap;
   prm.err = sa_device_error_ptr();
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream_);

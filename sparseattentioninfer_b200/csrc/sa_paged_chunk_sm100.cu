@@ -66,9 +66,9 @@ struct ChunkCfg {
   static_assert(kVStages < 8, "producer may run a batch ahead");
 };
 
-// The ascending union of the lists of one tile's tokens. Entries behind the first
-// -1 are nobody's; one that does not ascend or that its token does not see is
-// left out here, and with it what its row's walk would not reach.
+// The ascending union of the lists of one tile's tokens, and the length of each list.
+// A list ends at its first -1, and at the first entry that does not ascend or that its
+// token does not see.
 __global__ void __launch_bounds__(256) paged_union_kernel(const __grid_constant__ PagedAttnParams p, int64_t units) {
   extern __shared__ uint32_t bits[];
   __shared__ int s_cnt[8];
@@ -85,23 +85,24 @@ __global__ void __launch_bounds__(256) paged_union_kernel(const __grid_constant_
   bool bad = false;
   for (int t = warp; t < ut.n; t += 8) {
     const int32_t* list = a.blocks + (int64_t)(ut.t0 + t) * a.blocks_strides[0] + (int64_t)kvh * a.blocks_strides[1];
-    const int own = min(ut.pos0 + t, keys - 1) / ps;  // (a negative position sees nothing)
-    int before = -1;
+    const int own = min(ut.pos0 + t, keys - 1) / ps;
+    int before = -1, cnt = 0;
     for (int i0 = 0; i0 < a.n_blocks; i0 += 32) {
       const int i = i0 + lane;
       const int e = i < a.n_blocks ? __ldg(list + i) : -1;
       int prev = __shfl_up_sync(0xffffffffu, e, 1);
       if (lane == 0) prev = before;
-      before = __shfl_sync(0xffffffffu, e, 31);
-      const unsigned end = __ballot_sync(0xffffffffu, e < 0);
-      if (end == 0 || lane < __ffs(end) - 1) {
-        if (e > prev && e <= own && keys > 0)
-          atomicOr(&bits[e >> 5], 1u << (e & 31));
-        else
-          bad = true;
+      const unsigned m = __ballot_sync(0xffffffffu, e > prev && e <= own);
+      const int n = m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+      if (lane < n) atomicOr(&bits[e >> 5], 1u << (e & 31));
+      cnt += n;
+      before = __shfl_sync(0xffffffffu, e, n < 32 ? n : 31);
+      if (n < 32) {
+        bad |= before >= 0;
+        break;
       }
-      if (end) break;
     }
+    if (lane == 0) p.list_lens[(int64_t)(ut.t0 + t) * a.Hkv + kvh] = cnt;
   }
   if (bad) record_error(p.err, SA_DEV_ERR_INDEX);
   __syncthreads();
@@ -434,15 +435,14 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
     constexpr int kNone = 0x7fffffff;
     const int32_t* list = nullptr;
     int ptr = 0, want = kNone, ahead = kNone;
-    auto entry_at = [&](int i) {
-      const int e = i < a.n_blocks ? __ldg(list + i) : -1;
-      return e < 0 ? kNone : e;
-    };
+    int n_list = 0;
+    auto entry_at = [&](int i) { return i < n_list ? __ldg(list + i) : kNone; };
     if constexpr (SPARSE) {
       if (row_ok) {
         list = a.blocks + (int64_t)(ut.t0 + row / G) * a.blocks_strides[0] + (int64_t)kvh * a.blocks_strides[1];
+        n_list = __ldg(p.list_lens + (int64_t)(ut.t0 + row / G) * a.Hkv + kvh);
         const int from = __ldg(union_at + e0);  // first page of this split
-        int hi = c0 > 0 ? a.n_blocks : 0;
+        int hi = c0 > 0 ? n_list : 0;
         while (ptr < hi) {
           const int mid = (ptr + hi) >> 1;
           if (entry_at(mid) < from)
