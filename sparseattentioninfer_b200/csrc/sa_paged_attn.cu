@@ -308,8 +308,9 @@ __global__ void __launch_bounds__(PagedRowCfg<D, ROWS, WIDE>::kThreads) paged_ro
           m_run[r] = m_new;
           // P is rounded to the cache's type for the product; the sum takes the
           // rounded values, so that a row ruled by few keys loses nothing by it.
-          pa[2 * r] = Half<T>::pack(ex2(x[0] - mu), ex2(x[1] - mu));
-          pa[2 * r + 1] = Half<T>::pack(ex2(x[2] - mu), ex2(x[3] - mu));
+          const float base = mu - Half<T>::kLiftRows;
+          pa[2 * r] = Half<T>::pack(ex2(x[0] - base), ex2(x[1] - base));
+          pa[2 * r + 1] = Half<T>::pack(ex2(x[2] - base), ex2(x[3] - base));
           const float2 u = Half<T>::unpack(pa[2 * r]), v = Half<T>::unpack(pa[2 * r + 1]);
           l_run[r] = l_run[r] * alpha[r] + (u.x + u.y) + (v.x + v.y);
         }

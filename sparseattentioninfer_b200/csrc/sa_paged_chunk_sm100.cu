@@ -16,6 +16,8 @@
 //   warps 2-5  softmax, one thread a row: running maximum and sum in registers, P
 //              (16 bits) written over S, O rescaled in TMEM only when the maximum
 //              grew by more than 2^8 (the same stale maximum serves P, sum and O).
+//              The sum takes the weights before they are rounded: a row that one key
+//              rules is off by that weight's rounding, which by rows it is not.
 // Slots behind the last key may hold anything: S there is masked, and V's rows
 // are set to zero in shared memory by the softmax warps before P is handed over.
 // Unsplit tiles write out = O / l; split ones their O, maximum and sum.
@@ -568,7 +570,8 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         }
         if (need || m_ref == -INFINITY) m_ref = m_new;
         const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
-        const uint64_t sc2 = f2pack(p.scale_log2, p.scale_log2), nm2 = f2pack(-m_use, -m_use);
+        const float nm = Half<T>::kLiftTiles - m_use;
+        const uint64_t sc2 = f2pack(p.scale_log2, p.scale_log2), nm2 = f2pack(nm, nm);
         uint64_t rs4[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
