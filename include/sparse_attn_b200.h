@@ -425,8 +425,9 @@ SA_API int sa_paged_attn(const sa_paged_attn_args* args, sa_stream_t stream);
  * first `first`, the last `recent` (>= 1) and the best others by
  *   s = sum_{g in the kv head's group} sum_d max(q_gd * low_d, q_gd * high_d),
  * low/high the page's bounds: s bounds the group's summed scores q_g . k from
- * above for every key of the page. Equal scores go to the lower index, NaN counts
- * as -infinity. Order is that of the scores in 64 bits.
+ * above for every key of the page. 0 times an infinite bound counts as 0, a score
+ * that is no number as -infinity. Equal scores go to the lower index. Order is that
+ * of the scores in 64 bits.
  * out [N, Hkv, keep] (strides token, head): ascending logical page indexes, -1
  * behind the last. first + recent <= keep <= 4096, max_pages <= 16384. */
 typedef struct sa_paged_select_args {

@@ -72,12 +72,13 @@ __device__ __forceinline__ double page_score(const T* low, int64_t to_high, cons
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
   if (s != s) {
-    // An infinite bound met a factor of 0, which leaves it out of the maximum.
+    // An infinite bound may have met a factor of 0, which leaves it out of the maximum.
     s = 0.;
     for (int e = 0; e < E; ++e) {
       const int d = lane * E + e;
-      if (q[d] != 0.) s = fma(q[d], (double)Half<T>::to(low[d]), s);
-      if (q[D + d] != 0.) s = fma(q[D + d], (double)Half<T>::to(low[to_high + d]), s);
+      const double lo = (double)Half<T>::to(low[d]), hi = (double)Half<T>::to(low[to_high + d]);
+      if (q[d] != 0. || lo != lo) s = fma(q[d], lo, s);
+      if (q[D + d] != 0. || hi != hi) s = fma(q[D + d], hi, s);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);

@@ -1,5 +1,7 @@
-"""Page selection where scores cancel."""
+"""Page selection where scores cancel or bounds are not finite."""
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -42,3 +44,39 @@ def test_scores_that_cancel(new, pages, dtype, D, signs):
     bounds[bt.table[0].long()] = rows.to(dtype)[:, None, None].expand(-1, 1, 2, -1)
     for keep, first, recent in ((9, 1, 2), (12, 0, 1), (4, 1, 1)):
         _check(bt, q, bounds, keep, first, recent, max_q=new)
+
+
+@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("side", [0, 1])
+def test_a_bound_that_is_no_number_ranks_its_page_lowest(new, side):
+    """A NaN in either bound, whatever the sign of the heads' values in that channel."""
+    bt = P.Batch([50 * 16], [new], Hq=2, Hkv=1, D=64, page=16, device=DEV)
+    q = torch.randn(new, 2, 64, generator=bt.g).to(torch.bfloat16)
+    q[:, :, 7] = -q[:, :, 7].abs() - 0.5
+    q[:, :, 9] = q[:, :, 9].abs() + 0.5
+    bounds = torch.ones(bt.pages, 1, 2, 64, dtype=torch.bfloat16)
+    bounds[bt.table[0, 5:20].long(), 0, side, 7] = math.nan
+    bounds[bt.table[0, 20:30].long(), 0, side, 9] = math.nan
+    _check(bt, q, bounds, 30, 1, 1, max_q=new)
+
+
+@pytest.mark.parametrize("new", [1, 5])
+def test_zero_times_an_infinite_bound_is_zero(new):
+    """Heads whose value in the channel is 0 take nothing from it, others do."""
+    bt = P.Batch([50 * 16], [new], Hq=3, Hkv=1, D=64, page=16, device=DEV)
+    q = torch.randn(new, 3, 64, generator=bt.g).to(torch.bfloat16)
+    q[:, :, 7] = 0
+    q[:, 0, 9] = 0
+    q[:, 1:, 9] = -1
+    bounds = torch.ones(bt.pages, 1, 2, 64, dtype=torch.bfloat16)
+    low = torch.randn(bt.pages, 64, generator=bt.g)
+    bounds[:, 0, 0], bounds[:, 0, 1] = low.to(torch.bfloat16), (low + 1).to(torch.bfloat16)
+    plain = bounds.clone()
+    some = bt.table[0, 5:30].long()
+    bounds[some, 0, 0, 7], bounds[some, 0, 1, 7] = -math.inf, math.inf
+    bounds[some, 0, 1, 9] = math.inf  # (the heads of -1 take the low one)
+    plain[some, 0, :, 7] = 0
+    plain[some, 0, 1, 9] = plain[some, 0, 0, 9]
+    got = ops.paged_block_select(q.to(DEV), bounds.to(DEV), *bt.batch, page_size=16, keep=12, max_q=new)
+    assert torch.equal(got.cpu(), P.select(bt, q, plain, 12, 1, 1))
+    assert _capi.device_error() == 0
