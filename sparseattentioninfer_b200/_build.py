@@ -1,13 +1,15 @@
 """Build the in-tree C-ABI library ``_lib/libsa_b200.so`` with nvcc for sm_100a, and
-``_lib/_sa_paged.so``, the compiled Python binding of the paged-cache operators.
+``_lib/_sa_paged-*.so``, the compiled Python binding of the paged-cache operators.
 
 The library is plain CUDA C++ (no torch headers), so it builds without a GPU and
 loads in any process through ctypes; the binding is host C++ against the headers
-of the installed torch. Run ``python sparseattentioninfer_b200/_build.py`` (as a file: importing the
-package itself requires the built library).
+of the installed torch and Python, whose versions its file name carries. Run
+``python sparseattentioninfer_b200/_build.py`` (as a file: importing the package
+itself requires the built library).
 """
 from __future__ import annotations
 
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -22,7 +24,6 @@ LIB_DIR = PKG / "_lib"
 LIB_PATH = LIB_DIR / "libsa_b200.so"
 INCLUDE = PKG.parent / "include"
 BINDING_SRC = CSRC / "paged_binding.cpp"
-BINDING_PATH = LIB_DIR / "_sa_paged.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 BASE_FLAGS = [
@@ -50,7 +51,12 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 
 
 def needs_build() -> bool:
-    return _stale(LIB_PATH, _deps()) or _stale(BINDING_PATH, _binding_deps())
+    return _stale(LIB_PATH, _deps()) or _stale(binding_path(), _binding_deps())
+
+
+def binding_path() -> Path:
+    """Where the binding for this Python and the installed torch is."""
+    return LIB_DIR / f"_sa_paged-{sysconfig.get_config_var('SOABI')}-torch{importlib.metadata.version('torch')}.so"
 
 
 def _binding_deps() -> list[Path]:
@@ -64,7 +70,8 @@ def build_binding(verbose: bool = False) -> Path:
         raise RuntimeError("torch not found; the paged-cache binding cannot be built")
     torch = Path(spec.origin).parent
     cuda = Path(nvcc_path()).resolve().parent.parent
-    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    path = binding_path()
+    tmp = path.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", sysconfig.get_paths()["include"], "-isystem", str(torch / "include"),
            "-isystem", str(torch / "include/torch/csrc/api/include"), "-isystem", str(cuda / "include"),
@@ -73,8 +80,8 @@ def build_binding(verbose: bool = False) -> Path:
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)
-    os.replace(tmp, BINDING_PATH)
-    return BINDING_PATH
+    os.replace(tmp, path)
+    return path
 
 
 def nvcc_path() -> str:
@@ -85,13 +92,18 @@ def nvcc_path() -> str:
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
-    """Compile every ``csrc/*.cu`` into ``_lib/libsa_b200.so``, and the binding
+    """Compile every ``csrc/*.cu`` into ``_lib/libsa_b200.so``, then the binding
     (each skipped when up to date)."""
     LIB_DIR.mkdir(exist_ok=True)
-    if force or _stale(BINDING_PATH, _binding_deps()):
+    if force or _stale(LIB_PATH, _deps()):
+        build_library(verbose, extra_flags)
+    if force or _stale(binding_path(), _binding_deps()):
         build_binding(verbose)
-    if not force and not _stale(LIB_PATH, _deps()):
-        return LIB_PATH
+    return LIB_PATH
+
+
+def build_library(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
+    """Compile and link ``_lib/libsa_b200.so``."""
     nvcc = nvcc_path()
     objs = []
     build_dir = LIB_DIR / "obj"

@@ -10,9 +10,10 @@ import importlib.util
 import os
 from pathlib import Path
 
+from ._build import binding_path
+
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "_lib" / "libsa_b200.so"
-BINDING_PATH = _PKG / "_lib" / "_sa_paged.so"
 
 # Every symbol include/sparse_attn_b200.h declares (checked by the CPU tests).
 EXPORTED = (
@@ -202,14 +203,16 @@ _binding = None
 
 def paged_binding():
     """The compiled Python calls of the paged-cache operators (csrc/paged_binding.cpp),
-    loaded once and bound to the loaded library. torch must be imported."""
+    loaded by the first of them and bound to the loaded library: nothing else needs
+    them. torch must be imported."""
     global _binding
     if _binding is None:
-        if not BINDING_PATH.exists():
+        path = binding_path()
+        if not path.exists():
             raise ImportError(
-                f"sparseattentioninfer_b200 binding not found at {BINDING_PATH}; build it with "
+                f"sparseattentioninfer_b200 binding for this Python and torch not found at {path}; build it with "
                 "`python sparseattentioninfer_b200/_build.py`")
-        spec = importlib.util.spec_from_file_location("_sa_paged", BINDING_PATH)
+        spec = importlib.util.spec_from_file_location("_sa_paged", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         lib = load()

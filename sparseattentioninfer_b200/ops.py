@@ -451,7 +451,6 @@ def topk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: int
 # ---------------------------------------------------------------------------
 # (The checks of these calls are compiled, csrc/paged_binding.cpp: a decode step's
 # kernels are shorter than the same checks in Python.)
-_PAGED = _capi.paged_binding()
 
 
 def _paged_result(r):
@@ -482,8 +481,8 @@ def paged_qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor | None, 
     (rejected drafts). The batch tensors are read on the device, so
     the call can be captured; what they must satisfy is stated in
     sparse_attn_b200.h, and a violation sets the device error word."""
-    return _paged_result(_PAGED.append(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_table, cu_q, seq_lens,
-                                       Hq, Hkv, eps, k_bounds, q_out))
+    return _paged_result(_capi.paged_binding().append(qkv, q_weight, k_weight, cos, sin, k_pages, v_pages, page_table,
+                                                      cu_q, seq_lens, Hq, Hkv, eps, k_bounds, q_out))
 
 
 def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, page_table: torch.Tensor, cu_q: torch.Tensor,
@@ -499,8 +498,8 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, page_table: torc
     the lower index; scores are compared in 64 bits. q [N, Hq, D] and the batch
     tensors as in paged_qk_norm_rope_append; ``max_q`` (most new tokens of one
     sequence) only steers the launch."""
-    return _paged_result(_PAGED.select(q, k_bounds, page_table, cu_q, seq_lens, page_size, keep, first, recent, max_q,
-                                       out))
+    return _paged_result(_capi.paged_binding().select(q, k_bounds, page_table, cu_q, seq_lens, page_size, keep, first,
+                                                      recent, max_q, out))
 
 
 def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -508,7 +507,8 @@ def paged_attention_workspace(q: torch.Tensor, k_pages: torch.Tensor, v_pages: t
                               max_q: int | None = None, max_len: int | None = None,
                               blocks: torch.Tensor | None = None, split_len: int | None = None) -> int:
     """float32 elements of workspace that paged_attention with these arguments needs."""
-    n = _PAGED.workspace(q, k_pages, v_pages, page_table, cu_q, seq_lens, max_q, max_len, blocks, None, split_len, None)
+    n = _capi.paged_binding().workspace(q, k_pages, v_pages, page_table, cu_q, seq_lens, max_q, max_len, blocks, None,
+                                        split_len, None)
     if n < 0:
         _capi.check(n)
     return n
@@ -531,8 +531,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     their defaults are N and the page table's width. ``workspace``: 16-byte
     aligned float32 buffer of at least paged_attention_workspace(...) elements
     that a captured call keeps to itself (allocated per call when None)."""
-    return _paged_result(_PAGED.attention(q, k_pages, v_pages, page_table, cu_q, seq_lens, max_q, max_len, blocks, scale,
-                                          split_len, out, workspace))
+    return _paged_result(_capi.paged_binding().attention(q, k_pages, v_pages, page_table, cu_q, seq_lens, max_q,
+                                                         max_len, blocks, scale, split_len, out, workspace))
 
 
 def sparse_attn(q, k, v, block_pairs, block_pair_offsets, block_size: int, *, scale: float | None = None):
