@@ -236,9 +236,10 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 6)
   };
   // The keys that stay, before the page's first new one, are read again: the old bounds may
   // still be of keys that the sequence has taken back (rejected drafts).
+  // Where warps share the page the last ones begin: the first has the first new keys.
   constexpr int S = 8;  // rows in flight, each half warp its own
-  const int stay = bd ? p0 & (ps - 1) : 0;
-  for (int p = (shared ? warp * 2 * S : 0) + half; p - half < stay; p += 2 * S * (shared ? kAppendWarps : 1)) {
+  const int stay = bd ? p0 & (ps - 1) : 0, turn_s = 2 * S * (shared ? kAppendWarps : 1);
+  for (int p = (shared ? (kAppendWarps - 1 - warp) * 2 * S : 0) + half; p - half < stay; p += turn_s) {
     Raw<H> k[S];
 #pragma unroll
     for (int i = 0; i < S; ++i) k[i].load(kd + (int64_t)min(p + 2 * i, stay - 1) * a.k_strides[2]);
