@@ -496,7 +496,8 @@ __global__ void __launch_bounds__(kSelThreads, 3)
 template <typename T, int D>
 static int launch_select(const sa_paged_select_args& a, cudaStream_t stream) {
   using Cfg = SelectCfg<T, D>;
-  // Tokens per CTA: the keys of all of them within 64 KB, so that three CTAs fit on an SM.
+  // Tokens per CTA: the keys of all of them within 64 KB, so that with Q's 30 KB (heads of
+  // 64: 16) two CTAs fit on an SM, three up to some 680 pages at 8 tokens (900).
   int tq = a.max_q < kSelTokens ? a.max_q : kSelTokens;
   if ((int64_t)tq * a.batch.max_pages * 8 > 65536) tq = 65536 / (a.batch.max_pages * 8);
   if (tq < 1) tq = 1;

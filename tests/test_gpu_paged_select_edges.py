@@ -1,4 +1,4 @@
-"""Page selection where scores cancel or bounds are not finite."""
+"""Page selection where scores cancel, bounds are not finite and tables are long."""
 from __future__ import annotations
 
 import math
@@ -80,3 +80,16 @@ def test_zero_times_an_infinite_bound_is_zero(new):
     got = ops.paged_block_select(q.to(DEV), bounds.to(DEV), *bt.batch, page_size=16, keep=12, max_q=new)
     assert torch.equal(got.cpu(), P.select(bt, q, plain, 12, 1, 1))
     assert _capi.device_error() == 0
+
+
+@pytest.mark.parametrize("pages,Hkv", [(5000, 2), (16384, 1)])
+@pytest.mark.parametrize("spread", [1.0, 0.0])
+def test_long_tables(pages, Hkv, spread):
+    """One token over more pages than a CTA's registers hold, up to the longest table;
+    with all pages equal, too."""
+    bt = P.Batch([pages * 16 - 3, 40], [1, 1], Hq=3 * Hkv, Hkv=Hkv, D=64, page=16, device=DEV)
+    q = torch.randn(2, 3 * Hkv, 64, generator=bt.g).to(torch.bfloat16)
+    low = torch.randn(bt.pages, Hkv, 64, generator=bt.g) * spread
+    bounds = torch.stack([low - 1, low + 1], 2).to(torch.bfloat16)
+    _check(bt, q, bounds, 64, 1, 2, max_q=1)
+    _check(bt, q, bounds, 4096, 0, 1, max_q=1)
