@@ -599,7 +599,7 @@ static AttnPlan attn_plan(const sa_paged_attn_args& a, int sms) {
   const int64_t slots = (r.chunk || a.D == 128 ? 2ll : 4ll) * sms;  // resident CTAs
   // Units with tokens (others that are launched leave at once): known where every
   // sequence brings max_q, else as if a sequence's last unit were half full.
-  const int64_t even = (int64_t)a.batch.B * ((a.max_q + r.tq - 1) / r.tq);
+  const int64_t even = (int64_t)a.batch.B * (((int64_t)a.max_q + r.tq - 1) / r.tq);
   const double guess = ceil((double)a.batch.N / r.tq + a.batch.B * (r.tq - 1.) / (2. * r.tq));
   const double likely = r.tq == 1 ? r.units : (int64_t)a.batch.B * a.max_q == a.batch.N ? even : fmax(guess, some);
   auto fits = [&](int64_t n) { return n <= 8 && likely * a.Hkv * r.nhg <= clusters_at_once((int)n, sms); };

@@ -24,3 +24,17 @@ def test_a_workspace_that_is_not_aligned_is_refused(blocks, off):
     a.workspace = FAKE + off
     assert lib.sa_paged_attn(ctypes.byref(a), None) == _capi.SA_ERR_INVALID
     assert b"aligned" in lib.sa_last_error()
+
+
+@pytest.mark.parametrize("blocks", [None, FAKE])
+@pytest.mark.parametrize("split_len", [0, 64])
+def test_hints_up_to_the_largest_int(blocks, split_len):
+    """max_q steers by what it says of the batch, which has no more tokens than N."""
+    n = ctypes.c_int64(-1)
+    need = []
+    for max_q in (500, 2 ** 31 - 1):
+        a = _attn(batch=dict(N=500, B=1), max_q=max_q, split_len=split_len, blocks=blocks, n_blocks=40)
+        a.blocks_strides[0], a.blocks_strides[1] = 80, 40
+        assert _capi.load().sa_paged_attn_workspace(ctypes.byref(a), ctypes.byref(n)) == 0
+        need.append(n.value)
+    assert need[0] == need[1]
