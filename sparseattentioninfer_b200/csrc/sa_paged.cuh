@@ -139,7 +139,7 @@ template <typename T>
 struct Half;
 template <>
 struct Half<__nv_bfloat16> {
-  static constexpr float kLiftRows = 0.f, kLiftTiles = 0.f;
+  static constexpr int kLiftRows = 0, kLiftTiles = 0;
   __device__ static __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
   __device__ static __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16_rn(x); }
   __device__ static __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
@@ -153,7 +153,7 @@ struct Half<__nv_bfloat16> {
 };
 template <>
 struct Half<__half> {
-  static constexpr float kLiftRows = 15.f, kLiftTiles = 7.f;
+  static constexpr int kLiftRows = 15, kLiftTiles = 7;
   __device__ static __forceinline__ float to(__half x) { return __half2float(x); }
   __device__ static __forceinline__ __half from(float x) { return __float2half_rn(x); }
   __device__ static __forceinline__ uint32_t pack(float lo, float hi) {

@@ -308,9 +308,14 @@ __global__ void __launch_bounds__(PagedRowCfg<D, ROWS, WIDE>::kThreads) paged_ro
           m_run[r] = m_new;
           // P is rounded to the cache's type for the product; the sum takes the
           // rounded values, so that a row ruled by few keys loses nothing by it.
-          const float base = mu - Half<T>::kLiftRows;
-          pa[2 * r] = Half<T>::pack(ex2(x[0] - base), ex2(x[1] - base));
-          pa[2 * r + 1] = Half<T>::pack(ex2(x[2] - base), ex2(x[3] - base));
+          // (x - mu is at most 0 whatever their size, so the lift comes behind it)
+          auto weight = [&](float x) {
+            x -= mu;
+            if constexpr (Half<T>::kLiftRows != 0) x += Half<T>::kLiftRows;
+            return ex2(x);
+          };
+          pa[2 * r] = Half<T>::pack(weight(x[0]), weight(x[1]));
+          pa[2 * r + 1] = Half<T>::pack(weight(x[2]), weight(x[3]));
           const float2 u = Half<T>::unpack(pa[2 * r]), v = Half<T>::unpack(pa[2 * r + 1]);
           l_run[r] = l_run[r] * alpha[r] + (u.x + u.y) + (v.x + v.y);
         }

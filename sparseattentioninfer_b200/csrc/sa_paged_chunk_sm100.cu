@@ -548,30 +548,45 @@ __global__ void __launch_bounds__(kChThreads, 2) paged_chunk_kernel(const __grid
         if (SPARSE && drop) mraw = -INFINITY;
         const float m_new = fmaxf(m_ref, mraw * p.scale_log2);
         // (a row that has seen no key yet has nothing in O to rescale)
-        const bool need = m_ref > -INFINITY && m_new > m_ref + 8.0f;
-        if (__any_sync(FULL, need)) {
-          // O still takes the previous chunk's PV: wait for it, then rescale.
-          ok = mbar_wait(smem_u32(&bar_v_empty[(g - 1) % NSV]), ((g - 1) / NSV) & 1, abort_v, p.err);
-          if (!__all_sync(FULL, ok)) { ok = false; break; }
-          tc_fence_after();
-          const float alpha = need ? ex2(m_ref - m_new) : 1.0f;
+        const bool need = m_ref > -INFINITY && m_new - m_ref > 8.0f;
+        // Past 24 bits fma(s, scale, -m) is above that 8 by as much as m was rounded by, for
+        // which the range of fp16 has no room.
+        constexpr bool kNarrow = Half<T>::kLiftTiles != 0;
+        const bool far = kNarrow && fabsf(m_new) >= 1048576.f && m_new > -INFINITY;
+        bool any_far = false;
+        if (__any_sync(FULL, need || far)) {
+          any_far = kNarrow && __any_sync(FULL, far);
+          if (!kNarrow || __any_sync(FULL, need)) {
+            // O still takes the previous chunk's PV: wait for it, then rescale.
+            ok = mbar_wait(smem_u32(&bar_v_empty[(g - 1) % NSV]), ((g - 1) / NSV) & 1, abort_v, p.err);
+            if (!__all_sync(FULL, ok)) { ok = false; break; }
+            tc_fence_after();
+            const float alpha = need ? ex2(m_ref - m_new) : 1.0f;
 #pragma unroll
-          for (int cc = 0; cc < D / 32; ++cc) {
-            uint32_t o32[32];
-            tmem_ld32(tmem + lane_base + cc * 32, o32);
-            tmem_wait_ld();
-            reg_fence32(o32);
+            for (int cc = 0; cc < D / 32; ++cc) {
+              uint32_t o32[32];
+              tmem_ld32(tmem + lane_base + cc * 32, o32);
+              tmem_wait_ld();
+              reg_fence32(o32);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o32[i] = __float_as_uint(__uint_as_float(o32[i]) * alpha);
-            tmem_st32(tmem + lane_base + cc * 32, o32);
+              for (int i = 0; i < 32; ++i) o32[i] = __float_as_uint(__uint_as_float(o32[i]) * alpha);
+              tmem_st32(tmem + lane_base + cc * 32, o32);
+            }
+            tmem_wait_st();
+            if (need) l *= alpha;
           }
-          tmem_wait_st();
-          if (need) l *= alpha;
         }
         if (need || m_ref == -INFINITY) m_ref = m_new;
         const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
-        const float nm = Half<T>::kLiftTiles - m_use;
-        const uint64_t sc2 = f2pack(p.scale_log2, p.scale_log2), nm2 = f2pack(nm, nm);
+        float sc = p.scale_log2, nm = Half<T>::kLiftTiles - m_use;
+        if (any_far) {
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            s[i] = far ? __fsub_rn(__fmul_rn(s[i], sc), m_use) : fmaf(s[i], sc, -m_use);
+          sc = 1.f;
+          nm = Half<T>::kLiftTiles;
+        }
+        const uint64_t sc2 = f2pack(sc, sc), nm2 = f2pack(nm, nm);
         uint64_t rs4[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
