@@ -274,8 +274,8 @@ bool attn_args(Call& c, PyObject* const* o, sa_paged_attn_args& a, Tensor* out) 
     a.out = out->data_ptr();
   } else {
     a.out = q.data_ptr();
-    a.o_strides[0] = a.q_strides[0];
-    a.o_strides[1] = a.q_strides[1];
+    a.o_strides[0] = q.size(1) * D;
+    a.o_strides[1] = D;
   }
   const bool rows = c.batch(a.batch, N, o[3], o[4], o[5], k.size(0), k.size(2));
   a.max_q = o[6] == Py_None ? a.batch.N : c.int32(o[6], "max_q");

@@ -393,9 +393,10 @@ extern "C" int sa_paged_append(const sa_paged_append_args* args, sa_stream_t str
   const void* al[6] = {a->qkv, a->q_weight, a->k_weight, a->cos, a->sin, a->q_out};
   for (int i = 0; i < 6; ++i)
     if (reinterpret_cast<uintptr_t>(al[i]) & 7u) return sa_fail(SA_ERR_INVALID, "tensors must be 8-byte aligned");
-  if (a->qkv_st % 4 || a->q_strides[0] % 4 || a->q_strides[1] % 4 || a->qkv_st < 0 || a->q_strides[0] < 0 ||
-      a->q_strides[1] < 0)
-    return sa_fail(SA_ERR_INVALID, "strides must be non-negative multiples of 4 elements");
+  if (a->qkv_st % 4 || a->qkv_st < 0) return sa_fail(SA_ERR_INVALID, "qkv: bad token stride");
+  for (int i = 0; i < 2; ++i)
+    if (a->q_strides[i] % 4 || a->q_strides[i] < a->D)  // (rows that share memory would be written at once)
+      return sa_fail(SA_ERR_INVALID, "q_out: strides must be multiples of 4 elements, at least D");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream_);
   if (a->dtype == SA_BF16)
     return a->D == 128 ? launch_append<__nv_bfloat16, 4>(*a, st) : launch_append<__nv_bfloat16, 2>(*a, st);

@@ -764,6 +764,8 @@ static int check_paged_attn(sa_paged_attn_args* a) {
   for (int i = 0; i < 2; ++i)
     if (st[i][0] <= 0 || st[i][1] <= 0 || st[i][0] % 8 || st[i][1] % 8 || (st[i][0] | st[i][1]) >= (1ll << 36))
       return sa_fail(SA_ERR_INVALID, "q/out strides must be positive multiples of 8 elements (16 B) below 2^36");
+  if (a->o_strides[0] < a->D || a->o_strides[1] < a->D)
+    return sa_fail(SA_ERR_INVALID, "out: strides must be at least D");
   if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) & 15u)
     return sa_fail(SA_ERR_INVALID, "q/out must be 16-byte aligned");
   if (a->blocks) {
