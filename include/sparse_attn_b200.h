@@ -387,9 +387,12 @@ SA_API int sa_paged_append(const sa_paged_append_args* args, sa_stream_t stream)
  * kv head h / (Hq / Hkv). With blocks [N, Hkv, n_blocks] (logical page indexes,
  * strictly ascending, -1 behind the last) token t of a kv head sees only the
  * listed pages; an index that does not ascend or lies behind the token sets
- * SA_DEV_ERR_INDEX and ends its list. A row that sees no key is 0. Slots past a sequence's length are never used, whatever they hold; V
- * of the keys of a sequence has to be finite for those of its new tokens that do
- * not see them and share a tile with one that does (0 times infinity is NaN).
+ * SA_DEV_ERR_INDEX and ends its list. A row that sees no key is 0. Weights are
+ * rounded to the type for the product with V, everything else is in 32 bits.
+ * Slots past a sequence's length are never used, whatever they hold; V of the keys
+ * of a sequence has to be finite for those of its new tokens that do not see them
+ * (keys behind them, and pages that they do not keep) and share a tile with one
+ * that does (0 times infinity is NaN).
  * max_q (most new tokens of one sequence) and max_len (most keys) only steer the
  * choice of kernel and the split of long sequences: any value >= 1 is correct
  * for max_q; max_len must not be exceeded (SA_DEV_ERR_INDEX, keys cut).

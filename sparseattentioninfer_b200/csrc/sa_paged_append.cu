@@ -12,10 +12,12 @@
 // the page's bounds are the minimum and maximum of one warp: no atomics, and the
 // same bounds however the tokens were cut into calls (where sequences bring many
 // tokens the CTA's warps share a page). Keys that the page holds already are read
-// again for that: a sequence may have taken some back since the bounds were written;
-// q warps take up to kQHeads heads at once of one token, whose cos/sin row stays in registers.
-// 10,819 tokens, 32/8 heads of 128: 52 us, 5.2 TB/s; six CTAs a SM with two pairs of
-// tokens in flight (eight: 59 us, and spills; five: 55; four with four pairs: 57).
+// again for that: a sequence may have taken some back since the bounds were written.
+// q warps take up to kQHeads heads at once of one token, whose cos/sin row stays in
+// registers.
+// 10,819 tokens, 32/8 heads of 128: 54 us, 5.1 TB/s (before the older keys were read
+// again 52); six CTAs a SM with two pairs of tokens in flight (eight: 59 us, and
+// spills; five: 55; four with four pairs: 57).
 #include "sa_paged.cuh"
 
 namespace sa {

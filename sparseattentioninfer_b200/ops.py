@@ -497,7 +497,7 @@ def paged_block_select(q: torch.Tensor, k_bounds: torch.Tensor, page_table: torc
     above of the summed scores of every key in the page. Equal scores go to
     the lower index; scores are compared in 64 bits. q [N, Hq, D] and the batch
     tensors as in paged_qk_norm_rope_append; ``max_q`` (most new tokens of one
-    sequence) only steers the launch."""
+    sequence, N by default: give it in decode) only steers the launch."""
     return _paged_result(_capi.paged_binding().select(q, k_bounds, page_table, cu_q, seq_lens, page_size, keep, first,
                                                       recent, max_q, out))
 
@@ -525,10 +525,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     paged_qk_norm_rope_append, which has written them). One call serves single
     tokens, drafts, chunks of prompts and whole prompts side by side.
 
-    ``blocks`` [N, Hkv, n] int32 (paged_block_select's result): the token sees
-    only these pages. ``max_q`` (most new tokens of one sequence) and ``max_len``
-    (most keys of one sequence; must not be exceeded) only steer the launch;
-    their defaults are N and the page table's width. ``workspace``: 16-byte
+    ``blocks`` [N, Hkv, n] int32, n >= 1 (paged_block_select's result): the token
+    sees only these pages, up to the list's first -1 (or, reported, its first entry
+    that does not ascend or that the token does not see). V of keys that a token
+    does not see has to be finite where it shares a tile with one that does.
+    ``max_q`` (most new tokens of one sequence) and ``max_len`` (most keys of one
+    sequence; must not be exceeded) only steer the launch; their defaults are N and
+    the page table's width: give max_q in decode. ``workspace``: 16-byte
     aligned float32 buffer of at least paged_attention_workspace(...) elements
     that a captured call keeps to itself (allocated per call when None)."""
     return _paged_result(_capi.paged_binding().attention(q, k_pages, v_pages, page_table, cu_q, seq_lens, max_q,
